@@ -160,6 +160,104 @@ int qi_lm_head_argmax(const float* x, long long x_stride, const float* norm_w, f
 int qi_move_rows(uint16_t* k, uint16_t* v, int layers, int cache_rows, int max_len,
                  const int32_t* moves, int n_moves, qi_stream_t stream);
 
+/* ------------------------------------- cache layers: 8-bit append, attention */
+
+/* Element types of activations. */
+#define QI_F32 0
+#define QI_BF16 1
+#define QI_F16 2
+
+/* What a cache layer holds. */
+#define QI_KV_BF16 0 /* bf16 values                                              */
+#define QI_KV_INT8 1 /* int8 codes c, value c * scale                            */
+#define QI_KV_E4M3 2 /* 8-bit floats (4 exponent, 3 mantissa bits) times scale   */
+
+/* One layer of a KV cache. Unlike the model's own entry points above, the layer's calls
+ * below take any number of KV heads with head_dim 64 or 128. k and v are 16-byte aligned.
+ * The 8-bit formats keep one fp32 scale, a power of two, per block of `block` positions
+ * (16, 32, 64 or 128) of one cache row and head. No reference counterpart: the reference's
+ * cache (qweninfer/engine/kv_cache.py:24-46) has one dtype and no scales. */
+typedef struct {
+  void* k;                  /* (cache_rows, kv_heads, max_len, head_dim), or paged   */
+  void* v;
+  float* k_scale;           /* (cache_rows, kv_heads, ceil(max_len / block)), or     */
+  float* v_scale;           /* paged (n_pages, kv_heads, page_size / block)          */
+  int format;               /* QI_KV_*                                               */
+  int block;
+  int cache_rows;
+  int kv_heads;
+  int max_len;
+  int head_dim;
+  const int32_t* page_table; /* paged as in qi_cache, else NULL: k and v are pools    */
+  int page_size;             /* (n_pages, kv_heads, page_size, head_dim)              */
+  int pages_per_row;
+  int n_pages;
+} qi_kv_layer;
+
+/* Append M tokens to an 8-bit layer: token t's keys k[t, head, :] and values go to position
+ * pos[t] of cache row rows[t]. k and v: dtype QI_F32/BF16/F16, element strides of token and
+ * head as given, dims contiguous. pos[t] = -1 skips the token. A block's scale is the least
+ * power of two s with top * s >= |x| for every value x it has taken (top 127 for int8, 448
+ * for e4m3) and x is held as the code nearest to x / s, ties to even (of the codes whose
+ * value is finite in fp32). The positions of a
+ * block before the first appended one are kept: where the scale grows, their codes are
+ * rounded again. Positions after the last appended one of its block are dead, and a block
+ * whose first position is appended starts over. The result does not depend on the order of
+ * the tokens in the call; of two tokens with the same row and position the later one is
+ * kept. A value that is not finite makes its block's scale NaN. A position or row outside
+ * the cache sets *err to QI_ERR_INDEX and is skipped. */
+int qi_kv8_append(const qi_kv_layer* layer, const void* k, long long k_token_stride, long long k_head_stride,
+                  const void* v, long long v_token_stride, long long v_head_stride, int dtype, const int32_t* rows,
+                  const int32_t* pos, int M, int* err, qi_stream_t stream);
+
+/* The fp32 values of an 8-bit layer: k_out, v_out (cache_rows, kv_heads, max_len, head_dim),
+ * 16-byte aligned. Positions on unmapped pages give zeros. */
+int qi_kv8_values(const qi_kv_layer* layer, float* k_out, float* v_out, qi_stream_t stream);
+
+/* Attention of M query tokens over one cache layer of any format:
+ *   out[t, h] = softmax over the seen keys j of (q[t, h] . k_j / sqrt(head_dim)) @ v
+ * Token t at position pos[t] of cache row rows[t] sees key j if 0 <= j <= pos[t] and
+ * (window == 0 or j > pos[t] - window or j < sinks): a sliding window of `window` keys, its
+ * own among them, and the row's first `sinks` keys. pos[t] = -1 (an idle slot) sees
+ * nothing: its output is zero. Keys that are not seen are not read. q: dtype QI_F32/BF16/
+ * F16, element strides of token and head, dims contiguous; heads = group * kv_heads, group
+ * 1..8. out: (M, heads, head_dim) of the same dtype, must not overlap q. query_run: longest
+ * run of consecutive tokens of one cache row (a prompt's length), 1 for a decode step, 0 if
+ * unknown; it picks the kernel, any value gives the same result up to rounding.
+ * part: scratch of part_floats floats; counters: counters_len uint32, zero before the first
+ * call and left zero. qi_cache_attention_scratch gives the sizes that use the whole GPU;
+ * with less, the keys are split less. A position (other than -1) or row outside the cache
+ * and an unmapped page set *err to QI_ERR_INDEX; the token's output is zero, or the page's
+ * keys count as zeros. Replaces the attention core of qweninfer/models/qwen2.py:184-199,
+ * which has no window. */
+int qi_cache_attention(const qi_kv_layer* layer, const void* q, long long q_token_stride, long long q_head_stride,
+                       int dtype, int heads, const int32_t* rows, const int32_t* pos, int M, int window, int sinks,
+                       int query_run, void* out, float* part, long long part_floats, unsigned int* counters,
+                       long long counters_len, int* err, qi_stream_t stream);
+
+/* Scratch of a qi_cache_attention call of M tokens: floats of `part` and length of
+ * `counters` (either 0 when none is used). Returns 0 or QI_ERR_ARG. */
+int qi_cache_attention_scratch(const qi_kv_layer* layer, int heads, int M, int window, int sinks, int query_run,
+                               long long* part_floats, long long* counters_len);
+
+/* ----------------------------------------------------- token log probabilities */
+
+/* For each of M rows of logits (V values of dtype QI_F32/BF16/F16, row stride ld elements):
+ *   logprob[t] = log softmax(logits[t])[targets[t]],  entropy[t] = -sum p log p (nats),
+ *   top_ids[t, i], top_logprobs[t, i]: the top (0..32, at most V) largest, largest first,
+ *   equal values in the order of their index.
+ * targets: int32 (targets_64 = 0) or int64, or NULL; a negative target gives 0, one >= V
+ * NaN. logprob, entropy may be NULL. A logit of -inf has probability 0; a row with a NaN or
+ * +inf logit, or of -inf alone, has NaN results (NaN logits are no alternatives: missing
+ * ones have id -1). scratch: scratch_bytes bytes, 16-byte aligned, and counters (M uint32,
+ * zero before the first call and left zero); qi_token_logprobs_scratch gives the bytes that
+ * use the whole GPU for few rows, with less a row is cut into fewer slices. No reference
+ * counterpart: the reference takes the argmax (qweninfer/engine/engine.py:129,155). */
+int qi_token_logprobs(const void* logits, int dtype, long long ld, const void* targets, int targets_64, int M, int V,
+                      int top, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, void* scratch,
+                      long long scratch_bytes, unsigned int* counters, qi_stream_t stream);
+long long qi_token_logprobs_scratch(int M, int V);
+
 /* ------------------------------------------------------------- whole forward */
 
 typedef struct {

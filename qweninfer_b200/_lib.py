@@ -21,6 +21,9 @@ QI_ERR_TIMEOUT = 1002
 QI_ERR_DEVICE = 1003
 QI_ERR_TOO_LARGE = 1004
 QI_ERR_INDEX = 1005
+QI_KV_BF16, QI_KV_INT8, QI_KV_E4M3 = 0, 1, 2
+# element types of activations (QI_F32, QI_BF16, QI_F16)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # launch kinds of qi_forward_launch_times
 LAUNCH_KINDS = ("embed", "qkv", "attention", "o_proj", "gate_up", "down", "head")
 
@@ -43,6 +46,12 @@ class QiModel(C.Structure):
 
 class QiCache(C.Structure):
     _fields_ = [("k", vp), ("v", vp), ("cache_rows", i32), ("max_len", i32), ("page_table", vp),
+                ("page_size", i32), ("pages_per_row", i32), ("n_pages", i32)]
+
+
+class QiKvLayer(C.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("format", i32), ("block", i32),
+                ("cache_rows", i32), ("kv_heads", i32), ("max_len", i32), ("head_dim", i32), ("page_table", vp),
                 ("page_size", i32), ("pages_per_row", i32), ("n_pages", i32)]
 
 
@@ -74,6 +83,14 @@ SIGNATURES = {
                          i32, i32, i32, i32, vp, i32, i64, vp, vp]),
     "qi_forward_launch_times": (i32, [C.POINTER(QiModel), C.POINTER(QiCache), C.POINTER(QiWorkspace), vp, vp, vp,
                                       i32, i32, i32, i32, vp, i32, i64, vp, vp, vp, vp, i32, vp]),
+    "qi_kv8_append": (i32, [C.POINTER(QiKvLayer), vp, i64, i64, vp, i64, i64, i32, vp, vp, i32, vp, vp]),
+    "qi_kv8_values": (i32, [C.POINTER(QiKvLayer), vp, vp, vp]),
+    "qi_cache_attention": (i32, [C.POINTER(QiKvLayer), vp, i64, i64, i32, i32, vp, vp, i32, i32, i32, i32, vp, vp, i64,
+                                 vp, i64, vp, vp]),
+    "qi_cache_attention_scratch": (i32, [C.POINTER(QiKvLayer), i32, i32, i32, i32, i32, C.POINTER(i64),
+                                         C.POINTER(i64)]),
+    "qi_token_logprobs": (i32, [vp, i32, i64, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, i64, vp, vp]),
+    "qi_token_logprobs_scratch": (i64, [i32, i32]),
     "qi_act_tiles": (i32, [vp, vp, i32, i32, i32, vp, vp, i32, vp]),
     "qi_tc_linear": (i32, [vp, i32, i32, vp, i32, i32, vp, i32, f32, vp, i32, vp, i64, vp, i32, i32, vp, vp]),
     "qi_tc_gate_up_swiglu": (i32, [vp, vp, i32, i32, vp, i32, f32, vp, vp, i64, vp, i32, i32, vp, vp]),
@@ -132,6 +149,68 @@ def ensure_device(device: torch.device) -> None:
     check(lib().qi_init(idx), "qi_init")
     _current[0] = idx
     _inited.add(idx)
+
+
+class on_device:
+    """Context of one operator call on `device`'s tensors, which need not be on the current
+    device: PyTorch's current device (whose current stream the call uses) and the library's
+    are `device` inside it."""
+
+    def __init__(self, device: torch.device) -> None:
+        if device.type != "cuda":
+            raise QiError(f"qweninfer_b200 runs on CUDA (sm_100) devices only, got {device}")
+        self.idx = torch.cuda.current_device() if device.index is None else device.index
+        self.other = None
+
+    def __enter__(self) -> None:
+        if torch.cuda.current_device() != self.idx:
+            self.other = torch.cuda.device(self.idx)
+            self.other.__enter__()
+        # the library's current device is per thread, and other calls may have moved it
+        if torch.cuda.device_count() > 1 or self.idx not in _inited:
+            check(lib().qi_init(self.idx), "qi_init")
+            _inited.add(self.idx)
+            _current[0] = self.idx
+
+    def __exit__(self, *exc) -> None:
+        if self.other is not None:
+            self.other.__exit__(*exc)
+            _current[0] = -1
+
+
+class _Scratch:
+    """Scratch of the operator calls of one device and stream: calls of one stream run one
+    after another, so they share it. `counters` are zero between calls."""
+
+    def __init__(self) -> None:
+        self.bytes = 0
+        self.n = 0
+        self.data = self.counters = None
+
+
+_scratch: dict[tuple[int, int], _Scratch] = {}
+
+
+def scratch(device: torch.device, stream: int, nbytes: int, n_counters: int) -> tuple[int, int, object]:
+    """(address of nbytes of scratch, address of n_counters zeroed uint32, what keeps both
+    alive) for a call on `stream`, the current one. A call that is being captured gets its
+    own, from the graph's memory and zeroed by the graph, so that graphs which share no
+    stream when they are replayed share no scratch either."""
+    if nbytes == 0 and n_counters == 0:
+        return 0, 0, None
+    if torch.cuda.is_current_stream_capturing():
+        data = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        counters = torch.zeros(n_counters, dtype=torch.int32, device=device)
+        return data.data_ptr(), counters.data_ptr(), (data, counters)
+    with _lock:
+        s = _scratch.setdefault((device.index or 0, stream), _Scratch())
+        if s.bytes < nbytes:
+            s.data = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            s.bytes = nbytes
+        if s.n < n_counters:
+            s.counters = torch.zeros(max(n_counters, 1024), dtype=torch.int32, device=device)
+            s.n = s.counters.numel()
+        return s.data.data_ptr() if s.data is not None else 0, s.counters.data_ptr(), (s.data, s.counters)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -6,8 +6,11 @@
 #include <cstdlib>
 #include <cstring>
 
+#include "cache_attention.h"
+#include "cache_layer.cuh"
 #include "common.cuh"
 #include "internal.h"
+#include "logprobs.h"
 #include "tc_proj.h"
 
 #include <map>
@@ -386,6 +389,20 @@ int grid_for(int n_tiles, int KB, int max_contrib) {
   return (int)(g < sms ? g : sms);
 }
 
+// Largest number of key splits of a cached-attention call that its scratch holds.
+int splits_within(const qi_kv_layer* c, int group, int M, int window, int sinks, long long part_floats,
+                  long long counters_len) {
+  const long long units = (long long)M * c->kv_heads;
+  int n = cache_attention_splits(M, c->kv_heads, c->max_len, window, sinks);
+  if (counters_len < units) return 1;
+  while (n > 1 && units * n * group * (c->head_dim + 2) > part_floats) --n;
+  return n;
+}
+bool bad_attention(const qi_kv_layer* c, int heads, int M, int window, int sinks, int query_run) {
+  return bad_layer(c) || heads <= 0 || heads % c->kv_heads != 0 || heads / c->kv_heads > 8 || M <= 0 || window < 0 ||
+         sinks < 0 || query_run < 0 || c->kv_heads > 65535 || (long long)M * kMaxAttnSplits > 0x7fffffffLL;
+}
+
 // qi_forward on the tensor-core path: every projection is a tc_proj launch whose
 // epilogue writes the next projection's activation tiles (the RMSNorm weights folded in,
 // the per-token RMS applied in the consumer's epilogue from partial sums of squares).
@@ -695,6 +712,93 @@ int qi_move_rows(uint16_t* k, uint16_t* v, int layers, int cache_rows, int max_l
     if (r != QI_OK) return r;
   }
   return QI_OK;
+}
+
+int qi_kv8_append(const qi_kv_layer* layer, const void* k, long long k_token_stride, long long k_head_stride,
+                  const void* v, long long v_token_stride, long long v_head_stride, int dtype, const int32_t* rows,
+                  const int32_t* pos, int M, int* err, qi_stream_t stream) {
+  if (bad_layer(layer) || layer->format == QI_KV_BF16 || bad_ptr(k) || bad_ptr(v) || bad_dtype(dtype) ||
+      bad_ptr(rows) || bad_ptr(pos) || M <= 0 || layer->kv_heads > 65535)
+    return QI_ERR_ARG;
+  return rc(launch_kv8_append(*layer, k, v, dtype, k_token_stride, k_head_stride, v_token_stride, v_head_stride, rows,
+                              pos, M, err, as_stream(stream), false));
+}
+
+int qi_kv8_values(const qi_kv_layer* layer, float* k_out, float* v_out, qi_stream_t stream) {
+  if (bad_layer(layer) || layer->format == QI_KV_BF16 || bad_ptr(k_out) || bad_ptr(v_out) ||
+      (((uintptr_t)k_out | (uintptr_t)v_out) & 15))
+    return QI_ERR_ARG;
+  return rc(launch_kv8_values(*layer, k_out, v_out, as_stream(stream)));
+}
+
+int qi_cache_attention_scratch(const qi_kv_layer* layer, int heads, int M, int window, int sinks, int query_run,
+                               long long* part_floats, long long* counters_len) {
+  if (bad_attention(layer, heads, M, window, sinks, query_run) || !part_floats || !counters_len) return QI_ERR_ARG;
+  const int n = cache_attention_splits(M, layer->kv_heads, layer->max_len, window, sinks);
+  *part_floats = n > 1 ? (long long)M * heads * n * (layer->head_dim + 2) : 0;
+  *counters_len = n > 1 ? (long long)M * layer->kv_heads : 0;
+  return QI_OK;
+}
+
+int qi_cache_attention(const qi_kv_layer* layer, const void* q, long long q_token_stride, long long q_head_stride,
+                       int dtype, int heads, const int32_t* rows, const int32_t* pos, int M, int window, int sinks,
+                       int query_run, void* out, float* part, long long part_floats, unsigned int* counters,
+                       long long counters_len, int* err, qi_stream_t stream) {
+  if (bad_attention(layer, heads, M, window, sinks, query_run) || bad_ptr(q) || bad_dtype(dtype) || bad_ptr(rows) ||
+      bad_ptr(pos) || bad_ptr(out) || ((uintptr_t)part & 7))
+    return QI_ERR_ARG;
+  CacheAttnParams p = {};
+  p.c = *layer;
+  p.q = q;
+  p.dtype = dtype;
+  p.q_st = q_token_stride;
+  p.q_sh = q_head_stride;
+  p.heads = heads;
+  p.group = heads / layer->kv_heads;
+  p.rows = rows;
+  p.pos = pos;
+  p.M = M;
+  p.window = window;
+  p.sinks = sinks;
+  p.out = out;
+  p.part = part;
+  p.counters = counters;
+  p.splits = part && counters ? splits_within(layer, p.group, M, window, sinks, part_floats, counters_len) : 1;
+  p.err = err;
+  return rc(launch_cache_attention(p, query_run, as_stream(stream), false));
+}
+
+long long qi_token_logprobs_scratch(int M, int V) {
+  if (M <= 0 || V <= 0) return 0;
+  const int n = logprob_slices(M, V);
+  return n > 1 ? (long long)M * n * (16 + 32 * 8) : 0;
+}
+
+int qi_token_logprobs(const void* logits, int dtype, long long ld, const void* targets, int targets_64, int M, int V,
+                      int top, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, void* scratch,
+                      long long scratch_bytes, unsigned int* counters, qi_stream_t stream) {
+  if (bad_ptr(logits) || bad_dtype(dtype) || M <= 0 || V <= 0 || ld < V || top < 0 || top > 32 || top > V ||
+      (top > 0 && (bad_ptr(top_ids) || bad_ptr(top_logprobs))) || (long long)M * kMaxLogprobSlices > 0x7fffffffLL ||
+      ((uintptr_t)scratch & 15))
+    return QI_ERR_ARG;
+  LogprobParams p = {};
+  p.logits = logits;
+  p.ld = ld;
+  p.targets = targets;
+  p.targets64 = targets_64;
+  p.M = M;
+  p.V = V;
+  p.top = top;
+  p.logprob = logprob;
+  p.entropy = entropy;
+  p.top_ids = top_ids;
+  p.top_logprobs = top_logprobs;
+  p.slices = scratch && counters ? logprob_slices(M, V) : 1;
+  while (p.slices > 1 && (long long)M * p.slices * (16 + 32 * 8) > scratch_bytes) --p.slices;
+  p.part_stats = static_cast<float*>(scratch);
+  p.part_list = reinterpret_cast<unsigned long long*>(static_cast<char*>(scratch) + (size_t)M * p.slices * 16);
+  p.counters = counters;
+  return rc(launch_token_logprobs(p, dtype, as_stream(stream), false));
 }
 
 int qi_act_tiles(const float* x, const float* norm_w, int M, int K, int NT, uint16_t* act, float* ss, int ss_ld,

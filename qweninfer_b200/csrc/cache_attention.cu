@@ -1,0 +1,544 @@
+// Grouped-query attention over one cache layer for query tokens that each read their own
+// row: bf16, int8 or e4m3 keys and values, packed or paged, with an optional sliding
+// window and first tokens ("sinks") that stay visible.
+//
+//   o[t, h] = sum_j w_j v_j,  w = softmax over the seen j of q[t, h] . k_j / sqrt(D),
+//   seen: 0 <= j <= p and (no window, or j > p - window, or j < sinks), p = pos[t].
+//
+// One CTA per (key split, KV head, token), 4 warps. The seen keys of a token form a list of
+// granules of 32 aligned positions (the sinks' granules, then the window's); a split takes
+// a contiguous run of the list, of whatever length the token really has, and its warps take
+// the run's granules in turn. Nothing but seen keys is read: a granule's other keys are
+// zero-filled, so what dead positions hold (NaN included) never enters a product.
+//
+// Each warp streams its own granules through a private ring of shared memory with cp.async
+// and never waits for another warp before the merge. A call is bound by the cache's bytes,
+// so what counts is bytes in flight: 16 warps of an SM with two granules each requested.
+//
+// The group's query heads (at most 8) are rows of m16n8k16 MMAs. Row h holds the high part
+// of q_h, row h + 8 the next part: their products land in the same thread, which adds
+// them. 8-bit codes are exact in fp16, so both products run in fp16: q is scaled by a power
+// of two to a maximum in [1, 2) and split into two fp16 parts (22 bits), the probabilities
+// are computed as 2^12 p (the factor cancels in the normalisation) and split the same
+// way. A bf16 cache multiplies in bf16 with three parts of q and p for fp32 callers (24
+// bits) and two for 16-bit ones; the third part is a second MMA. Scores, softmax statistics
+// and outputs are fp32; the block scales multiply scores and products of 16 keys in fp32.
+//
+// The dims of a k-step are permuted: a thread's share of a key is 16 contiguous bytes (one
+// shared-memory load gives 4 k-steps of 8-bit codes or 2 of bf16), and the query fragments
+// are loaded in the same order, which leaves the dot product unchanged. V goes through
+// ldmatrix.trans; for 8-bit codes its 16-bit elements are pairs of neighbouring dims, taken
+// apart into an even and an odd n-tile.
+#include "cache_attention.h"
+#include "cache_layer.cuh"
+#include "tc_proj.h"
+
+namespace qi {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kGran = 32;  // keys per granule
+constexpr int kMaxGroup = 8;
+
+template <int FMT, int D>
+struct Shape {
+  static constexpr int kRow = D * (FMT == QI_KV_BF16 ? 2 : 1);  // bytes of one key
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kTensor = kGran * kRow;                   // K or V of a granule
+  static constexpr int kStage = 2 * kTensor + 16;                // + 2 K scales, 2 V scales
+  static constexpr int kStages = kStage > 9000 ? 2 : 3;
+  static constexpr size_t kRing = (size_t)kWarps * kStages * kStage;
+};
+
+// physical 16-byte chunk c of key r: 8 keys at one chunk (ldmatrix) and 2 keys at 4
+// chunks of one quad (K loads) both cover all banks
+template <int CH>
+__device__ __forceinline__ int swizzle(int r, int c) {
+  if constexpr (CH == 4) return c ^ ((r >> 1) & 3);
+  else return c ^ (((r & 1) << 2) | ((r >> 1) & 3));
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
+  return r;
+}
+__device__ __forceinline__ float lds32(uint32_t addr) {
+  float r;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(addr) : "memory");
+  return r;
+}
+template <bool F16>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// ---- parts of fp32 pairs as 16-bit pairs (a in the low half)
+__device__ __forceinline__ uint32_t f16x2(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t b16x2(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+// the 16-bit parts of (a, b): part 0 = round(x), each next part = round(rest)
+template <bool F16, int N>
+__device__ __forceinline__ void split(float a, float b, uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (F16) {
+      r[i] = f16x2(a, b);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
+      a -= f.x, b -= f.y;
+    } else {
+      r[i] = b16x2(a, b);
+      a -= bf16lo(r[i]), b -= bf16hi(r[i]);
+    }
+  }
+}
+
+// ---- 8-bit codes as fp16 pairs. SEL 0: bytes 0, 1 and 2, 3 (K); SEL 1: bytes 0, 2 and 1, 3
+// (V, where a 16-bit element holds two neighbouring dims of one key). int8: the code plus
+// 128 as the low byte of 0x6400 is 1024 + 128 + code exactly; minus 1152.
+template <int FMT, int SEL>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& p0, uint32_t& p1) {
+  if constexpr (FMT == QI_KV_INT8) {
+    w ^= 0x80808080u;
+    const uint32_t a = __byte_perm(w, 0x64646464u, SEL ? 0x4240 : 0x4140);
+    const uint32_t b = __byte_perm(w, 0x64646464u, SEL ? 0x4341 : 0x4342);
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    p0 = *reinterpret_cast<const uint32_t*>(&x);
+    p1 = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    if constexpr (SEL) w = __byte_perm(w, 0u, 0x3120);
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(p0), "=r"(p1)
+        : "r"(w));
+  }
+}
+
+// Output values of features f .. f + N - 1 (N even, f a multiple of N) of a token.
+template <int N>
+__device__ __forceinline__ void emit(const CacheAttnParams& p, int tok, int f, int width, const float (&v)[N]) {
+  if (p.out) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) store_elem(p.out, p.dtype, (long long)tok * width + f + i, v[i]);
+  }
+  if (p.out_act) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint32_t hi = b16x2(v[i], v[i + 1]);
+      const uint32_t lo = b16x2(v[i] - bf16lo(hi), v[i + 1] - bf16hi(hi));
+      *reinterpret_cast<uint32_t*>(p.out_act + act_offset(tok, f + i, 0, width, p.out_nt)) = hi;
+      *reinterpret_cast<uint32_t*>(p.out_act + act_offset(tok, f + i, 1, width, p.out_nt)) = lo;
+    }
+  }
+}
+
+// The list of granules a token sees.
+struct Seen {
+  int p;      // its position
+  int lo;     // first position of the window
+  int sinks;  // visible first positions (0 when the window reaches position 0)
+  int ns;     // granules of the sinks, before the window's
+  int g0;     // first granule of the window
+  int n;      // granules in all
+  __device__ __forceinline__ int granule(int i) const { return i < ns ? i : g0 + i - ns; }
+  __device__ __forceinline__ bool sees(int j) const { return j <= p && (j >= lo || j < sinks); }
+};
+__device__ __forceinline__ Seen seen_keys(int p, int window, int sinks) {
+  Seen s;
+  s.p = p;
+  s.lo = window > 0 && p >= window ? p - window + 1 : 0;
+  s.sinks = min(sinks, s.lo);
+  s.g0 = s.lo / kGran;
+  s.ns = min((s.sinks + kGran - 1) / kGran, s.g0);
+  s.n = s.ns + p / kGran + 1 - s.g0;
+  return s;
+}
+
+// Granules a split has at least, so that its warps have two each.
+constexpr int kMinSplit = 2 * kWarps;
+
+// F16 products for 8-bit codes, bf16 for a bf16 cache; P3: three parts of q and p (bf16).
+template <int FMT, int D, bool P3>
+__global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAttnParams p) {
+  using S = Shape<FMT, D>;
+  constexpr bool F16 = FMT != QI_KV_BF16;
+  constexpr int kParts = P3 ? 3 : 2, kA = P3 ? 2 : 1;  // parts, A operands
+  constexpr int kSteps = D / 16;                       // k-steps of a key
+  constexpr int kPer = F16 ? 4 : 2;                    // k-steps in 16 bytes
+  constexpr int kOut = D / 4;                          // output dims of a thread
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, qd = lane & 3;
+  const int tok = blockIdx.x / p.splits, split_i = blockIdx.x - tok * p.splits, g = blockIdx.y;
+  const qi_kv_layer& c = p.c;
+  const int G = p.group, width = p.heads * D;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int ps = p.pos[tok], row = p.rows[tok];
+  const bool ok = ps >= 0 && ps < c.max_len && row >= 0 && row < c.cache_rows;
+  if (!ok) {  // nothing seen: zeros; a position or row outside the cache is reported
+    if (split_i == 0) {
+      if (ps != -1 && tid == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
+      const float z[2] = {0.f, 0.f};
+      for (int e = tid; e < G * D / 2; e += kThreads) emit<2>(p, tok, g * G * D + 2 * e, width, z);
+    }
+    return;
+  }
+  const Seen seen = seen_keys(ps, p.window, p.sinks);
+  const int nsplit = min(p.splits, (seen.n + kMinSplit - 1) / kMinSplit);
+  if (split_i >= nsplit) return;
+  const int gbeg = (int)((long long)seen.n * split_i / nsplit), gend = (int)((long long)seen.n * (split_i + 1) / nsplit);
+
+  const uint32_t ring = smem_u32(smem) + (uint32_t)(warp * S::kStages * S::kStage);
+  // granule i (its place in the list) into ring stage st; nothing for i >= gend
+  auto issue = [&](int i, int st) {
+    if (i < gend) {
+      const int k0 = seen.granule(i) * kGran;
+      long long o = layer_offset(c, D, row, g, k0);
+      if (o < 0) {  // an unmapped page: reported, read as zeros
+        if (lane == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
+      }
+      const bool mapped = o >= 0;
+      const uint8_t* kb = static_cast<const uint8_t*>(c.k) + (mapped ? o : 0) * (S::kRow / D);
+      const uint8_t* vb = static_cast<const uint8_t*>(c.v) + (mapped ? o : 0) * (S::kRow / D);
+      const uint32_t dst = ring + (uint32_t)(st * S::kStage);
+#pragma unroll
+      for (int j = 0; j < S::kChunks; ++j) {
+        const int x = lane + 32 * j, r = x / S::kChunks, ch = x % S::kChunks;
+        const uint32_t n = mapped && seen.sees(k0 + r) ? 16u : 0u;
+        const uint32_t at = dst + (uint32_t)(r * S::kRow + swizzle<S::kChunks>(r, ch) * 16);
+        // a key that is not seen reads nothing; its address stays at the granule's first key
+        cp16(at, kb + (n ? x * 16 : 0), n);
+        cp16(at + S::kTensor, vb + (n ? x * 16 : 0), n);
+      }
+      if constexpr (F16) {
+        if (lane < 4) {  // scales of the granule's halves: K, K, V, V
+          const int h0 = k0 + 16 * (lane & 1);
+          const bool any = mapped && h0 <= seen.p && (h0 + 15 >= seen.lo || h0 < seen.sinks);
+          const long long si = any ? scale_index(c, row, g, h0) : 0;
+          cp4(dst + 2 * S::kTensor + 4 * lane, (lane < 2 ? c.k_scale : c.v_scale) + si, any ? 4u : 0u);
+        }
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S::kStages - 1; ++s) issue(gbeg + warp + s * kWarps, s);
+
+  // the query fragments: dims 16 bytes apart per quad, in the keys' chunk order
+  uint32_t qa[kA][kSteps][4];
+  float qscale = p.scale_log2;
+  {
+    float x[D / 4];
+    const long long qo = (long long)tok * p.q_st + (long long)(g * G + (gq < G ? gq : 0)) * p.q_sh;
+#pragma unroll
+    for (int i = 0; i < D / 4; i += 4) {
+      // i-th value of this thread: k-step i / 4 lies in chunk 4 * (i / 4 / kPer) + qd
+      const int d = (4 * (i / 4 / kPer) + qd) * 4 * kPer + (i / 4 % kPer) * 4;
+      if (p.q_vec && p.dtype == QI_F32) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + qo + d));
+        x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[i + e] = p.dtype == QI_F32    ? load_elem<QI_F32>(p.q, qo + d + e)
+                     : p.dtype == QI_BF16 ? load_elem<QI_BF16>(p.q, qo + d + e)
+                                          : load_elem<QI_F16>(p.q, qo + d + e);
+      }
+    }
+    if (gq >= G) {
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+    }
+    if constexpr (F16) {
+      // q * 2^-e in [1, 2) at its largest: fp16 parts keep 22 bits of every head's scale
+      float am = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) am = fmaxf(am, fabsf(x[i]));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+      const uint32_t e = __float_as_uint(am) >> 23;  // biased exponent (am >= 0)
+      if (e > 0 && e < 253) {
+        const float inv = __uint_as_float((254u - e) << 23);
+        qscale *= __uint_as_float(e << 23);
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) x[i] *= inv;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      uint32_t a[kParts], b[kParts];
+      split<F16, kParts>(x[4 * s], x[4 * s + 1], a);
+      split<F16, kParts>(x[4 * s + 2], x[4 * s + 3], b);
+      qa[0][s][0] = a[0], qa[0][s][1] = a[1], qa[0][s][2] = b[0], qa[0][s][3] = b[1];
+      if constexpr (P3) qa[1][s][0] = a[2], qa[1][s][1] = 0u, qa[1][s][2] = b[2], qa[1][s][3] = 0u;
+    }
+  }
+
+  float m = -INFINITY, l = 0.f, o[kOut];
+#pragma unroll
+  for (int i = 0; i < kOut; ++i) o[i] = 0.f;
+
+  int st = 0;
+  for (int i = gbeg + warp; i < gend; i += kWarps) {
+    cp_wait<S::kStages - 2>();
+    __syncwarp();  // the granule is in place for every lane, and the last one is read
+    issue(i + (S::kStages - 1) * kWarps, st == 0 ? S::kStages - 1 : st - 1);
+    const uint32_t kt = ring + (uint32_t)(st * S::kStage), vt = kt + S::kTensor;
+    st = st + 1 == S::kStages ? 0 : st + 1;
+    const int k0 = seen.granule(i) * kGran;
+
+    // scores of head gq for keys 8 t + 2 qd + e
+    float sc[4][2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < S::kChunks / 4; ++h) {
+        const uint4 w = lds128(kt + (uint32_t)((8 * t + gq) * S::kRow + swizzle<S::kChunks>(8 * t + gq, 4 * h + qd) * 16));
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          uint32_t b0, b1;
+          if constexpr (F16) widen<FMT, 0>(ws[j], b0, b1);
+          else b0 = ws[2 * j], b1 = ws[2 * j + 1];
+          mma<F16>(acc, qa[0][kPer * h + j], b0, b1);
+          if constexpr (P3) mma<F16>(acc, qa[1][kPer * h + j], b0, b1);
+        }
+      }
+      float f = qscale;
+      if constexpr (F16) f *= lds32(kt + 2 * S::kTensor + 4 * (t >> 1));
+      sc[t][0] = (acc[0] + acc[2]) * f;
+      sc[t][1] = (acc[1] + acc[3]) * f;
+    }
+    if (k0 + kGran - 1 > seen.p || (k0 < seen.lo && k0 + kGran > seen.sinks)) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (!seen.sees(k0 + 8 * t + 2 * qd + e)) sc[t][e] = -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])),
+                     fmaxf(fmaxf(sc[2][0], sc[2][1]), fmaxf(sc[3][0], sc[3][1])));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    if (__any_sync(0xffffffffu, mx > m)) {  // a new maximum: rescale what is summed so far
+      const float mn = fmaxf(m, mx);
+      const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < kOut; ++d) o[d] *= alpha;
+    }
+    // probabilities relative to the running maximum (8-bit: times 2^12, which keeps the
+    // second fp16 part of small ones above the subnormal range)
+    const float mref = (m == -INFINITY ? 0.f : m) - (F16 ? 12.f : 0.f);
+    uint32_t pa[2][kA][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const float p0 = ex2(sc[t][0] - mref), p1 = ex2(sc[t][1] - mref);
+      l += p0 + p1;
+      uint32_t r[kParts];
+      split<F16, kParts>(p0, p1, r);
+      pa[t >> 1][0][2 * (t & 1)] = r[0];
+      pa[t >> 1][0][2 * (t & 1) + 1] = r[1];
+      if constexpr (P3) pa[t >> 1][1][2 * (t & 1)] = r[2], pa[t >> 1][1][2 * (t & 1) + 1] = 0u;
+    }
+    // O += P V, 16 keys at a time (one block scale each)
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      float sv = 1.f;
+      if constexpr (F16) sv = lds32(kt + 2 * S::kTensor + 8 + 4 * hf);
+#pragma unroll
+      for (int h = 0; h < S::kChunks / 2; ++h) {
+        // matrices: keys 16 hf + 8 (j & 1) .., chunk 2 h + (j >> 1)
+        const int lj = lane >> 3, r = 16 * hf + 8 * (lj & 1) + (lane & 7), ch = 2 * h + (lj >> 1);
+        uint32_t b[4];
+        ldsm4t(vt + (uint32_t)(r * S::kRow + swizzle<S::kChunks>(r, ch) * 16), b);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (F16) {
+            // chunk of 16 dims: this thread's columns are dims 4 qd + {0, 2} of the even and
+            // {1, 3} of the odd n-tile
+            uint32_t e0, e1, d0, d1;
+            widen<FMT, 1>(b[2 * u], e0, d0);
+            widen<FMT, 1>(b[2 * u + 1], e1, d1);
+            mma<F16>(acc, pa[hf][0], e0, e1);
+            float* oo = o + 4 * (2 * h + u);
+            oo[0] = fmaf(sv, acc[0] + acc[2], oo[0]);
+            oo[2] = fmaf(sv, acc[1] + acc[3], oo[2]);
+            float ac2[4] = {0.f, 0.f, 0.f, 0.f};
+            mma<F16>(ac2, pa[hf][0], d0, d1);
+            oo[1] = fmaf(sv, ac2[0] + ac2[2], oo[1]);
+            oo[3] = fmaf(sv, ac2[1] + ac2[3], oo[3]);
+          } else {
+            mma<F16>(acc, pa[hf][0], b[2 * u], b[2 * u + 1]);
+            if constexpr (P3) mma<F16>(acc, pa[hf][1], b[2 * u], b[2 * u + 1]);
+            float* oo = o + 2 * (2 * h + u);
+            oo[0] += acc[0] + acc[2];
+            oo[1] += acc[1] + acc[3];
+          }
+        }
+      }
+    }
+  }
+  cp_wait<0>();
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+
+  // merge of the warps, in shared memory that the rings no longer need
+  constexpr int kPart = D + 2;
+  float* wp = reinterpret_cast<float*>(smem);  // [warp][head][D values, m, l]
+  __syncthreads();
+  if (gq < G) {
+    float* w = wp + (warp * G + gq) * kPart;
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+      const int d = F16 ? 16 * (i / 4) + 4 * qd + i % 4 : 8 * (i / 2) + 2 * qd + i % 2;
+      w[d] = o[i];
+    }
+    if (qd == 0) w[D] = m, w[D + 1] = l;
+  }
+  __syncthreads();
+  // weighted sum over n partials (stride floats apart) of head h, dims d and d + 1
+  auto merge2 = [&](auto load, int n, int h, int d, float& m_out, float& l_out, float& a, float& b) {
+    float mx = -INFINITY;
+    for (int w = 0; w < n; ++w) mx = fmaxf(mx, load(w, h * kPart + D));
+    m_out = mx, l_out = 0.f, a = 0.f, b = 0.f;
+    for (int w = 0; w < n; ++w) {
+      const float mw = load(w, h * kPart + D);
+      // a partial without keys (maximum -inf) has nothing to add; a NaN stays one
+      const float f = mw == -INFINITY ? (load(w, h * kPart + D + 1) == 0.f ? 0.f : 1.f) : ex2(mw - mx);
+      l_out = fmaf(f, load(w, h * kPart + D + 1), l_out);
+      a = fmaf(f, load(w, h * kPart + d), a);
+      b = fmaf(f, load(w, h * kPart + d + 1), b);
+    }
+  };
+  const long long unit = (long long)tok * c.kv_heads + g;
+  float* part = p.part + (unit * p.splits + split_i) * (long long)(G * kPart);
+  auto from_smem = [&](int w, int i) { return wp[w * G * kPart + i]; };
+  for (int e = tid; e < G * D / 2; e += kThreads) {
+    const int h = e / (D / 2), d = 2 * (e - h * (D / 2));
+    float mm, ll, a, b;
+    merge2(from_smem, kWarps, h, d, mm, ll, a, b);
+    if (nsplit == 1) {
+      const float inv = ll != 0.f ? 1.f / ll : 0.f;
+      const float v[2] = {a * inv, b * inv};
+      emit<2>(p, tok, g * G * D + h * D + d, width, v);
+    } else {
+      __stcg(reinterpret_cast<float2*>(part + h * kPart + d), make_float2(a, b));
+      if (d == 0) __stcg(reinterpret_cast<float2*>(part + h * kPart + D), make_float2(mm, ll));
+    }
+  }
+  if (nsplit == 1) return;
+  // the last split of the unit merges them all, in split order, and leaves the counter zero
+  __syncthreads();
+  if (tid == 0) last = atomic_add_acq_rel(p.counters + unit, 1u) == (unsigned)(nsplit - 1);
+  __syncthreads();
+  if (!last) return;
+  const float* parts = p.part + unit * p.splits * (long long)(G * kPart);
+  auto from_part = [&](int w, int i) { return __ldcg(parts + (long long)w * (G * kPart) + i); };
+  for (int e = tid; e < G * D / 2; e += kThreads) {
+    const int h = e / (D / 2), d = 2 * (e - h * (D / 2));
+    float mm, ll, a, b;
+    merge2(from_part, nsplit, h, d, mm, ll, a, b);
+    const float inv = ll != 0.f ? 1.f / ll : 0.f;
+    const float v[2] = {a * inv, b * inv};
+    emit<2>(p, tok, g * G * D + h * D + d, width, v);
+  }
+  if (tid == 0) p.counters[unit] = 0u;
+}
+
+template <int FMT, int D, bool P3>
+cudaError_t launch_token(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
+  auto kernel = cache_attention_kernel<FMT, D, P3>;
+  constexpr size_t merge = sizeof(float) * kWarps * kMaxGroup * (D + 2);
+  constexpr size_t smem = Shape<FMT, D>::kRing > merge ? Shape<FMT, D>::kRing : merge;
+  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.M * p.splits), p.c.kv_heads, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int D>
+cudaError_t launch_dim(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
+  if (p.c.format == QI_KV_INT8) return launch_token<QI_KV_INT8, D, false>(p, s, pdl);
+  if (p.c.format == QI_KV_E4M3) return launch_token<QI_KV_E4M3, D, false>(p, s, pdl);
+  return p.dtype == QI_F32 ? launch_token<QI_KV_BF16, D, true>(p, s, pdl) : launch_token<QI_KV_BF16, D, false>(p, s, pdl);
+}
+
+}  // namespace
+
+int cache_attention_splits(int M, int kv_heads, int max_len, int window, int sinks) {
+  long long keys = max_len;
+  if (window > 0 && (long long)window + sinks < keys) keys = (long long)window + sinks;
+  const long long gran = keys / kGran + 2;
+  const long long units = (long long)M * kv_heads;
+  const long long most = (gran + kMinSplit - 1) / kMinSplit;
+  long long want = (4LL * sm_count() + units - 1) / units;  // four CTAs per SM
+  if (want > most) want = most;
+  if (want > kMaxAttnSplits) want = kMaxAttnSplits;
+  return (int)(want < 1 ? 1 : want);
+}
+
+cudaError_t launch_cache_attention(const CacheAttnParams& args, int query_run, cudaStream_t s, bool pdl) {
+  (void)query_run;
+  CacheAttnParams p = args;
+  p.scale_log2 = 1.4426950408889634f / sqrtf((float)p.c.head_dim);
+  p.q_vec = p.dtype == QI_F32 && ((uintptr_t)p.q & 15) == 0 && (p.q_st & 3) == 0 && (p.q_sh & 3) == 0;
+  return p.c.head_dim == 64 ? launch_dim<64>(p, s, pdl) : launch_dim<128>(p, s, pdl);
+}
+
+}  // namespace qi

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/qi.h"
 #include "kv_layout.h"
 
 namespace qi {
@@ -112,6 +113,12 @@ cudaError_t launch_rmsnorm(const float* x, const float* w, float eps, int M, flo
 
 cudaError_t launch_rope(float* q, int hq, float* k, int hk, int B, int S, const int32_t* pos, const float* cos_t,
                         const float* sin_t, cudaStream_t s);
+
+// 8-bit cache layers (kv8.cu)
+cudaError_t launch_kv8_append(const qi_kv_layer& c, const void* k, const void* v, int dtype, long long k_st,
+                              long long k_sh, long long v_st, long long v_sh, const int32_t* rows, const int32_t* pos,
+                              int M, int* err, cudaStream_t s, bool pdl);
+cudaError_t launch_kv8_values(const qi_kv_layer& c, float* k_out, float* v_out, cudaStream_t s);
 
 // Device ordinals the per-device caches of this library cover.
 constexpr int kMaxDevices = 64;

@@ -1,0 +1,215 @@
+// The 8-bit KV cache: append with block scales, and the values a layer stands for.
+//
+// A block is `block` consecutive positions of one cache row and KV head, K and V apart. Its
+// scale s is a power of two with top * s >= |x| for all it holds (top = 127 for int8, 448
+// for e4m3), and x is held as the code nearest to x / s, ties to even. Multiplying by a
+// power of two is exact, so a code depends on nothing but the values; when an append needs
+// a larger scale the earlier codes of its block are rounded again to code * old / new, and
+// because a scale at least doubles each time, all roundings of one value together stay
+// below one step of the final scale.
+#include "cache_layer.cuh"
+
+namespace qi {
+
+namespace {
+
+constexpr int kAppendThreads = 256;  // half for K, half for V
+constexpr int kHalf = kAppendThreads / 2;
+constexpr int kMaxBlock = 128;
+
+struct Kv8AppendParams {
+  qi_kv_layer c;
+  const void* k;
+  const void* v;
+  long long k_st, k_sh, v_st, v_sh;  // element strides of token and head
+  const int32_t* rows;
+  const int32_t* pos;
+  int M;
+  int* err;
+};
+
+// 4 consecutive elements; `vec`: the address is aligned for one load
+template <int DT>
+__device__ __forceinline__ void load4(const void* p, long long i, bool vec, float (&x)[4]) {
+  if (vec) {
+    if constexpr (DT == QI_F32) {
+      const float4 f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
+      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+    } else {
+      const uint2 u = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i));
+      if constexpr (DT == QI_BF16) {
+        x[0] = bf16lo(u.x), x[1] = bf16hi(u.x), x[2] = bf16lo(u.y), x[3] = bf16hi(u.y);
+      } else {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = load_elem<DT>(p, i + e);
+  }
+}
+
+// CTA (token t, head g). The tokens of one call may come in any order, so one of a block's
+// tokens takes all of them: the one with the lowest position. A token right behind its
+// predecessor in the same block ends at once; the others (run starts: one for each block
+// of a prompt, every token of a decode step) look through rows and positions for the
+// block's tokens. Of two tokens with the same row and position the later one is kept.
+template <int FMT, int DT>
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8AppendParams p) {
+  __shared__ int slot[kMaxBlock];  // token that holds the block's position, -1: none
+  __shared__ float red[kAppendThreads / 32];
+  grid_dep_wait();
+  grid_dep_launch();
+  const qi_kv_layer& c = p.c;
+  const int t = blockIdx.x, g = blockIdx.y, tid = threadIdx.x;
+  const int D = c.head_dim, block = c.block;
+  const int ps = p.pos[t], row = p.rows[t];
+  if (ps == -1) return;  // an idle slot
+  if (ps < 0 || ps >= c.max_len || row < 0 || row >= c.cache_rows) {
+    if (tid == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
+    return;
+  }
+  if (t > 0 && ps % block != 0 && p.rows[t - 1] == row && p.pos[t - 1] == ps - 1) return;
+  const int first = ps - ps % block;  // the block's first position
+  for (int i = tid; i < block; i += kAppendThreads) slot[i] = -1;
+  __syncthreads();
+  for (int i = tid; i < p.M; i += kAppendThreads) {
+    const int q = p.pos[i];
+    if (q >= first && q < first + block && q < c.max_len && p.rows[i] == row) atomicMax(&slot[q - first], i);
+  }
+  __syncthreads();
+  int f = 0;
+  while (slot[f] < 0) ++f;  // ends: this token's own slot is taken
+  if (slot[f] != t) return;
+
+  const long long base = layer_offset(c, D, row, g, first);
+  if (base < 0) {
+    if (tid == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
+    return;
+  }
+  const long long si = scale_index(c, row, g, first);
+  const bool isv = tid >= kHalf;
+  const int ht = tid & (kHalf - 1);
+  const void* x = isv ? p.v : p.k;
+  const long long st = isv ? p.v_st : p.k_st;
+  const long long xo = (long long)g * (isv ? p.v_sh : p.k_sh);
+  uint8_t* codes = static_cast<uint8_t*>(isv ? c.v : c.k) + base;
+  float* scale = (isv ? c.v_scale : c.k_scale) + si;
+  const int esz = DT == QI_F32 ? 4 : 2;
+  const bool vec = ((uintptr_t)x % (4 * esz)) == 0 && (st & 3) == 0 && (xo & 3) == 0;
+  const int quads = D / 4, n = block * quads;
+
+  float amax = 0.f;
+  bool bad = false;
+  for (int i = ht; i < n; i += kHalf) {
+    const int s = i / quads, tok = slot[s];
+    if (tok < 0) continue;
+    float v[4];
+    load4<DT>(x, tok * st + xo + (i - s * quads) * 4, vec, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      bad |= !(fabsf(v[e]) <= 3.402823466e38f);
+      amax = fmaxf(amax, fabsf(v[e]));
+    }
+  }
+  amax = warp_max(bad ? INFINITY : amax);
+  if ((tid & 31) == 0) red[tid >> 5] = amax;
+  __syncthreads();
+  const int w0 = isv ? kHalf / 32 : 0;
+  amax = fmaxf(fmaxf(red[w0], red[w0 + 1]), fmaxf(red[w0 + 2], red[w0 + 3]));
+  // A value that is not finite makes the block's scale NaN, and with it every result that
+  // reads the block, as the value itself would.
+  float s_new = amax == INFINITY ? __uint_as_float(0x7fc00000u) : scale_for<FMT>(amax);
+  float s_old = s_new;
+  if (f > 0) {  // the block keeps its earlier positions
+    s_old = *scale;
+    s_new = s_old >= s_new || s_old != s_old ? s_old : s_new;
+  }
+  // 1 / s is exact: s = 2^e with -126 <= e <= 122
+  const float inv = 1.0f / s_new, again = s_old * inv;
+  // Values next to the largest float would round to 2^128: their code stops at the last
+  // one whose value is finite (63 * 2^122 for int8, 240 * 2^120 for e4m3).
+  constexpr float kHugeScale = FMT == QI_KV_INT8 ? 0x1p122f : 0x1p120f, kHugeTop = FMT == QI_KV_INT8 ? 63.f : 240.f;
+  const float most = s_new >= kHugeScale ? kHugeTop : INFINITY;
+  auto code = [&](float x) { return encode<FMT>(x == x ? fminf(fmaxf(x, -most), most) : x); };
+  __syncthreads();  // every thread has read *scale
+  if (ht == 0) *scale = s_new;
+  for (int i = ht; i < n; i += kHalf) {
+    const int s = i / quads, d = (i - s * quads) * 4, tok = slot[s];
+    uchar4* out = reinterpret_cast<uchar4*>(codes + s * D + d);
+    if (tok >= 0) {
+      float v[4];
+      load4<DT>(x, tok * st + xo + d, vec, v);
+      *out = make_uchar4(code(v[0] * inv), code(v[1] * inv), code(v[2] * inv), code(v[3] * inv));
+    } else if (s < f && again != 1.0f) {
+      const uchar4 o = *out;
+      *out = make_uchar4(code(decode<FMT>(o.x) * again), code(decode<FMT>(o.y) * again),
+                         code(decode<FMT>(o.z) * again), code(decode<FMT>(o.w) * again));
+    }
+  }
+}
+
+// fp32 values of a layer by (row, head, position): one thread for 4 dims of K and of V.
+// Positions on unmapped pages are zero.
+template <int FMT>
+__global__ void __launch_bounds__(256) kv8_values_kernel(const qi_kv_layer c, float* __restrict__ ko,
+                                                         float* __restrict__ vo, long long n) {
+  const int quads = c.head_dim / 4;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+    const long long cell = i / quads;  // (row, head, position)
+    const int d = (int)(i - cell * quads) * 4;
+    const long long rg = cell / c.max_len;
+    const int pos = (int)(cell - rg * c.max_len), row = (int)(rg / c.kv_heads), g = (int)(rg - (long long)row * c.kv_heads);
+    const long long o = layer_offset(c, c.head_dim, row, g, pos);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (o >= 0) {
+      const long long si = scale_index(c, row, g, pos);
+      const uchar4 x = *reinterpret_cast<const uchar4*>(static_cast<const uint8_t*>(c.k) + o + d);
+      const uchar4 y = *reinterpret_cast<const uchar4*>(static_cast<const uint8_t*>(c.v) + o + d);
+      const float s = __ldg(c.k_scale + si), u = __ldg(c.v_scale + si);
+      a = make_float4(decode<FMT>(x.x) * s, decode<FMT>(x.y) * s, decode<FMT>(x.z) * s, decode<FMT>(x.w) * s);
+      b = make_float4(decode<FMT>(y.x) * u, decode<FMT>(y.y) * u, decode<FMT>(y.z) * u, decode<FMT>(y.w) * u);
+    }
+    reinterpret_cast<float4*>(ko)[i] = a;
+    reinterpret_cast<float4*>(vo)[i] = b;
+  }
+}
+
+template <int FMT>
+cudaError_t launch_append(const Kv8AppendParams& p, int dtype, cudaStream_t s, bool pdl) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.M, p.c.kv_heads, 1);
+  cfg.blockDim = dim3(kAppendThreads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  if (dtype == QI_F32) return cudaLaunchKernelEx(&cfg, kv8_append_kernel<FMT, QI_F32>, p);
+  if (dtype == QI_BF16) return cudaLaunchKernelEx(&cfg, kv8_append_kernel<FMT, QI_BF16>, p);
+  return cudaLaunchKernelEx(&cfg, kv8_append_kernel<FMT, QI_F16>, p);
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_append(const qi_kv_layer& c, const void* k, const void* v, int dtype, long long k_st,
+                              long long k_sh, long long v_st, long long v_sh, const int32_t* rows, const int32_t* pos,
+                              int M, int* err, cudaStream_t s, bool pdl) {
+  const Kv8AppendParams p = {c, k, v, k_st, k_sh, v_st, v_sh, rows, pos, M, err};
+  return c.format == QI_KV_INT8 ? launch_append<QI_KV_INT8>(p, dtype, s, pdl)
+                                : launch_append<QI_KV_E4M3>(p, dtype, s, pdl);
+}
+
+cudaError_t launch_kv8_values(const qi_kv_layer& c, float* k_out, float* v_out, cudaStream_t s) {
+  const long long n = (long long)c.cache_rows * c.kv_heads * c.max_len * (c.head_dim / 4);
+  const long long want = (n + 255) / 256, most = 16LL * sm_count();
+  const int grid = (int)(want < most ? want : most);
+  if (c.format == QI_KV_INT8) kv8_values_kernel<QI_KV_INT8><<<grid, 256, 0, s>>>(c, k_out, v_out, n);
+  else kv8_values_kernel<QI_KV_E4M3><<<grid, 256, 0, s>>>(c, k_out, v_out, n);
+  return cudaGetLastError();
+}
+
+}  // namespace qi

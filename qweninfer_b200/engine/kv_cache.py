@@ -13,6 +13,11 @@ so `update` exists for API compatibility only; `move_row` runs the qi_move_rows 
 stores positions in pages of 128 slots taken from a pool on demand, so the cache holds
 the live tokens rather than rows x max_len, and a retired row's hole is filled by moving
 page-table entries instead of copying K/V.
+
+`Kv8Cache` (no reference counterpart either) holds 8-bit codes with a scale for each block
+of positions and KV head: half the bytes to keep and to read. Every cache answers
+`attend`, grouped-query attention of query tokens over one of its layers, with an optional
+sliding window and first tokens that stay visible.
 """
 
 from __future__ import annotations
@@ -24,6 +29,14 @@ import torch
 
 from qweninfer_b200 import _lib
 from qweninfer_b200.models.config import Qwen2Config
+
+
+def _require(t: torch.Tensor, name: str, device: torch.device) -> None:
+    if device.type != "cuda" or t.device != device:
+        raise _lib.QiError(f"{name}: qweninfer_b200 computes on CUDA (sm_100) tensors of one device only, "
+                           f"got {t.device} and a cache on {device}")
+    if t.dtype not in _lib.DTYPES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
 
 
 class KVCache:
@@ -48,6 +61,118 @@ class KVCache:
             self._native = _lib.QiCache(self.k.data_ptr(), self.v.data_ptr(), self.max_batch, self.max_len,
                                         None, 0, 0, 0)
         return self._native
+
+    # ---------------------------------------------------------- operators of a layer
+
+    def layer(self, layer: int) -> _lib.QiKvLayer:
+        """The qi_kv_layer descriptor of one layer (kept for further calls)."""
+        layers = self.__dict__.setdefault("_layers", {})
+        if layer not in layers:
+            if not 0 <= layer < self.k.shape[0]:
+                raise IndexError(f"layer {layer} outside 0..{self.k.shape[0] - 1}")
+            layers[layer] = self._layer(layer)
+        return layers[layer]
+
+    def _layer(self, i: int) -> _lib.QiKvLayer:
+        return _lib.QiKvLayer(self.k[i].data_ptr(), self.v[i].data_ptr(), None, None, _lib.QI_KV_BF16, 0,
+                              self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1], None, 0, 0, 0)
+
+    def _errors(self) -> torch.Tensor:
+        err = self.__dict__.get("_err")
+        if err is None:
+            err = self._err = torch.zeros(1, dtype=torch.int32, device=self.k.device)
+        return err
+
+    def check(self) -> None:
+        """Raise if an `attend` or `append` of this cache met a position, cache row or page
+        outside it (synchronises)."""
+        e = int(self._errors().item())
+        if e:
+            raise _lib.QiError(f"device error word = {e} (a position, cache row or page outside the cache)")
+
+    def _tokens(self, M: int, rows: torch.Tensor, pos: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """Rows and positions of M tokens as int32 on the device; those given on the host are
+        checked there."""
+        out = []
+        for name, t, lo, hi in (("rows", rows, 0, self.max_batch), ("pos", pos, -1, self.max_len)):
+            if t.dim() != 1 or t.shape[0] != M:
+                raise ValueError(f"{name} must have shape ({M},), got {tuple(t.shape)}")
+            if t.device.type == "cpu":
+                if t.dtype not in (torch.int32, torch.int64):
+                    raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+                if M and (int(t.min()) < lo or int(t.max()) >= hi):
+                    raise IndexError(f"{name} [{int(t.min())}, {int(t.max())}] outside {lo}..{hi - 1}")
+                t = t.to(torch.int32).to(self.k.device)
+            elif t.dtype != torch.int32 or t.device != self.k.device:
+                raise ValueError(f"{name} on a device must be int32 on {self.k.device}, got {t.dtype} on {t.device}")
+            out.append(t if t.is_contiguous() else t.contiguous())
+        return out[0], out[1]
+
+    def _operand(self, name: str, t: torch.Tensor, heads: int | None) -> None:
+        _require(t, name, self.k.device)
+        if t.dim() != 3 or t.shape[2] != self.k.shape[-1] or (heads is not None and t.shape[1] != heads):
+            raise ValueError(f"{name} must be (tokens, {'heads' if heads is None else heads}, {self.k.shape[-1]}), "
+                             f"got {tuple(t.shape)}")
+        if t.stride(2) != 1:
+            raise ValueError(f"the last dimension of {name} must be contiguous")
+
+    @torch.no_grad()
+    def attend(self, layer: int, q: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor, window: int = 0,
+               sinks: int = 0, query_run: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Grouped-query attention of M query tokens over layer `layer` (qi_cache_attention).
+
+        q: (M, heads, head_dim) float32, bfloat16 or float16, any strides of the first two
+        dimensions; heads is 1 to 8 times the cache's KV heads and head_dim 64 or 128. Token
+        t, at position pos[t] of cache row rows[t], sees key j if 0 <= j <= pos[t] and, with
+        a `window` (> 0), j > pos[t] - window or j < sinks. pos[t] = -1 marks an idle slot:
+        its output is zero. rows and pos: (M,) int32 on the cache's device, or integers on
+        the host, which are checked (on the device, one outside the cache is recorded for
+        `check()` and gives a zero output). `query_run`: the longest run of consecutive
+        tokens of one row (a prompt's length), 1 for a decode step, 0 if unknown; it only
+        picks the kernel. Returns (M, heads, head_dim) of q's dtype (`out`, if given:
+        contiguous and apart from q), enqueued on the current stream.
+
+        Scores, softmax and sums are fp32; q and the probabilities keep at least 22 bits for
+        an 8-bit cache, 24 (16 for 16-bit q) for a bf16 one."""
+        d = self.layer(layer)
+        self._operand("q", q, None)
+        M, heads, D = q.shape
+        if D not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {D}")
+        if heads == 0 or heads % d.kv_heads or heads // d.kv_heads > 8:
+            raise ValueError(f"{heads} query heads are not 1 to 8 for each of {d.kv_heads} KV heads")
+        if window < 0 or sinks < 0 or query_run < 0:
+            raise ValueError("window, sinks and query_run must not be negative")
+        rows, pos = self._tokens(M, rows, pos)
+        if out is None:
+            out = torch.empty((M, heads, D), dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {q.device}")
+        elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+            raise ValueError("out must not share q's storage")
+        if M == 0:
+            return out
+        lim = 2**31 - 1
+        window, sinks, query_run = min(window, lim), min(sinks, lim), min(query_run, lim)
+        with _lib.on_device(self.k.device):
+            L = _lib.lib()
+            plan = self.__dict__.setdefault("_plans", {})
+            key = (M, heads, window, sinks, query_run)
+            need = plan.get(key)
+            if need is None:
+                a, b = C.c_longlong(), C.c_longlong()
+                _lib.check(L.qi_cache_attention_scratch(C.byref(d), heads, M, window, sinks, query_run, C.byref(a),
+                                                        C.byref(b)), "qi_cache_attention_scratch")
+                if len(plan) >= 4096:
+                    plan.clear()
+                need = plan[key] = (a.value, b.value)
+            stream = _lib.stream_ptr(self.k.device)
+            part, counters, _keep = _lib.scratch(self.k.device, stream, 4 * need[0], need[1])
+            _lib.check(L.qi_cache_attention(
+                C.byref(d), q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPES[q.dtype], heads, rows.data_ptr(),
+                pos.data_ptr(), M, window, sinks, query_run, out.data_ptr(), part, need[0], counters, need[1],
+                self._errors().data_ptr(), stream), "qi_cache_attention")
+        return out
 
     # storage management hooks of the paged cache (every slot of a packed row exists)
     def reserve(self, row: int, length: int) -> None:
@@ -131,6 +256,19 @@ class PagedKVCache(KVCache):
                                         self.table.data_ptr(), self.page_size, self.pages_per_row, self.n_pages)
         return self._native
 
+    def _layer(self, i: int) -> _lib.QiKvLayer:
+        return _lib.QiKvLayer(self.k[i].data_ptr(), self.v[i].data_ptr(), None, None, _lib.QI_KV_BF16, 0,
+                              self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1],
+                              self.table.data_ptr(), self.page_size, self.pages_per_row, self.n_pages)
+
+    def attend(self, layer: int, q: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor, window: int = 0,
+               sinks: int = 0, query_run: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+        """KVCache.attend; page-table changes are published first (`sync`). A page that a
+        token sees but the table does not map is recorded for `check()` and counts as
+        zeros."""
+        self.sync()
+        return super().attend(layer, q, rows, pos, window, sinks, query_run, out)
+
     def reserve(self, row: int, length: int) -> None:
         if not 0 <= row < self.max_batch or not 0 <= length <= self.max_len:
             raise IndexError(f"row {row} / length {length} outside the cache")
@@ -176,6 +314,116 @@ class PagedKVCache(KVCache):
 
     def update(self, layer: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor):
         raise NotImplementedError("the paged cache is written by the forward's kernels only")
+
+
+class Kv8Cache(KVCache):
+    """K and V as 8-bit codes with block scales: `k`, `v` (layers, max_batch, kv_heads,
+    max_len, head_dim) int8 or float8_e4m3fn and `k_scale`, `v_scale` (layers, max_batch,
+    kv_heads, ceil(max_len / block_tokens)) fp32. The scale of a block of `block_tokens`
+    (16, 32, 64 or 128) positions of one row and head is the least power of two s with
+    127 s (int8) or 448 s (e4m3) >= all its values; the codes stand for code * s. `int8`
+    is the more exact on even-sized values (a step of at most amax / 63.5), `e4m3` keeps
+    small values next to large ones (relative steps of 2^-3).
+
+    `append` writes new tokens, `attend` reads them (KVCache.attend), `values` gives back
+    what the codes stand for."""
+
+    FORMATS = {"int8": (_lib.QI_KV_INT8, torch.int8), "e4m3": (_lib.QI_KV_E4M3, torch.float8_e4m3fn)}
+
+    def __init__(self, cfg: Qwen2Config, max_batch: int, max_len: int,
+                 dtype: torch.dtype = torch.float16, device: str | torch.device = "cuda",
+                 format: str = "int8", block_tokens: int = 32) -> None:
+        if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise ValueError(f"KV cache dtype must be bfloat16, float16 or float32; got {dtype}")
+        if format not in self.FORMATS:
+            raise ValueError(f"format must be one of {sorted(self.FORMATS)}; got {format!r}")
+        if block_tokens not in (16, 32, 64, 128):
+            raise ValueError(f"block_tokens must be 16, 32, 64 or 128; got {block_tokens}")
+        self.format, self.block_tokens = format, block_tokens
+        shape = (cfg.num_hidden_layers, max_batch, cfg.num_key_value_heads, max_len, cfg.head_dim)
+        blocks = shape[:3] + (-(-max_len // block_tokens),)
+        code = self.FORMATS[format][1]
+        self.k = torch.zeros(shape, dtype=torch.int8, device=device).view(code)
+        self.v = torch.zeros(shape, dtype=torch.int8, device=device).view(code)
+        self.k_scale = torch.zeros(blocks, dtype=torch.float32, device=device)
+        self.v_scale = torch.zeros(blocks, dtype=torch.float32, device=device)
+        self.max_batch = max_batch
+        self.max_len = max_len
+        self.window = 0
+        self.row_start = 0
+        self._native = None
+
+    def _layer(self, i: int) -> _lib.QiKvLayer:
+        return _lib.QiKvLayer(self.k[i].data_ptr(), self.v[i].data_ptr(), self.k_scale[i].data_ptr(),
+                              self.v_scale[i].data_ptr(), self.FORMATS[self.format][0], self.block_tokens,
+                              self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1], None, 0, 0, 0)
+
+    @torch.no_grad()
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor) -> None:
+        """Write M tokens' keys and values into layer `layer` (qi_kv8_append): token t at
+        position pos[t] of cache row rows[t]; pos[t] = -1 skips it.
+
+        k, v: (M, kv_heads, head_dim) of one dtype (float32, bfloat16 or float16), any
+        strides of the first two dimensions (slices of a fused projection's output will
+        do). A row grows from its end: the positions before the first appended one keep
+        their values (rounded again where their block's scale grows, at most one step of the
+        final scale in all), those after the last one of its block are dead, and a block whose
+        first position is appended starts over. The tokens may come in any order; of two with
+        the same row and position the later one is kept. A value that is not finite makes
+        its block's scale NaN, and so the outputs that read the block. rows and pos as in
+        `attend`."""
+        d = self.layer(layer)
+        self._operand("k", k, d.kv_heads)
+        self._operand("v", v, d.kv_heads)
+        if v.dtype != k.dtype or v.shape != k.shape:
+            raise ValueError(f"k and v must have one shape and dtype, got {tuple(k.shape)} {k.dtype} and "
+                             f"{tuple(v.shape)} {v.dtype}")
+        if d.head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {d.head_dim}")
+        M = k.shape[0]
+        rows, pos = self._tokens(M, rows, pos)
+        if M == 0:
+            return
+        with _lib.on_device(self.k.device):
+            _lib.check(_lib.lib().qi_kv8_append(
+                C.byref(d), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                _lib.DTYPES[k.dtype], rows.data_ptr(), pos.data_ptr(), M, self._errors().data_ptr(),
+                _lib.stream_ptr(self.k.device)), "qi_kv8_append")
+
+    @torch.no_grad()
+    def values(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """What layer `layer` stands for: K and V (max_batch, kv_heads, max_len, head_dim)
+        fp32 (qi_kv8_values). Dead positions give whatever their codes say."""
+        d = self.layer(layer)
+        _require(self.k_scale, "values", self.k.device)
+        if d.head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {d.head_dim}")
+        k = torch.empty(self.k.shape[1:], dtype=torch.float32, device=self.k.device)
+        v = torch.empty_like(k)
+        with _lib.on_device(self.k.device):
+            _lib.check(_lib.lib().qi_kv8_values(C.byref(d), k.data_ptr(), v.data_ptr(),
+                                                _lib.stream_ptr(self.k.device)), "qi_kv8_values")
+        return k, v
+
+    def native(self) -> _lib.QiCache:
+        raise NotImplementedError("the model's forward does not read an 8-bit cache yet")
+
+    def update(self, layer: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor):
+        raise NotImplementedError("the 8-bit cache is written by append")
+
+    def move_rows(self, moves: list[tuple[int, int, int]]) -> None:
+        """KVCache.move_rows: codes of positions [0, length) and the scales of their blocks."""
+        for src, dst, length in moves:
+            if not (0 <= src < self.max_batch and 0 <= dst < self.max_batch and 0 <= length <= self.max_len):
+                raise IndexError(f"row move {(src, dst, length)} outside the cache")
+            if src == dst or length == 0:
+                continue
+            blocks = -(-length // self.block_tokens)
+            for t, n in ((self.k, length), (self.v, length), (self.k_scale, blocks), (self.v_scale, blocks)):
+                t[:, dst, :, :n] = t[:, src, :, :n]
+
+    def memory_bytes(self) -> int:
+        return 2 * (self.k.numel() + 4 * self.k_scale.numel())
 
 
 def _single_layer_view(cache: KVCache, layer: int) -> tuple[torch.Tensor, torch.Tensor]:

@@ -1,0 +1,78 @@
+"""Log probabilities of tokens from a model's logits, with entropy and alternatives.
+
+The reference only takes the argmax of its logits (qweninfer/engine/engine.py:129,155);
+`token_logprobs` is what a caller needs to score given text or to report how sure a
+generated token was. One kernel (qi_token_logprobs) reads the logits once.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from qweninfer_b200 import _lib
+
+MAX_TOP = 32
+
+
+@dataclass
+class TokenLogprobs:
+    """`logprob`, `entropy` (M,) fp32; `top_ids` (M, top) int32 and `top_logprobs` (M, top)
+    fp32, largest first (None for top = 0). Natural logarithms."""
+    logprob: torch.Tensor | None
+    entropy: torch.Tensor
+    top_ids: torch.Tensor | None
+    top_logprobs: torch.Tensor | None
+
+
+@torch.no_grad()
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0) -> TokenLogprobs:
+    """Per row of `logits` (M, V) (float32, bfloat16 or float16; rows may be strided):
+    log softmax at targets[t], the entropy of the distribution, and its `top` (0..32, at
+    most V) largest entries, equal logits in the order of their index.
+
+    targets: (M,) int32 or int64 on the logits' device, or on the host, where they are
+    checked; a negative target has no log probability and gives 0, one outside the
+    vocabulary NaN. A logit of -inf has probability 0. A row with a NaN or +inf logit, or of
+    -inf alone, has NaN results. Exponentials and sums are fp32. Enqueued on the current
+    stream."""
+    if logits.device.type != "cuda":
+        raise _lib.QiError(f"token_logprobs: qweninfer_b200 computes on CUDA (sm_100) tensors only, got {logits.device}")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"logits must be (tokens, vocabulary), got {tuple(logits.shape)}")
+    if logits.dtype not in _lib.DTYPES:
+        raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    M, V = logits.shape
+    if logits.stride(1) != 1 or (M > 1 and logits.stride(0) < V):
+        raise ValueError("a row of logits must be contiguous and rows must not overlap")
+    if not 0 <= top <= min(MAX_TOP, V):
+        raise ValueError(f"top must be 0..{min(MAX_TOP, V)}, got {top}")
+    if targets is not None:
+        if targets.dim() != 1 or targets.shape[0] != M or targets.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"targets must be ({M},) int32 or int64, got {tuple(targets.shape)} {targets.dtype}")
+        if targets.device.type == "cpu":
+            if M and int(targets.max()) >= V:
+                raise IndexError("target outside the vocabulary")
+            targets = targets.to(logits.device)
+        elif targets.device != logits.device:
+            raise ValueError(f"targets on {targets.device}, logits on {logits.device}")
+        targets = targets.contiguous()
+    dev = logits.device
+    f32 = dict(dtype=torch.float32, device=dev)
+    r = TokenLogprobs(torch.empty(M, **f32) if targets is not None else None, torch.empty(M, **f32),
+                      torch.empty(M, top, dtype=torch.int32, device=dev) if top else None,
+                      torch.empty(M, top, **f32) if top else None)
+    if M == 0:
+        return r
+    with _lib.on_device(dev):
+        L = _lib.lib()
+        stream = _lib.stream_ptr(dev)
+        nbytes = L.qi_token_logprobs_scratch(M, V)
+        data, counters, _keep = _lib.scratch(dev, stream, nbytes, M if nbytes else 0)
+        _lib.check(L.qi_token_logprobs(
+            logits.data_ptr(), _lib.DTYPES[logits.dtype], logits.stride(0) if M > 1 else V, _lib.ptr(targets),
+            int(targets is not None and targets.dtype == torch.int64), M, V, top, _lib.ptr(r.logprob),
+            r.entropy.data_ptr(), _lib.ptr(r.top_ids), _lib.ptr(r.top_logprobs), data, nbytes, counters, stream),
+            "qi_token_logprobs")
+    return r
