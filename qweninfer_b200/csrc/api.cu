@@ -389,15 +389,6 @@ int grid_for(int n_tiles, int KB, int max_contrib) {
   return (int)(g < sms ? g : sms);
 }
 
-// Largest number of key splits of a cached-attention call that its scratch holds.
-int splits_within(const qi_kv_layer* c, int group, int M, int window, int sinks, long long part_floats,
-                  long long counters_len) {
-  const long long units = (long long)M * c->kv_heads;
-  int n = cache_attention_splits(M, c->kv_heads, c->max_len, window, sinks);
-  if (counters_len < units) return 1;
-  while (n > 1 && units * n * group * (c->head_dim + 2) > part_floats) --n;
-  return n;
-}
 bool bad_attention(const qi_kv_layer* c, int heads, int M, int window, int sinks, int query_run) {
   return bad_layer(c) || heads <= 0 || heads % c->kv_heads != 0 || heads / c->kv_heads > 8 || M <= 0 || window < 0 ||
          sinks < 0 || query_run < 0 || c->kv_heads > 65535 || (long long)M * kMaxAttnSplits > 0x7fffffffLL;
@@ -734,9 +725,9 @@ int qi_kv8_values(const qi_kv_layer* layer, float* k_out, float* v_out, qi_strea
 int qi_cache_attention_scratch(const qi_kv_layer* layer, int heads, int M, int window, int sinks, int query_run,
                                long long* part_floats, long long* counters_len) {
   if (bad_attention(layer, heads, M, window, sinks, query_run) || !part_floats || !counters_len) return QI_ERR_ARG;
-  const int n = cache_attention_splits(M, layer->kv_heads, layer->max_len, window, sinks);
-  *part_floats = n > 1 ? (long long)M * heads * n * (layer->head_dim + 2) : 0;
-  *counters_len = n > 1 ? (long long)M * layer->kv_heads : 0;
+  const CacheAttnPlan plan = cache_attention_plan(*layer, heads, M, window, sinks, query_run);
+  *part_floats = plan.part_floats;
+  *counters_len = plan.counters;
   return QI_OK;
 }
 
@@ -763,9 +754,10 @@ int qi_cache_attention(const qi_kv_layer* layer, const void* q, long long q_toke
   p.out = out;
   p.part = part;
   p.counters = counters;
-  p.splits = part && counters ? splits_within(layer, p.group, M, window, sinks, part_floats, counters_len) : 1;
   p.err = err;
-  return rc(launch_cache_attention(p, query_run, as_stream(stream), false));
+  CacheAttnPlan plan = cache_attention_plan(*layer, heads, M, window, sinks, query_run);
+  cache_attention_fit(plan, *layer, heads, M, part ? part_floats : 0, counters ? counters_len : 0);
+  return rc(launch_cache_attention(p, plan, as_stream(stream), false));
 }
 
 long long qi_token_logprobs_scratch(int M, int V) {

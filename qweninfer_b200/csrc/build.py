@@ -22,7 +22,7 @@ PKG = CSRC.parent
 REPO = PKG.parent
 LIB = PKG / "libqi.so"
 SOURCES = ["gemv.cu", "attention.cu", "attention_block.cu", "misc.cu", "norm_rope.cu", "tc_proj.cu", "kv8.cu",
-           "cache_attention.cu", "logprobs.cu", "api.cu"]
+           "cache_attention.cu", "cache_attention_prompt.cu", "logprobs.cu", "api.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -29,18 +29,18 @@
 // are loaded in the same order, which leaves the dot product unchanged. V goes through
 // ldmatrix.trans; for 8-bit codes its 16-bit elements are pairs of neighbouring dims, taken
 // apart into an even and an odd n-tile.
-#include "cache_attention.h"
-#include "cache_layer.cuh"
-#include "tc_proj.h"
+#include "cache_attention.cuh"
 
 namespace qi {
 
 namespace {
 
+using namespace cattn;
+
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kGran = 32;  // keys per granule
-constexpr int kMaxGroup = 8;
+constexpr int kPromptRows = 128, kPromptKeys = 128;  // cache_attention_prompt.cu's tiles
 
 template <int FMT, int D>
 struct Shape {
@@ -60,17 +60,6 @@ __device__ __forceinline__ int swizzle(int r, int c) {
   else return c ^ (((r & 1) << 2) | ((r >> 1) & 3));
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -100,102 +89,6 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// ---- parts of fp32 pairs as 16-bit pairs (a in the low half)
-__device__ __forceinline__ uint32_t f16x2(float a, float b) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
-}
-__device__ __forceinline__ uint32_t b16x2(float a, float b) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
-}
-// the 16-bit parts of (a, b): part 0 = round(x), each next part = round(rest)
-template <bool F16, int N>
-__device__ __forceinline__ void split(float a, float b, uint32_t (&r)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if constexpr (F16) {
-      r[i] = f16x2(a, b);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
-      a -= f.x, b -= f.y;
-    } else {
-      r[i] = b16x2(a, b);
-      a -= bf16lo(r[i]), b -= bf16hi(r[i]);
-    }
-  }
-}
-
-// ---- 8-bit codes as fp16 pairs. SEL 0: bytes 0, 1 and 2, 3 (K); SEL 1: bytes 0, 2 and 1, 3
-// (V, where a 16-bit element holds two neighbouring dims of one key). int8: the code plus
-// 128 as the low byte of 0x6400 is 1024 + 128 + code exactly; minus 1152.
-template <int FMT, int SEL>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& p0, uint32_t& p1) {
-  if constexpr (FMT == QI_KV_INT8) {
-    w ^= 0x80808080u;
-    const uint32_t a = __byte_perm(w, 0x64646464u, SEL ? 0x4240 : 0x4140);
-    const uint32_t b = __byte_perm(w, 0x64646464u, SEL ? 0x4341 : 0x4342);
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-    p0 = *reinterpret_cast<const uint32_t*>(&x);
-    p1 = *reinterpret_cast<const uint32_t*>(&y);
-  } else {
-    if constexpr (SEL) w = __byte_perm(w, 0u, 0x3120);
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(p0), "=r"(p1)
-        : "r"(w));
-  }
-}
-
-// Output values of features f .. f + N - 1 (N even, f a multiple of N) of a token.
-template <int N>
-__device__ __forceinline__ void emit(const CacheAttnParams& p, int tok, int f, int width, const float (&v)[N]) {
-  if (p.out) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) store_elem(p.out, p.dtype, (long long)tok * width + f + i, v[i]);
-  }
-  if (p.out_act) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint32_t hi = b16x2(v[i], v[i + 1]);
-      const uint32_t lo = b16x2(v[i] - bf16lo(hi), v[i + 1] - bf16hi(hi));
-      *reinterpret_cast<uint32_t*>(p.out_act + act_offset(tok, f + i, 0, width, p.out_nt)) = hi;
-      *reinterpret_cast<uint32_t*>(p.out_act + act_offset(tok, f + i, 1, width, p.out_nt)) = lo;
-    }
-  }
-}
-
-// The list of granules a token sees.
-struct Seen {
-  int p;      // its position
-  int lo;     // first position of the window
-  int sinks;  // visible first positions (0 when the window reaches position 0)
-  int ns;     // granules of the sinks, before the window's
-  int g0;     // first granule of the window
-  int n;      // granules in all
-  __device__ __forceinline__ int granule(int i) const { return i < ns ? i : g0 + i - ns; }
-  __device__ __forceinline__ bool sees(int j) const { return j <= p && (j >= lo || j < sinks); }
-};
-__device__ __forceinline__ Seen seen_keys(int p, int window, int sinks) {
-  Seen s;
-  s.p = p;
-  s.lo = window > 0 && p >= window ? p - window + 1 : 0;
-  s.sinks = min(sinks, s.lo);
-  s.g0 = s.lo / kGran;
-  s.ns = min((s.sinks + kGran - 1) / kGran, s.g0);
-  s.n = s.ns + p / kGran + 1 - s.g0;
-  return s;
-}
-
 // Granules a split has at least, so that its warps have two each.
 constexpr int kMinSplit = 2 * kWarps;
 
@@ -217,16 +110,20 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
   grid_dep_wait();
   grid_dep_launch();
   const int ps = p.pos[tok], row = p.rows[tok];
-  const bool ok = ps >= 0 && ps < c.max_len && row >= 0 && row < c.cache_rows;
-  if (!ok) {  // nothing seen: zeros; a position or row outside the cache is reported
-    if (split_i == 0) {
+  if (!token_ok(p, ps, row)) {  // nothing seen: zeros; a position or row outside the cache is reported
+    if (split_i == 0 && !p.only_single) {
       if (ps != -1 && tid == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
       const float z[2] = {0.f, 0.f};
       for (int e = tid; e < G * D / 2; e += kThreads) emit<2>(p, tok, g * G * D + 2 * e, width, z);
     }
     return;
   }
-  const Seen seen = seen_keys(ps, p.window, p.sinks);
+  if (p.only_single) {  // the tokens that the prompt kernel left out
+    const int n = kPromptRows / G, t = tok / n * n + tid;
+    const bool same = tid < n && t < p.M && p.rows[t] == row && token_ok(p, p.pos[t], row);
+    if (__syncthreads_count(same) != 1) return;
+  }
+  const Seen<kGran> seen = seen_range<kGran>(ps, window_start(ps, p.window), p.sinks);
   const int nsplit = min(p.splits, (seen.n + kMinSplit - 1) / kMinSplit);
   if (split_i >= nsplit) return;
   const int gbeg = (int)((long long)seen.n * split_i / nsplit), gend = (int)((long long)seen.n * (split_i + 1) / nsplit);
@@ -256,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
       if constexpr (F16) {
         if (lane < 4) {  // scales of the granule's halves: K, K, V, V
           const int h0 = k0 + 16 * (lane & 1);
-          const bool any = mapped && h0 <= seen.p && (h0 + 15 >= seen.lo || h0 < seen.sinks);
+          const bool any = mapped && seen.sees16(h0);
           const long long si = any ? scale_index(c, row, g, h0) : 0;
           cp4(dst + 2 * S::kTensor + 4 * lane, (lane < 2 ? c.k_scale : c.v_scale) + si, any ? 4u : 0u);
         }
@@ -443,27 +340,12 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
     if (qd == 0) w[D] = m, w[D + 1] = l;
   }
   __syncthreads();
-  // weighted sum over n partials (stride floats apart) of head h, dims d and d + 1
-  auto merge2 = [&](auto load, int n, int h, int d, float& m_out, float& l_out, float& a, float& b) {
-    float mx = -INFINITY;
-    for (int w = 0; w < n; ++w) mx = fmaxf(mx, load(w, h * kPart + D));
-    m_out = mx, l_out = 0.f, a = 0.f, b = 0.f;
-    for (int w = 0; w < n; ++w) {
-      const float mw = load(w, h * kPart + D);
-      // a partial without keys (maximum -inf) has nothing to add; a NaN stays one
-      const float f = mw == -INFINITY ? (load(w, h * kPart + D + 1) == 0.f ? 0.f : 1.f) : ex2(mw - mx);
-      l_out = fmaf(f, load(w, h * kPart + D + 1), l_out);
-      a = fmaf(f, load(w, h * kPart + d), a);
-      b = fmaf(f, load(w, h * kPart + d + 1), b);
-    }
-  };
   const long long unit = (long long)tok * c.kv_heads + g;
   float* part = p.part + (unit * p.splits + split_i) * (long long)(G * kPart);
-  auto from_smem = [&](int w, int i) { return wp[w * G * kPart + i]; };
-  for (int e = tid; e < G * D / 2; e += kThreads) {
+    for (int e = tid; e < G * D / 2; e += kThreads) {
     const int h = e / (D / 2), d = 2 * (e - h * (D / 2));
     float mm, ll, a, b;
-    merge2(from_smem, kWarps, h, d, mm, ll, a, b);
+    merge2<D>([&](int w, int i) { return wp[(w * G + h) * kPart + i]; }, kWarps, d, mm, ll, a, b);
     if (nsplit == 1) {
       const float inv = ll != 0.f ? 1.f / ll : 0.f;
       const float v[2] = {a * inv, b * inv};
@@ -480,11 +362,10 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
   __syncthreads();
   if (!last) return;
   const float* parts = p.part + unit * p.splits * (long long)(G * kPart);
-  auto from_part = [&](int w, int i) { return __ldcg(parts + (long long)w * (G * kPart) + i); };
-  for (int e = tid; e < G * D / 2; e += kThreads) {
+    for (int e = tid; e < G * D / 2; e += kThreads) {
     const int h = e / (D / 2), d = 2 * (e - h * (D / 2));
     float mm, ll, a, b;
-    merge2(from_part, nsplit, h, d, mm, ll, a, b);
+    merge2<D>([&](int w, int i) { return __ldcg(parts + ((long long)w * G + h) * kPart + i); }, nsplit, d, mm, ll, a, b);
     const float inv = ll != 0.f ? 1.f / ll : 0.f;
     const float v[2] = {a * inv, b * inv};
     emit<2>(p, tok, g * G * D + h * D + d, width, v);
@@ -521,23 +402,85 @@ cudaError_t launch_dim(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
 
 }  // namespace
 
-int cache_attention_splits(int M, int kv_heads, int max_len, int window, int sinks) {
-  long long keys = max_len;
-  if (window > 0 && (long long)window + sinks < keys) keys = (long long)window + sinks;
-  const long long gran = keys / kGran + 2;
-  const long long units = (long long)M * kv_heads;
-  const long long most = (gran + kMinSplit - 1) / kMinSplit;
-  long long want = (4LL * sm_count() + units - 1) / units;  // four CTAs per SM
-  if (want > most) want = most;
-  if (want > kMaxAttnSplits) want = kMaxAttnSplits;
-  return (int)(want < 1 ? 1 : want);
+namespace {
+
+constexpr int kMinTiles = 4;
+
+long long seen_at_most(const qi_kv_layer& c, int window, int sinks) {
+  const long long w = (long long)window + sinks;
+  return window > 0 && w < c.max_len ? w : c.max_len;
 }
 
-cudaError_t launch_cache_attention(const CacheAttnParams& args, int query_run, cudaStream_t s, bool pdl) {
-  (void)query_run;
+// Key splits of the per-token kernel: four CTAs for every SM, as far as rows are long
+// enough to give each split kMinSplit granules.
+int token_splits(const qi_kv_layer& c, int M, int window, int sinks) {
+  const long long gran = seen_at_most(c, window, sinks) / kGran + 2, units = (long long)M * c.kv_heads;
+  const long long most = (gran + kMinSplit - 1) / kMinSplit;
+  long long want = (4LL * sm_count() + units - 1) / units;
+  want = want > most ? most : want;
+  return (int)(want > kMaxAttnSplits ? kMaxAttnSplits : want < 1 ? 1 : want);
+}
+
+// Key splits of the prompt kernel: as many as fill the CTAs that are resident at once.
+int prompt_splits(const qi_kv_layer& c, int tiles, int window, int sinks) {
+  const long long slots = (c.head_dim == 64 ? 2LL : 1LL) * sm_count();
+  const long long n = slots / ((long long)tiles * c.kv_heads);
+  const long long most = (seen_at_most(c, window, sinks) / kPromptKeys + 2) / kMinTiles;
+  const long long want = n < most ? n : most;
+  return (int)(want > kMaxAttnSplits ? kMaxAttnSplits : want < 1 ? 1 : want);
+}
+
+int prompt_tiles(int M, int group) { return (M + kPromptRows / group - 1) / (kPromptRows / group); }
+
+void sizes(CacheAttnPlan& r, const qi_kv_layer& c, int heads, int M) {
+  r.part_floats = r.counters = 0;
+  if (r.prompt && r.splits > 1) {
+    const long long units = (long long)prompt_tiles(M, heads / c.kv_heads) * c.kv_heads;
+    r.part_floats = units * r.splits * kPromptRows * (c.head_dim + 2);
+    r.counters = units;
+  }
+  if ((!r.prompt || r.singles) && r.token_splits > 1) {
+    const long long f = (long long)M * heads * r.token_splits * (c.head_dim + 2), n = (long long)M * c.kv_heads;
+    r.part_floats = f > r.part_floats ? f : r.part_floats;
+    r.counters = n > r.counters ? n : r.counters;
+  }
+}
+
+}  // namespace
+
+CacheAttnPlan cache_attention_plan(const qi_kv_layer& c, int heads, int M, int window, int sinks, int query_run) {
+  CacheAttnPlan r = {};
+  r.prompt = query_run > 0 ? query_run >= 16 : M > 128;
+  r.singles = r.prompt && query_run != M;
+  r.splits = r.prompt ? prompt_splits(c, prompt_tiles(M, heads / c.kv_heads), window, sinks) : 1;
+  r.token_splits = token_splits(c, M, window, sinks);
+  sizes(r, c, heads, M);
+  return r;
+}
+
+void cache_attention_fit(CacheAttnPlan& r, const qi_kv_layer& c, int heads, int M, long long part_floats,
+                         long long counters) {
+  while (r.part_floats > part_floats || r.counters > counters) {
+    if (r.splits > 1) --r.splits;
+    if (r.token_splits > 1) --r.token_splits;
+    sizes(r, c, heads, M);
+  }
+}
+
+cudaError_t launch_cache_attention(const CacheAttnParams& args, const CacheAttnPlan& plan, cudaStream_t s, bool pdl) {
   CacheAttnParams p = args;
   p.scale_log2 = 1.4426950408889634f / sqrtf((float)p.c.head_dim);
-  p.q_vec = p.dtype == QI_F32 && ((uintptr_t)p.q & 15) == 0 && (p.q_st & 3) == 0 && (p.q_sh & 3) == 0;
+  const int per = p.dtype == QI_F32 ? 4 : 8;
+  p.q_vec = ((uintptr_t)p.q & 15) == 0 && p.q_st % per == 0 && p.q_sh % per == 0;
+  if (plan.prompt) {
+    p.min_tiles = kMinTiles;
+    p.splits = plan.splits;
+    p.skip_single = plan.singles;
+    const cudaError_t e = launch_cache_attention_prompt(p, s, pdl);
+    if (e != cudaSuccess || !plan.singles) return e;
+    p.only_single = 1;
+  }
+  p.splits = plan.token_splits;
   return p.c.head_dim == 64 ? launch_dim<64>(p, s, pdl) : launch_dim<128>(p, s, pdl);
 }
 

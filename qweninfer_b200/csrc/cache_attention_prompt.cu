@@ -1,0 +1,848 @@
+// Attention over one cache layer for prompts: tiles of consecutive query tokens share their
+// keys on the 5th-generation tensor cores (the formula is in cache_attention.cu).
+//
+// A CTA takes the query rows of 128 / group consecutive tokens and one KV head (row = token
+// x head of the group) and a share of the 128-key tiles that any of them sees:
+//   S = Q K^T     M 128 x N 128 x K D, fp32 in TMEM; Q in shared memory
+//   T = P V       M 128 x N D x K 128, fp32 in TMEM; P in TMEM, where it takes the place of S
+// Threads r and r + 128 of the softmax warps share query row r (TMEM lane r), 64 keys and
+// half of the output dims each: two passes over their scores (maximum, then exponentials),
+// and O += T of the tile before in registers: the tensor cores' own accumulation truncates,
+// so it stays within a tile and sums over tiles are rounded fp32 additions. The passes are
+// chains of dependent instructions; two threads a row and two CTAs an SM hide each other's
+// latencies. Four producer warps bring keys and values into
+// the K-major layout of UMMA descriptors as fp16; V in the same layout is the MN-major
+// operand of the second product, so nothing is transposed. One warp issues the MMAs. Two
+// CTAs share an SM at head_dim 64: one's softmax runs during the other's products.
+//
+// Every format is multiplied in fp16 with a scale for 16 keys: 8-bit codes are exact and
+// have their block's scale; bf16 values get a power of two that puts the largest of 16 keys
+// in [2^14, 2^15), which leaves all within 2^-28 of it exact and errors of 2^-40 of it
+// otherwise. q is scaled per row to a maximum in [1, 2). fp32 callers: q and p in two fp16
+// parts (22 bits), each part one UMMA chain into the same accumulator, the small ones first.
+// 16-bit callers: one part, exact for q (to 2^-25 of the row's largest) and good to 2^-12 for
+// p, below the output's own rounding.
+//
+// The K scale multiplies scores, the V scale of a block its probabilities: P holds 2^(x_j +
+// log2 s_j - R + 14), where R is the largest x + log2 s of the row in the tile, so that what
+// counts uses fp16's range whatever the scales are; T is brought back to the running maximum
+// of the softmax when it is added to O.
+//
+// Tokens of several cache rows in one tile are segments, worked off one after another with
+// the other rows masked. Tokens alone in their tile's segment (a batched prefill's last
+// tokens) are left to the per-token kernel in a second launch.
+//
+// What masked keys hold must not reach a row. Scores are replaced, keys that no row of the
+// tile sees are zero-filled; but in P V a zero weight times a NaN or infinity that another
+// row does see would be NaN. A row that ends up not finite is therefore computed again, key
+// by key (8-bit codes are always finite: only the bf16 cache needs it).
+#include "cache_attention.cuh"
+#include "tc_device.cuh"
+
+namespace qi {
+
+namespace {
+
+using namespace cattn;
+using namespace tc;
+
+constexpr int kRows = 128;   // query rows of a tile
+constexpr int kKeys = 128;   // keys of a tile
+// warpgroups: two of softmax, producers, and one whose first warp issues the MMAs
+constexpr int kSoftWarps = 8, kLoadWarp = 8, kLoadWarps = 4, kMmaWarp = 12;
+constexpr int kThreads = 512;
+constexpr int kLoadThreads = 32 * kLoadWarps;
+constexpr float kLift = 14.f;
+constexpr unsigned kAll = 0xffffffffu;
+
+struct True {
+  static constexpr bool value = true;
+};
+struct False {
+  static constexpr bool value = false;
+};
+
+template <int FMT, int D, int PARTS>
+struct Shape {
+  static constexpr uint32_t kQ = kRows * D * 2;   // one part of Q
+  static constexpr uint32_t kT = kKeys * D * 2;   // K or V tile
+  static constexpr uint32_t kOffK = PARTS * kQ, kOffV = kOffK + 2 * kT, kOffMisc = kOffV + 2 * kT;
+  static constexpr uint32_t kColT = 128, kCols = 256;  // TMEM: S (P in its place), T
+  // Registers of a thread: of the launch, and of the warpgroups, which together have no more.
+  static constexpr int kCtas = D == 64 ? 2 : 1;
+  static constexpr int kRegLaunch = D == 64 ? 64 : 128;
+  static constexpr int kRegSoft = D == 64 ? 80 : 152, kRegLoad = D == 64 ? 64 : 160, kRegMma = D == 64 ? 32 : 48;
+  static_assert(2 * kRegSoft + kRegLoad + kRegMma <= 4 * kRegLaunch, "the increase must be covered");
+};
+
+// the part of a tile's tokens that lies in one cache row
+struct Seg {
+  int row, lo, hi, sinks, first;  // positions lo..hi and 0..sinks-1 seen; first tile in the list
+};
+
+struct Misc {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, p_full, t_full;
+  uint32_t tmem;
+  int nseg, ntiles, last;
+  int abort;  // a wait of this CTA gave up: the others do not wait any more
+  int pos[kRows], row[kRows], seg[kRows];  // per token
+  Seg segs[kRows];
+  float scale[2][2][8];                    // [stage][K, V][16 keys]
+  float2 pair[2][kRows];                   // what the two threads of a row tell each other
+};
+constexpr uint32_t kMiscBytes = (sizeof(Misc) + 15) / 16 * 16;
+
+__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46);
+}
+// kind::f16 instruction: fp16 operands, fp32 accumulator; bit 16: B is MN-major
+__device__ __forceinline__ uint32_t idesc_f16(bool b_mn, int N) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+// One UMMA, issued by the lane whose `lead` is not 0. Executed by the whole warp, so that
+// descriptors and addresses stay in uniform registers. A in shared memory, or (ts) in TMEM.
+__device__ __forceinline__ void umma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+// 16 columns of this thread's lane, asynchronously: valid after tmem_ready on them
+__device__ __forceinline__ void tmem_get16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// every load so far is complete; the registers pass through so that no use moves before it
+__device__ __forceinline__ void tmem_ready(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+// f(j, columns 16 j .. 16 j + 15) for j < N, the next load under way meanwhile
+template <int N, class F>
+__device__ __forceinline__ void tmem_each16(uint32_t taddr, F f) {
+  uint32_t r[2][16];
+  tmem_get16(taddr, r[0]);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    tmem_ready(r[j & 1]);
+    if (j + 1 < N) tmem_get16(taddr + 16 * (j + 1), r[(j + 1) & 1]);
+    f(j, r[j & 1]);
+  }
+}
+__device__ __forceinline__ void tmem_put8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- pairs of fp32 values in 64 bits: one instruction for two operations
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(f2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// byte offset of (row r, 8-element chunk c) of an operand with D elements a row: 8x8 core
+// matrices of 128 bytes, chunks 128 bytes apart, groups of 8 rows D * 16
+template <int D>
+__device__ __forceinline__ uint32_t core(int r, int c) {
+  return (uint32_t)((r >> 3) * (D * 16) + c * 128 + (r & 7) * 16);
+}
+
+// Bounded wait (mbar_wait) that ends at once when another wait of the CTA has given up.
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, Misc& X, int* err) {
+  if (mbar_try_wait(bar, parity)) return;
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*reinterpret_cast<volatile int*>(&X.abort)) return;
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      *reinterpret_cast<volatile int*>(&X.abort) = 1;
+      if (err) atomicExch(err, QI_ERR_TIMEOUT);
+      return;
+    }
+  }
+}
+
+// 8 consecutive elements of a query row as fp32
+__device__ __forceinline__ void load_q8(const CacheAttnParams& p, long long o, float (&x)[8]) {
+  if (p.q_vec) {
+    if (p.dtype == QI_F32) {
+      const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + o);
+      const float4 a = __ldcg(f), b = __ldcg(f + 1);
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + o));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (p.dtype == QI_BF16) {
+          x[2 * i] = bf16lo(w[i]), x[2 * i + 1] = bf16hi(w[i]);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] = p.dtype == QI_F32    ? load_elem<QI_F32>(p.q, o + i)
+             : p.dtype == QI_BF16 ? load_elem<QI_BF16>(p.q, o + i)
+                                  : load_elem<QI_F16>(p.q, o + i);
+  }
+}
+
+// Key by key: the partial of token t's head over the given tiles of its segment (bf16
+// layers), dims d0 .. d0 + D / 2 - 1 of the output. The weights of masked keys are left out, not multiplied by zero.
+template <int D>
+__device__ __noinline__ void plain_row(const CacheAttnParams& p, const Seg& sg, int tbeg, int tend, int tok, int head, int g,
+                                       int ps, int d0, float& m, float& l, float* o) {
+  const Seen<kKeys> list = seen_range<kKeys>(sg.hi, sg.lo, sg.sinks);
+  const Seen<kKeys> mine = seen_range<kKeys>(ps, window_start(ps, p.window), p.sinks);
+  const long long qo = (long long)tok * p.q_st + (long long)head * p.q_sh;
+  m = -INFINITY, l = 0.f;
+  for (int d = 0; d < D / 2; ++d) o[d] = 0.f;
+  for (int i = tbeg; i < tend; ++i) {
+    const int k0 = list.granule(i) * kKeys;
+    const long long base = layer_offset(p.c, D, sg.row, g, k0);
+    for (int j = 0; j < kKeys; ++j) {
+      if (!mine.sees(k0 + j)) continue;
+      float s = 0.f;
+      const uint16_t* k = static_cast<const uint16_t*>(p.c.k) + (base < 0 ? 0 : base) + j * D;
+      const uint16_t* v = static_cast<const uint16_t*>(p.c.v) + (base < 0 ? 0 : base) + j * D;
+      if (base >= 0)
+        for (int d = 0; d < D; d += 8) {
+          float x[8];
+          load_q8(p, qo + d, x);
+          for (int e = 0; e < 8; ++e) s = fmaf(x[e], bf16_to_f32(k[d + e]), s);
+        }
+      s *= p.scale_log2;
+      if (s > m) {
+        const float a = m == -INFINITY ? 0.f : ex2(m - s);
+        l *= a;
+        for (int d = 0; d < D / 2; ++d) o[d] *= a;
+        m = s;
+      }
+      const float w = ex2(s - (m == -INFINITY ? 0.f : m));
+      l += w;
+      if (base >= 0)
+        for (int d = 0; d < D / 2; ++d) o[d] = fmaf(w, bf16_to_f32(v[d0 + d]), o[d]);
+    }
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void more_regs() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_regs() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int FMT, int D, int PARTS>
+__global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_kernel(const CacheAttnParams p) {
+  using H = Shape<FMT, D, PARTS>;
+  constexpr bool BF = FMT == QI_KV_BF16;
+  constexpr int kPart = D + 2;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Misc& X = *reinterpret_cast<Misc*>(smem + H::kOffMisc);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const qi_kv_layer& c = p.c;
+  const int G = p.group, TT = kRows / G, width = p.heads * D;
+  const int tiles_m = (p.M + TT - 1) / TT;
+  // the last tokens see most: they start first
+  const int split_i = blockIdx.x % p.splits, tile = tiles_m - 1 - (int)(blockIdx.x / p.splits), g = blockIdx.y;
+  const int t0 = tile * TT, ntok = min(TT, p.M - t0);
+
+  grid_dep_wait();
+  if (warp == kMmaWarp) {
+    tmem_alloc(&X.tmem, H::kCols);
+    tmem_relinquish();
+  }
+  grid_dep_launch();
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&X.k_full[s], kLoadWarps);
+      mbar_init(&X.v_full[s], kLoadWarps);
+      mbar_init(&X.k_empty[s], 1);
+      mbar_init(&X.v_empty[s], 1);
+    }
+    mbar_init(&X.s_full, 1);
+    mbar_init(&X.p_full, kSoftWarps);
+    mbar_init(&X.t_full, 1);
+    X.abort = 0;
+    fence_barrier_init();
+  }
+  if (tid < kRows) {
+    int ps = -1, rw = -1;
+    if (tid < ntok) {
+      ps = p.pos[t0 + tid], rw = p.rows[t0 + tid];
+      if (!token_ok(p, ps, rw)) {
+        if (ps != -1 && g == 0 && split_i == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
+        ps = -1;
+      }
+    }
+    X.pos[tid] = ps;
+    X.row[tid] = rw;
+  }
+  __syncthreads();
+  // segments: the first token of each cache row gathers what its tokens see
+  if (tid < kRows) {
+    int first = -1;
+    Seg s = {0, 0x7fffffff, -1, 0, 0};
+    if (X.pos[tid] >= 0) {
+      int n = 0;
+      for (int i = 0; i < ntok; ++i) {
+        if (X.pos[i] < 0 || X.row[i] != X.row[tid]) continue;
+        if (first < 0) first = i;
+        if (first != tid) break;
+        const int ps = X.pos[i], lo = window_start(ps, p.window);
+        ++n;
+        s.lo = min(s.lo, lo);
+        s.hi = max(s.hi, ps);
+        s.sinks = max(s.sinks, min(p.sinks, lo));
+      }
+      s.row = X.row[tid];
+      if (p.skip_single && first == tid && n == 1) s.hi = -1;  // left to the per-token kernel
+    }
+    X.seg[tid] = first;
+    X.segs[tid] = s;
+  }
+  __syncthreads();
+  if (tid == 0) {  // the list of key tiles: segment after segment
+    int n = 0, t = 0;
+    for (int i = 0; i < ntok; ++i) {
+      if (X.seg[i] != i || X.segs[i].hi < 0) continue;
+      Seg s = X.segs[i];
+      s.first = t;
+      t += seen_range<kKeys>(s.hi, s.lo, s.sinks).n;
+      // compacted in place: the segments before it are at places up to i
+      X.segs[n++] = s;
+    }
+    X.nseg = n;
+    X.ntiles = t;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = X.tmem;
+  const int nsplit = max(1, min(p.splits, X.ntiles / p.min_tiles));
+  const bool work = split_i < nsplit;
+  const int tbeg = work ? (int)((long long)X.ntiles * split_i / nsplit) : 0;
+  const int tend = work ? (int)((long long)X.ntiles * (split_i + 1) / nsplit) : 0;
+  const int n = tend - tbeg;
+  if (warp >= kMmaWarp) {
+    // ------------------------------------------------------------------- MMA
+    fewer_regs<H::kRegMma>();
+    if (warp == kMmaWarp) {
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");  // Q is in place
+      const uint32_t sb = smem_u32(smem), lead = lane == 0;
+      const uint32_t id_s = idesc_f16(false, kKeys), id_t = idesc_f16(true, D);
+      const uint64_t qd = desc(sb, 128, D * 16);
+      for (int i = 0; i < n; ++i) {
+        const int st = i & 1;
+        const uint32_t ph = (uint32_t)(i >> 1) & 1u;
+        wait(&X.k_full[st], ph, X, p.err);
+        tc_fence_after();
+        // S(i) takes the place of P(i - 1): the product that reads it was issued before
+        const uint64_t kd = desc(sb + H::kOffK + st * H::kT, 128, D * 16);
+#pragma unroll
+        for (int q = PARTS - 1; q >= 0; --q)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_ss(lead, tmem, qd + (uint64_t)(q * (H::kQ >> 4) + k * 16), kd + (uint64_t)(k * 16), id_s,
+                    q < PARTS - 1 || k > 0 ? 1u : 0u);
+        commit(lead, &X.s_full);
+        commit(lead, &X.k_empty[st]);
+        const uint64_t vd = desc(sb + H::kOffV + st * H::kT, D * 16, 128);
+        wait(&X.v_full[st], ph, X, p.err);
+        wait(&X.p_full, (uint32_t)i & 1u, X, p.err);
+        tc_fence_after();
+#pragma unroll
+        for (int q = PARTS - 1; q >= 0; --q)
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            // 16 keys: 8 columns of P for each part; 2 key groups of V
+            umma_ts(lead, tmem + H::kColT, tmem + 16 * k + 8 * q, vd + (uint64_t)(k * 2 * D), id_t,
+                    q < PARTS - 1 || k > 0 ? 1u : 0u);
+        commit(lead, &X.v_empty[st]);
+      }
+      commit(lead, &X.t_full);
+      __syncwarp();
+    }
+    __syncthreads();
+  } else if (warp >= kLoadWarp) {
+    // ------------------------------------------------------------- producers
+    if constexpr (H::kRegLoad > H::kRegLaunch) more_regs<H::kRegLoad>();
+    else fewer_regs<H::kRegLoad>();
+    const int lt = tid - 32 * kLoadWarp, lw = warp - kLoadWarp;
+    constexpr int kCh = D * (BF ? 2 : 1) / 16;        // 16-byte chunks of a key
+    constexpr int kN = kKeys * kCh / kLoadThreads;    // of a thread
+    // a warp takes 32 keys; one of its loads is 8 keys x 4 chunks: whole lines, and the
+    // lanes of a store phase hold 8 keys
+    auto place = [&](int j, int& r, int& ch) {
+      r = lw * 32 + (j / (kCh / 4)) * 8 + (lane & 7);
+      ch = (j % (kCh / 4)) * 4 + (lane >> 3);
+    };
+    uint4 kr[kN], vr[BF ? 1 : kN];  // bf16: V follows K in the same registers
+    float sc = 1.f;
+    int si = 0;  // segment of the tile at hand (entries come in order)
+    auto fetch = [&](int i, bool k_side) {
+      while (si + 1 < X.nseg && i >= X.segs[si + 1].first) ++si;
+      const Seg& sg = X.segs[si];
+      const Seen<kKeys> list = seen_range<kKeys>(sg.hi, sg.lo, sg.sinks);
+      const int k0 = list.granule(i - sg.first) * kKeys;
+      const long long o = layer_offset(c, D, sg.row, g, k0);
+      if (o < 0 && lt == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
+      const long long base = (o < 0 ? 0 : o) * (BF ? 2 : 1);
+      const uint8_t* kb = static_cast<const uint8_t*>(c.k) + base;
+      const uint8_t* vb = static_cast<const uint8_t*>(c.v) + base;
+      const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        int r, ch;
+        place(j, r, ch);
+        const bool in = o >= 0 && list.sees(k0 + r);
+        const int x = (r * kCh + ch) * 16;
+        if constexpr (BF) {
+          kr[j] = in ? __ldcg(reinterpret_cast<const uint4*>((k_side ? kb : vb) + x)) : z;
+        } else {
+          kr[j] = in ? __ldcg(reinterpret_cast<const uint4*>(kb + x)) : z;
+          vr[j] = in ? __ldcg(reinterpret_cast<const uint4*>(vb + x)) : z;
+        }
+      }
+      if constexpr (!BF) {
+        if (lt < 16) {
+          const int h0 = k0 + 16 * (lt & 7);
+          const bool any = o >= 0 && list.sees16(h0);
+          sc = any ? __ldg((lt < 8 ? c.k_scale : c.v_scale) + scale_index(c, sg.row, g, h0)) : 1.f;
+        }
+      }
+    };
+    // 8-bit codes in registers -> fp16 operand rows
+    auto store8 = [&](const uint4* regs, uint8_t* t) {
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        int r, ch;
+        place(j, r, ch);
+        const uint32_t w[4] = {regs[j].x, regs[j].y, regs[j].z, regs[j].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) widen<BF ? QI_KV_INT8 : FMT, 0>(w[e], h[2 * e], h[2 * e + 1]);
+        *reinterpret_cast<uint4*>(t + core<D>(r, 2 * ch)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(t + core<D>(r, 2 * ch + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+      }
+    };
+    // bf16 values -> fp16 operand rows, and the scales of the warp's two blocks of 16 keys
+    auto store16 = [&](const uint4* regs, uint8_t* t, float* scales) {
+      constexpr int kB = kN / 2;  // chunks of a block
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t mx = 0u;
+#pragma unroll
+        for (int j = b * kB; j < (b + 1) * kB; ++j) {
+          const uint32_t w[4] = {regs[j].x, regs[j].y, regs[j].z, regs[j].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            mx = max(mx, max((w[e] << 16) & 0x7fff0000u, w[e] & 0x7fff0000u));
+        }
+        mx = __reduce_max_sync(kAll, mx);
+        if (mx >= 0x7f800000u) {  // the largest of the finite values
+          mx = 0u;
+#pragma unroll
+          for (int j = b * kB; j < (b + 1) * kB; ++j) {
+            const uint32_t w[4] = {regs[j].x, regs[j].y, regs[j].z, regs[j].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t lo = (w[e] << 16) & 0x7fff0000u, hi = w[e] & 0x7fff0000u;
+              mx = max(mx, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+            }
+          }
+          mx = __reduce_max_sync(kAll, mx);
+        }
+        // largest value 2^(e - 127) * [1, 2): scale 2^(e - 127 - 14), for e in 15..253 (the
+        // scale and its reciprocal are normal); tiny blocks are left with a smaller maximum
+        const uint32_t e = min(max(mx >> 23, 15u), 253u);
+        const float inv = __uint_as_float((268u - e) << 23);
+        if (lane == 0) scales[lw * 2 + b] = __uint_as_float((e - 14u) << 23);
+#pragma unroll
+        for (int j = b * kB; j < (b + 1) * kB; ++j) {
+          int r, ch;
+          place(j, r, ch);
+          const uint32_t w[4] = {regs[j].x, regs[j].y, regs[j].z, regs[j].w};
+          uint32_t h[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) h[x] = f16x2(bf16lo(w[x]) * inv, bf16hi(w[x]) * inv);
+          *reinterpret_cast<uint4*>(t + core<D>(r, ch)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+      }
+    };
+    auto publish = [&](uint64_t* bar) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    if (n > 0) fetch(tbeg, true);
+    for (int i = 0; i < n; ++i) {
+      const int st = i & 1;
+      const uint32_t ph = (uint32_t)((i >> 1) - 1) & 1u;
+      uint8_t* kt = smem + H::kOffK + st * H::kT;
+      uint8_t* vt = smem + H::kOffV + st * H::kT;
+      if (i >= 2) {  // tile i - 2 is done with: its products, and its scales
+        wait(&X.k_empty[st], ph, X, p.err);
+        wait(&X.v_empty[st], ph, X, p.err);
+      }
+      if constexpr (BF) {
+        store16(kr, kt, X.scale[st][0]);
+        publish(&X.k_full[st]);
+        fetch(tbeg + i, false);
+        store16(kr, vt, X.scale[st][1]);
+        publish(&X.v_full[st]);
+      } else {
+        if (lt < 16) X.scale[st][lt >> 3][lt & 7] = sc;
+        store8(kr, kt);
+        publish(&X.k_full[st]);
+        store8(vr, vt);
+        publish(&X.v_full[st]);
+      }
+      if (i + 1 < n) fetch(tbeg + i + 1, true);
+    }
+    __syncthreads();
+  } else {
+    // --------------------------------------------------------------- softmax
+    more_regs<H::kRegSoft>();
+    constexpr int DH = D / 2;
+    const int r = tid & (kRows - 1), hf = tid >> 7;  // row; 64 keys and DH dims of the two halves
+    const int tl = r / G, head = g * G + r - tl * G;
+    auto pair_bar = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };
+    const int ps = tl < ntok ? X.pos[tl] : -1;
+    // the row's segment, by cache row (segments left out have no entry)
+    int seg = -1;
+    for (int s = 0; s < X.nseg && ps >= 0; ++s)
+      if (X.segs[s].row == X.row[tl]) seg = s;
+    const bool live = ps >= 0 && seg >= 0;
+    float qs = p.scale_log2;
+    {
+      float am = 0.f;
+      const long long qo = (long long)(t0 + (live ? tl : 0)) * p.q_st + (long long)(live ? head : 0) * p.q_sh;
+#pragma unroll 2
+      for (int ch = 0; ch < D / 8; ++ch) {
+        float x[8];
+        if (live) load_q8(p, qo + 8 * ch, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) am = live ? fmaxf(am, fabsf(x[e])) : 0.f;
+      }
+      float inv = 1.f;
+      const uint32_t e = __float_as_uint(am) >> 23;
+      if (e > 0 && e < 253) {
+        inv = __uint_as_float((254u - e) << 23);
+        qs *= __uint_as_float(e << 23);
+      }
+#pragma unroll 2
+      for (int ch = hf * (DH / 8); ch < (hf + 1) * (DH / 8); ++ch) {
+        float x[8];
+        if (live) load_q8(p, qo + 8 * ch, x);
+        uint32_t w[4][PARTS];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          split<true, PARTS>(live ? x[2 * i] * inv : 0.f, live ? x[2 * i + 1] * inv : 0.f, w[i]);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+          *reinterpret_cast<uint4*>(smem + q * H::kQ + core<D>(r, ch)) = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+      }
+      fence_async_smem();
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");
+    const Seen<kKeys> mine = seen_range<kKeys>(live ? ps : 0, live ? window_start(ps, p.window) : 0, p.sinks);
+    const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+
+    float m = -INFINITY, l = 0.f;  // maximum of the scores (log2 units), sum of 2^(x - m)
+    f2 o[DH / 2];                  // sum of 2^(x - m) v (this half's dims; l: this half's keys)
+#pragma unroll
+    for (int d = 0; d < DH / 2; ++d) o[d] = 0ull;
+    // the last tile: O = O * oa + T * ob
+    float oa = 1.f, ob = 0.f;
+    auto add_tile = [&] {
+      if (__any_sync(kAll, oa != 1.f)) {
+        const f2 f = pack2(oa, oa);
+#pragma unroll
+        for (int d = 0; d < DH / 2; ++d) o[d] = mul2(o[d], f);
+      }
+      const f2 f = pack2(ob, ob);
+      tmem_each16<DH / 16>(trow + H::kColT + hf * DH, [&](int c, const uint32_t(&t)[16]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          o[8 * c + j] = fma2(pack2(__uint_as_float(t[2 * j]), __uint_as_float(t[2 * j + 1])), f, o[8 * c + j]);
+      });
+    };
+    int si = 0;
+    for (int i = 0; i < n; ++i) {
+      const int at = tbeg + i, st = i & 1;
+      while (si + 1 < X.nseg && at >= X.segs[si + 1].first) ++si;
+      const Seen<kKeys> list = seen_range<kKeys>(X.segs[si].hi, X.segs[si].lo, X.segs[si].sinks);
+      const int k0 = list.granule(at - X.segs[si].first) * kKeys;
+      // the row's keys of this tile: [a, b] and [0, s0)
+      const int b = live && seg == si ? min(mine.p - k0, kKeys - 1) : -1;
+      const int a = mine.lo - k0, s0 = min(mine.sinks - k0, b + 1);
+      // (what rows without a token do is not used)
+      const bool whole = !live || (b == kKeys - 1 && (a <= 0 || s0 >= kKeys));
+      const bool masked = __any_sync(kAll, !whole);
+      auto mask16 = [&](int c0) -> uint32_t {  // bit j < 16: key c0 + j is seen
+        auto below = [](int x) { return x <= 0 ? 0u : x >= 16 ? 0xffffu : (1u << x) - 1u; };
+        return (below(b + 1 - c0) & ~below(a - c0)) | below(s0 - c0);
+      };
+      wait(&X.k_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);  // the scales
+      wait(&X.v_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);
+      wait(&X.s_full, (uint32_t)i & 1u, X, p.err);  // S(i), and T(i - 1) before it
+      tc_fence_after();
+      if (i > 0) add_tile();
+      const float* ks = X.scale[st][0] + 4 * hf;
+      const float* vs = X.scale[st][1] + 4 * hf;
+      const uint32_t tcol = trow + 64 * hf;  // this half's scores
+      // pass 1: the maxima of the scores and of score + log2(V scale)
+      float mx = -INFINITY, R = -INFINITY;
+      auto maxima = [&](auto some_masked) {
+        tmem_each16<4>(tcol, [&](int c, const uint32_t(&s)[16]) {
+          float v = -INFINITY;
+          if constexpr (decltype(some_masked)::value) {
+            const uint32_t mk = mask16(64 * hf + 16 * c);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v = fmaxf(v, (mk >> j) & 1u ? __uint_as_float(s[j]) : -INFINITY);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v = fmaxf(v, __uint_as_float(s[j]));
+          }
+          // a block without seen keys has no say; its scale may be anything
+          v = v == -INFINITY ? v : v * (qs * ks[c]);
+          const uint32_t ev = __float_as_uint(vs[c]) >> 23;
+          R = fmaxf(R, v + (ev < 255u ? (float)ev - 127.f : 0.f));
+          mx = fmaxf(mx, v);
+        });
+      };
+      if (masked) maxima(True{});
+      else maxima(False{});
+      X.pair[hf][r] = make_float2(mx, R);
+      pair_bar();  // (the next tile's values are written after both halves' weights of this one)
+      const float2 other = X.pair[hf ^ 1][r];
+      R = fmaxf(R, other.y);
+      const float mn = fmaxf(m, fmaxf(mx, other.x));
+      oa = m == -INFINITY ? 1.f : ex2(m - mn);  // nothing summed yet: nothing to rescale
+      l *= oa;
+      m = mn;
+      const float mr = m == -INFINITY ? 0.f : m, Rr = R == -INFINITY ? 0.f : R;
+      ob = ex2(Rr - kLift - mr);
+      // pass 2: weights and their parts
+      f2 sum = 0ull;
+      auto weights = [&](auto some_masked) {
+        tmem_each16<4>(tcol, [&](int c, const uint32_t(&s)[16]) {
+          const float fk = qs * ks[c];
+          // 2^(x - m) * fv = 2^(x + log2(V scale) - R + lift)
+          const uint32_t bits = __float_as_uint(vs[c]), ev = bits >> 23;
+          const float mant = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+          const float fv = ev < 255u ? mant * ex2(fminf(mr + ((float)ev - 127.f) - Rr + kLift, 126.f))
+                                     : __uint_as_float(0x7fc00000u);
+          const f2 fk2 = pack2(fk, fk), fv2 = pack2(fv, fv), mr2 = pack2(-mr, -mr);
+          const uint32_t mk = decltype(some_masked)::value ? mask16(64 * hf + 16 * c) : 0u;
+          uint32_t part[PARTS][8];
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float2 x = unpack2(fma2(pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), fk2, mr2));
+            float w0 = ex2(x.x), w1 = ex2(x.y);
+            if constexpr (decltype(some_masked)::value) {
+              w0 = (mk >> j) & 1u ? w0 : 0.f;
+              w1 = (mk >> (j + 1)) & 1u ? w1 : 0.f;
+            }
+            const f2 w = pack2(w0, w1);
+            sum = add2(sum, w);
+            float2 u = unpack2(mul2(w, fv2));
+            if constexpr (decltype(some_masked)::value) {  // the scale of a block without seen keys may be NaN
+              u.x = (mk >> j) & 1u ? u.x : 0.f;
+              u.y = (mk >> (j + 1)) & 1u ? u.y : 0.f;
+            }
+            uint32_t y[PARTS];
+            split<true, PARTS>(u.x, u.y, y);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) part[q][j / 2] = y[q];
+          }
+          // the block's 16 columns of S are read: its P takes them
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) tmem_put8(tcol + 16 * c + 8 * q, part[q]);
+        });
+      };
+      if (masked) weights(True{});
+      else weights(False{});
+      const float2 sum2 = unpack2(sum);
+      l += sum2.x + sum2.y;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&X.p_full);
+    }
+    wait(&X.t_full, 0u, X, p.err);
+    tc_fence_after();
+    if (n > 0) add_tile();
+
+    // ---------------------------------------------------------------- output
+    const long long unit = (long long)tile * c.kv_heads + g;
+    const bool row_in = tl < ntok && work && !(ps >= 0 && seg < 0);  // rows left out write nothing
+    float of[DH];
+#pragma unroll
+    for (int d = 0; d < DH; d += 2) {
+      const float2 x = unpack2(o[d / 2]);
+      of[d] = live ? x.x : 0.f, of[d + 1] = live ? x.y : 0.f;
+    }
+    if (!live) m = -INFINITY, l = 0.f;
+    bool bad = false;
+    if constexpr (BF) {
+#pragma unroll
+      for (int d = 0; d < DH; ++d) bad |= !(fabsf(of[d]) <= 3.402823466e38f);
+    }
+    pair_bar();
+    X.pair[hf][r] = make_float2(l, bad ? 1.f : 0.f);
+    pair_bar();
+    const float2 other = X.pair[hf ^ 1][r];
+    l = hf ? other.x + l : l + other.x;
+    if constexpr (BF) {
+      if (row_in && live && (bad || other.y != 0.f)) {
+        const Seg sg = X.segs[seg];
+        const int end = sg.first + seen_range<kKeys>(sg.hi, sg.lo, sg.sinks).n;
+        plain_row<D>(p, sg, max(tbeg, sg.first) - sg.first, min(tend, end) - sg.first, t0 + tl, head, g, ps, hf * DH, m, l, of);
+      }
+    }
+    if (row_in) {
+      if (nsplit == 1) {
+        const float f = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int d = 0; d < DH; d += 8) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = of[d + j] * f;
+          emit<8>(p, t0 + tl, head * D + hf * DH + d, width, v);
+        }
+      } else {
+        float* part = p.part + ((unit * p.splits + split_i) * kRows + r) * kPart;
+#pragma unroll
+        for (int d = 0; d < DH; d += 2) __stcg(reinterpret_cast<float2*>(part + hf * DH + d), make_float2(of[d], of[d + 1]));
+        if (hf == 0) __stcg(reinterpret_cast<float2*>(part + D), make_float2(m, l));
+      }
+    }
+    tc_fence_before();
+    __syncthreads();
+  }
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, H::kCols);
+  }
+  if (nsplit == 1 || !work) return;
+  // the last split of the tile merges them all, in split order, and leaves the counter zero
+  const long long unit = (long long)tile * c.kv_heads + g;
+  if (tid == 0) X.last = atomic_add_acq_rel(p.counters + unit, 1u) == (unsigned)(nsplit - 1);
+  __syncthreads();
+  if (!X.last) return;
+  const float* parts = p.part + unit * p.splits * (long long)(kRows * kPart);
+  for (int e = tid; e < ntok * G * (D / 2); e += kThreads) {
+    const int r = e / (D / 2), d = 2 * (e - r * (D / 2)), tl = r / G;
+    if (X.pos[tl] >= 0) {
+      bool in = false;
+      for (int s = 0; s < X.nseg; ++s) in |= X.segs[s].row == X.row[tl];
+      if (!in) continue;
+    }
+    float mm, ll, a, b;
+    merge2<D>([&](int w, int i) { return __ldcg(parts + ((long long)w * kRows + r) * kPart + i); }, nsplit, d, mm, ll, a, b);
+    const float inv = ll != 0.f ? 1.f / ll : 0.f;
+    const float v[2] = {a * inv, b * inv};
+    emit<2>(p, t0 + tl, (g * G + r - tl * G) * D + d, width, v);
+  }
+  if (tid == 0) p.counters[unit] = 0u;
+}
+
+template <int FMT, int D, int PARTS>
+cudaError_t launch(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
+  using H = Shape<FMT, D, PARTS>;
+  auto kernel = prompt_kernel<FMT, D, PARTS>;
+  constexpr int smem = H::kOffMisc + kMiscBytes;
+  static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  // the warpgroups' register counts are made for this launch size
+  static const cudaError_t regs = [&] {
+    cudaFuncAttributes a;
+    const cudaError_t r = cudaFuncGetAttributes(&a, reinterpret_cast<const void*>(kernel));
+    return r != cudaSuccess ? r : a.numRegs < H::kRegLaunch ? cudaErrorInvalidConfiguration : cudaSuccess;
+  }();
+  if (regs != cudaSuccess) return regs;
+  const int TT = kRows / p.group;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.M + TT - 1) / TT * p.splits), p.c.kv_heads, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int D>
+cudaError_t launch_dim(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
+  const bool f32 = p.dtype == QI_F32;
+  if (p.c.format == QI_KV_INT8) return f32 ? launch<QI_KV_INT8, D, 2>(p, s, pdl) : launch<QI_KV_INT8, D, 1>(p, s, pdl);
+  if (p.c.format == QI_KV_E4M3) return f32 ? launch<QI_KV_E4M3, D, 2>(p, s, pdl) : launch<QI_KV_E4M3, D, 1>(p, s, pdl);
+  return f32 ? launch<QI_KV_BF16, D, 2>(p, s, pdl) : launch<QI_KV_BF16, D, 1>(p, s, pdl);
+}
+
+}  // namespace
+
+cudaError_t launch_cache_attention_prompt(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
+  return p.c.head_dim == 64 ? launch_dim<64>(p, s, pdl) : launch_dim<128>(p, s, pdl);
+}
+
+}  // namespace qi
