@@ -736,7 +736,7 @@ int qi_cache_attention(const qi_kv_layer* layer, const void* q, long long q_toke
                        int query_run, void* out, float* part, long long part_floats, unsigned int* counters,
                        long long counters_len, int* err, qi_stream_t stream) {
   if (bad_attention(layer, heads, M, window, sinks, query_run) || bad_ptr(q) || bad_dtype(dtype) || bad_ptr(rows) ||
-      bad_ptr(pos) || bad_ptr(out) || ((uintptr_t)part & 7))
+      bad_ptr(pos) || bad_ptr(out) || ((uintptr_t)out & 15) || ((uintptr_t)part & 7))
     return QI_ERR_ARG;
   CacheAttnParams p = {};
   p.c = *layer;

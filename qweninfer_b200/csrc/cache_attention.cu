@@ -421,28 +421,23 @@ int token_splits(const qi_kv_layer& c, int M, int window, int sinks) {
   return (int)(want > kMaxAttnSplits ? kMaxAttnSplits : want < 1 ? 1 : want);
 }
 
-// Key splits of the prompt kernel: as many as fill the CTAs that are resident at once.
+// Key splits of the prompt kernel, the CTAs of a cluster: as many as fill the CTAs that are
+// resident at once.
 int prompt_splits(const qi_kv_layer& c, int tiles, int window, int sinks) {
   const long long slots = (c.head_dim == 64 ? 2LL : 1LL) * sm_count();
   const long long n = slots / ((long long)tiles * c.kv_heads);
   const long long most = (seen_at_most(c, window, sinks) / kPromptKeys + 2) / kMinTiles;
   const long long want = n < most ? n : most;
-  return (int)(want > kMaxAttnSplits ? kMaxAttnSplits : want < 1 ? 1 : want);
+  return (int)(want > 8 ? 8 : want < 1 ? 1 : want);
 }
 
 int prompt_tiles(int M, int group) { return (M + kPromptRows / group - 1) / (kPromptRows / group); }
 
 void sizes(CacheAttnPlan& r, const qi_kv_layer& c, int heads, int M) {
   r.part_floats = r.counters = 0;
-  if (r.prompt && r.splits > 1) {
-    const long long units = (long long)prompt_tiles(M, heads / c.kv_heads) * c.kv_heads;
-    r.part_floats = units * r.splits * kPromptRows * (c.head_dim + 2);
-    r.counters = units;
-  }
   if ((!r.prompt || r.singles) && r.token_splits > 1) {
-    const long long f = (long long)M * heads * r.token_splits * (c.head_dim + 2), n = (long long)M * c.kv_heads;
-    r.part_floats = f > r.part_floats ? f : r.part_floats;
-    r.counters = n > r.counters ? n : r.counters;
+    r.part_floats = (long long)M * heads * r.token_splits * (c.head_dim + 2);
+    r.counters = (long long)M * c.kv_heads;
   }
 }
 
@@ -461,7 +456,6 @@ CacheAttnPlan cache_attention_plan(const qi_kv_layer& c, int heads, int M, int w
 void cache_attention_fit(CacheAttnPlan& r, const qi_kv_layer& c, int heads, int M, long long part_floats,
                          long long counters) {
   while (r.part_floats > part_floats || r.counters > counters) {
-    if (r.splits > 1) --r.splits;
     if (r.token_splits > 1) --r.token_splits;
     sizes(r, c, heads, M);
   }

@@ -78,28 +78,44 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& p0, uint32_t& p1) {
   }
 }
 
-// Output values of features f .. f + N - 1 (N even, f a multiple of N) of a token.
+// Output values of features f .. f + N - 1 (N 2 or 8, f a multiple of N) of a token.
 template <int N>
 __device__ __forceinline__ void emit(const CacheAttnParams& p, int tok, int f, int width, const float (&v)[N]) {
+  static_assert(N == 2 || N == 8, "one store, or a row of 16 bytes");
   if (p.out) {
     const long long o = (long long)tok * width + f;
     if (p.dtype == QI_F32) {
-      float2* d = reinterpret_cast<float2*>(static_cast<float*>(p.out) + o);
-#pragma unroll
-      for (int i = 0; i < N; i += 2) d[i / 2] = make_float2(v[i], v[i + 1]);
+      float* d = static_cast<float*>(p.out) + o;
+      if constexpr (N == 2) {
+        *reinterpret_cast<float2*>(d) = make_float2(v[0], v[1]);
+      } else {
+        *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(d + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      }
     } else {
-      uint32_t* d = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + o);
+      uint16_t* d = static_cast<uint16_t*>(p.out) + o;
+      uint32_t w[N / 2];
 #pragma unroll
-      for (int i = 0; i < N; i += 2) d[i / 2] = p.dtype == QI_BF16 ? b16x2(v[i], v[i + 1]) : f16x2(v[i], v[i + 1]);
+      for (int i = 0; i < N; i += 2) w[i / 2] = p.dtype == QI_BF16 ? b16x2(v[i], v[i + 1]) : f16x2(v[i], v[i + 1]);
+      if constexpr (N == 2) *reinterpret_cast<uint32_t*>(d) = w[0];
+      else *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  if (p.out_act) {
+  if (p.out_act) {  // N consecutive features lie side by side in an activation tile
+    uint32_t hi[N / 2], lo[N / 2];
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      const uint32_t hi = b16x2(v[i], v[i + 1]);
-      const uint32_t lo = b16x2(v[i] - bf16lo(hi), v[i + 1] - bf16hi(hi));
-      *reinterpret_cast<uint32_t*>(p.out_act + act_offset(tok, f + i, 0, width, p.out_nt)) = hi;
-      *reinterpret_cast<uint32_t*>(p.out_act + act_offset(tok, f + i, 1, width, p.out_nt)) = lo;
+      hi[i / 2] = b16x2(v[i], v[i + 1]);
+      lo[i / 2] = b16x2(v[i] - bf16lo(hi[i / 2]), v[i + 1] - bf16hi(hi[i / 2]));
+    }
+    uint16_t* h = p.out_act + act_offset(tok, f, 0, width, p.out_nt);
+    uint16_t* l = p.out_act + act_offset(tok, f, 1, width, p.out_nt);
+    if constexpr (N == 2) {
+      *reinterpret_cast<uint32_t*>(h) = hi[0];
+      *reinterpret_cast<uint32_t*>(l) = lo[0];
+    } else {
+      *reinterpret_cast<uint4*>(h) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(l) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   }
 }

@@ -28,6 +28,9 @@
 // counts uses fp16's range whatever the scales are; T is brought back to the running maximum
 // of the softmax when it is added to O.
 //
+// With few tiles the keys are split over the CTAs of a cluster, which exchange their partials
+// through distributed shared memory: no scratch in global memory, no waiting CTA.
+//
 // Tokens of several cache rows in one tile are segments, worked off one after another with
 // the other rows masked. Tokens alone in their tile's segment (a batched prefill's last
 // tokens) are left to the per-token kernel in a second launch.
@@ -83,12 +86,15 @@ struct Seg {
 struct Misc {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, p_full, t_full;
   uint32_t tmem;
-  int nseg, ntiles, last;
+  int nseg, ntiles;
   int abort;  // a wait of this CTA gave up: the others do not wait any more
   int pos[kRows], row[kRows], seg[kRows];  // per token
   Seg segs[kRows];
-  float scale[2][2][8];                    // [stage][K, V][16 keys]
+  // of 16 keys, by stage: K scale, exponent and significand of the V scale (s = 2^e * f; a
+  // scale that is not finite has f = NaN)
+  float ks[2][8], ve[2][8], vf[2][8];
   float2 pair[2][kRows];                   // what the two threads of a row tell each other
+  float2 ml[kRows];                        // maximum and sum of the rows' partials
 };
 constexpr uint32_t kMiscBytes = (sizeof(Misc) + 15) / 16 * 16;
 
@@ -208,33 +214,39 @@ __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, Misc& X, in
   }
 }
 
-// 8 consecutive elements of a query row as fp32
-__device__ __forceinline__ void load_q8(const CacheAttnParams& p, long long o, float (&x)[8]) {
+// N 16-byte pieces of a query row (fp32, or a 16-bit type) from element o on, as they are
+template <int N, bool F32>
+__device__ __forceinline__ void load_row(const CacheAttnParams& p, long long o, uint4 (&x)[N]) {
   if (p.q_vec) {
-    if (p.dtype == QI_F32) {
-      const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + o);
-      const float4 a = __ldcg(f), b = __ldcg(f + 1);
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + o));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.q) + o * (F32 ? 4 : 2));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (p.dtype == QI_BF16) {
-          x[2 * i] = bf16lo(w[i]), x[2 * i + 1] = bf16hi(w[i]);
+    for (int i = 0; i < N; ++i) x[i] = __ldcg(q + i);
+  } else {
+    for (int i = 0; i < N; ++i) {
+      uint32_t w[4];
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (F32) {
+          w[e] = __ldcg(static_cast<const uint32_t*>(p.q) + o + 4 * i + e);
         } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          x[2 * i] = f.x, x[2 * i + 1] = f.y;
+          const unsigned short* h = static_cast<const unsigned short*>(p.q) + o + 8 * i + 2 * e;
+          w[e] = (uint32_t)__ldcg(h) | (uint32_t)__ldcg(h + 1) << 16;
         }
       }
+      x[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = p.dtype == QI_F32    ? load_elem<QI_F32>(p.q, o + i)
-             : p.dtype == QI_BF16 ? load_elem<QI_BF16>(p.q, o + i)
-                                  : load_elem<QI_F16>(p.q, o + i);
   }
+}
+// values 2 i and 2 i + 1 of such a row
+template <bool F32>
+__device__ __forceinline__ float2 row_pair(const uint4* x, int i, int dtype) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+  if constexpr (F32) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  else if (dtype == QI_BF16) return make_float2(bf16lo(w[i]), bf16hi(w[i]));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+}
+// one element of q
+__device__ __forceinline__ float load_q(const CacheAttnParams& p, long long i) {
+  return p.dtype == QI_F32 ? load_elem<QI_F32>(p.q, i) : p.dtype == QI_BF16 ? load_elem<QI_BF16>(p.q, i) : load_elem<QI_F16>(p.q, i);
 }
 
 // Key by key: the partial of token t's head over the given tiles of its segment (bf16
@@ -256,11 +268,7 @@ __device__ __noinline__ void plain_row(const CacheAttnParams& p, const Seg& sg, 
       const uint16_t* k = static_cast<const uint16_t*>(p.c.k) + (base < 0 ? 0 : base) + j * D;
       const uint16_t* v = static_cast<const uint16_t*>(p.c.v) + (base < 0 ? 0 : base) + j * D;
       if (base >= 0)
-        for (int d = 0; d < D; d += 8) {
-          float x[8];
-          load_q8(p, qo + d, x);
-          for (int e = 0; e < 8; ++e) s = fmaf(x[e], bf16_to_f32(k[d + e]), s);
-        }
+        for (int d = 0; d < D; ++d) s = fmaf(load_q(p, qo + d), bf16_to_f32(k[d]), s);
       s *= p.scale_log2;
       if (s > m) {
         const float a = m == -INFINITY ? 0.f : ex2(m - s);
@@ -276,6 +284,23 @@ __device__ __noinline__ void plain_row(const CacheAttnParams& p, const Seg& sg, 
   }
 }
 
+// the same shared memory of CTA w of the cluster (of C CTAs)
+__device__ __forceinline__ float peer(const float* x, int w, int C) {
+  if (C == 1) return *x;
+  float r;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r) : "r"(map_rank(x, (uint32_t)w)) : "memory");
+  return r;
+}
+__device__ __forceinline__ float4 peer4(const float* x, int w, int C) {
+  if (C == 1) return *reinterpret_cast<const float4*>(x);
+  float4 r;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
+               : "r"(map_rank(x, (uint32_t)w))
+               : "memory");
+  return r;
+}
+
 template <int N>
 __device__ __forceinline__ void more_regs() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -289,7 +314,7 @@ template <int FMT, int D, int PARTS>
 __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_kernel(const CacheAttnParams p) {
   using H = Shape<FMT, D, PARTS>;
   constexpr bool BF = FMT == QI_KV_BF16;
-  constexpr int kPart = D + 2;
+  constexpr int kPitch = D + 4;  // floats of a row of partial outputs
   extern __shared__ __align__(1024) uint8_t smem[];
   Misc& X = *reinterpret_cast<Misc*>(smem + H::kOffMisc);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -306,6 +331,13 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
     tmem_relinquish();
   }
   grid_dep_launch();
+  // Threads r and r + 128 of the softmax warps: query row r = (token, head), half of its
+  // dims (and 64 of a tile's keys). The loads overlap the setup.
+  constexpr int DH = D / 2, kRaw = DH / (PARTS == 2 ? 4 : 8);
+  const int r = tid & (kRows - 1), hf = tid >> 7;
+  const int tl = r / G, head = g * G + r - tl * G;
+  uint4 raw[kRaw];
+  if (warp < kSoftWarps) load_row<kRaw, PARTS == 2>(p, (long long)(t0 + min(tl, ntok - 1)) * p.q_st + (long long)head * p.q_sh + hf * DH, raw);
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&X.k_full[s], kLoadWarps);
@@ -480,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       }
     };
     // bf16 values -> fp16 operand rows, and the scales of the warp's two blocks of 16 keys
-    auto store16 = [&](const uint4* regs, uint8_t* t, float* scales) {
+    auto store16 = [&](const uint4* regs, uint8_t* t, int st, bool k_side) {
       constexpr int kB = kN / 2;  // chunks of a block
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -510,7 +542,10 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
         // scale and its reciprocal are normal); tiny blocks are left with a smaller maximum
         const uint32_t e = min(max(mx >> 23, 15u), 253u);
         const float inv = __uint_as_float((268u - e) << 23);
-        if (lane == 0) scales[lw * 2 + b] = __uint_as_float((e - 14u) << 23);
+        if (lane == 0) {
+          if (k_side) X.ks[st][lw * 2 + b] = __uint_as_float((e - 14u) << 23);
+          else X.ve[st][lw * 2 + b] = (float)((int)e - 141), X.vf[st][lw * 2 + b] = 1.f;
+        }
 #pragma unroll
         for (int j = b * kB; j < (b + 1) * kB; ++j) {
           int r, ch;
@@ -539,13 +574,19 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
         wait(&X.v_empty[st], ph, X, p.err);
       }
       if constexpr (BF) {
-        store16(kr, kt, X.scale[st][0]);
+        store16(kr, kt, st, true);
         publish(&X.k_full[st]);
         fetch(tbeg + i, false);
-        store16(kr, vt, X.scale[st][1]);
+        store16(kr, vt, st, false);
         publish(&X.v_full[st]);
       } else {
-        if (lt < 16) X.scale[st][lt >> 3][lt & 7] = sc;
+        if (lt < 8) X.ks[st][lt] = sc;
+        else if (lt < 16) {
+          const uint32_t bits = __float_as_uint(sc);
+          X.ve[st][lt - 8] = (float)((int)(bits >> 23) - 127);
+          X.vf[st][lt - 8] = bits < 0x7f800000u ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u)
+                                                : __uint_as_float(0x7fc00000u);
+        }
         store8(kr, kt);
         publish(&X.k_full[st]);
         store8(vr, vt);
@@ -557,9 +598,6 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
   } else {
     // --------------------------------------------------------------- softmax
     more_regs<H::kRegSoft>();
-    constexpr int DH = D / 2;
-    const int r = tid & (kRows - 1), hf = tid >> 7;  // row; 64 keys and DH dims of the two halves
-    const int tl = r / G, head = g * G + r - tl * G;
     auto pair_bar = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };
     const int ps = tl < ntok ? X.pos[tl] : -1;
     // the row's segment, by cache row (segments left out have no entry)
@@ -570,31 +608,32 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
     float qs = p.scale_log2;
     {
       float am = 0.f;
-      const long long qo = (long long)(t0 + (live ? tl : 0)) * p.q_st + (long long)(live ? head : 0) * p.q_sh;
-#pragma unroll 2
-      for (int ch = 0; ch < D / 8; ++ch) {
-        float x[8];
-        if (live) load_q8(p, qo + 8 * ch, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) am = live ? fmaxf(am, fabsf(x[e])) : 0.f;
+      for (int i = 0; i < DH / 2; ++i) {
+        const float2 x = row_pair<PARTS == 2>(raw, i, p.dtype);
+        am = fmaxf(am, fmaxf(fabsf(x.x), fabsf(x.y)));
       }
-      float inv = 1.f;
+      X.pair[hf][r].x = am;
+      pair_bar();
+      am = fmaxf(am, X.pair[hf ^ 1][r].x);
+      float inv = live ? 1.f : 0.f;
       const uint32_t e = __float_as_uint(am) >> 23;
-      if (e > 0 && e < 253) {
+      if (live && e > 0 && e < 253) {
         inv = __uint_as_float((254u - e) << 23);
         qs *= __uint_as_float(e << 23);
       }
-#pragma unroll 2
-      for (int ch = hf * (DH / 8); ch < (hf + 1) * (DH / 8); ++ch) {
-        float x[8];
-        if (live) load_q8(p, qo + 8 * ch, x);
+#pragma unroll
+      for (int ch = 0; ch < DH / 8; ++ch) {
         uint32_t w[4][PARTS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          split<true, PARTS>(live ? x[2 * i] * inv : 0.f, live ? x[2 * i + 1] * inv : 0.f, w[i]);
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = row_pair<PARTS == 2>(raw, 4 * ch + i, p.dtype);
+          split<true, PARTS>(live ? x.x * inv : 0.f, live ? x.y * inv : 0.f, w[i]);
+        }
 #pragma unroll
         for (int q = 0; q < PARTS; ++q)
-          *reinterpret_cast<uint4*>(smem + q * H::kQ + core<D>(r, ch)) = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+          *reinterpret_cast<uint4*>(smem + q * H::kQ + core<D>(r, hf * (DH / 8) + ch)) =
+              make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
       }
       fence_async_smem();
     }
@@ -639,29 +678,29 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       };
       wait(&X.k_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);  // the scales
       wait(&X.v_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);
+      float ks[4], ve[4];  // of this half's 4 blocks
+#pragma unroll
+      for (int c = 0; c < 4; ++c) ks[c] = qs * X.ks[st][4 * hf + c], ve[c] = X.ve[st][4 * hf + c];
       wait(&X.s_full, (uint32_t)i & 1u, X, p.err);  // S(i), and T(i - 1) before it
       tc_fence_after();
       if (i > 0) add_tile();
-      const float* ks = X.scale[st][0] + 4 * hf;
-      const float* vs = X.scale[st][1] + 4 * hf;
       const uint32_t tcol = trow + 64 * hf;  // this half's scores
       // pass 1: the maxima of the scores and of score + log2(V scale)
       float mx = -INFINITY, R = -INFINITY;
       auto maxima = [&](auto some_masked) {
         tmem_each16<4>(tcol, [&](int c, const uint32_t(&s)[16]) {
-          float v = -INFINITY;
-          if constexpr (decltype(some_masked)::value) {
-            const uint32_t mk = mask16(64 * hf + 16 * c);
+          float a4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          const uint32_t mk = decltype(some_masked)::value ? mask16(64 * hf + 16 * c) : 0u;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v = fmaxf(v, (mk >> j) & 1u ? __uint_as_float(s[j]) : -INFINITY);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v = fmaxf(v, __uint_as_float(s[j]));
+          for (int j = 0; j < 16; ++j) {
+            const float x = __uint_as_float(s[j]);
+            if constexpr (decltype(some_masked)::value) a4[j & 3] = fmaxf(a4[j & 3], (mk >> j) & 1u ? x : -INFINITY);
+            else a4[j & 3] = fmaxf(a4[j & 3], x);
           }
+          float v = fmaxf(fmaxf(a4[0], a4[1]), fmaxf(a4[2], a4[3]));
           // a block without seen keys has no say; its scale may be anything
-          v = v == -INFINITY ? v : v * (qs * ks[c]);
-          const uint32_t ev = __float_as_uint(vs[c]) >> 23;
-          R = fmaxf(R, v + (ev < 255u ? (float)ev - 127.f : 0.f));
+          v = v == -INFINITY ? v : v * ks[c];
+          R = fmaxf(R, v + ve[c]);
           mx = fmaxf(mx, v);
         });
       };
@@ -677,17 +716,14 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       m = mn;
       const float mr = m == -INFINITY ? 0.f : m, Rr = R == -INFINITY ? 0.f : R;
       ob = ex2(Rr - kLift - mr);
+      const float rest = mr - Rr + kLift;
       // pass 2: weights and their parts
-      f2 sum = 0ull;
+      f2 sum[2] = {0ull, 0ull};
       auto weights = [&](auto some_masked) {
         tmem_each16<4>(tcol, [&](int c, const uint32_t(&s)[16]) {
-          const float fk = qs * ks[c];
           // 2^(x - m) * fv = 2^(x + log2(V scale) - R + lift)
-          const uint32_t bits = __float_as_uint(vs[c]), ev = bits >> 23;
-          const float mant = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
-          const float fv = ev < 255u ? mant * ex2(fminf(mr + ((float)ev - 127.f) - Rr + kLift, 126.f))
-                                     : __uint_as_float(0x7fc00000u);
-          const f2 fk2 = pack2(fk, fk), fv2 = pack2(fv, fv), mr2 = pack2(-mr, -mr);
+          const float fv = X.vf[st][4 * hf + c] * ex2(fminf(ve[c] + rest, 126.f));
+          const f2 fk2 = pack2(ks[c], ks[c]), fv2 = pack2(fv, fv), mr2 = pack2(-mr, -mr);
           const uint32_t mk = decltype(some_masked)::value ? mask16(64 * hf + 16 * c) : 0u;
           uint32_t part[PARTS][8];
 #pragma unroll
@@ -699,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
               w1 = (mk >> (j + 1)) & 1u ? w1 : 0.f;
             }
             const f2 w = pack2(w0, w1);
-            sum = add2(sum, w);
+            sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], w);
             float2 u = unpack2(mul2(w, fv2));
             if constexpr (decltype(some_masked)::value) {  // the scale of a block without seen keys may be NaN
               u.x = (mk >> j) & 1u ? u.x : 0.f;
@@ -717,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       };
       if (masked) weights(True{});
       else weights(False{});
-      const float2 sum2 = unpack2(sum);
+      const float2 sum2 = unpack2(add2(sum[0], sum[1]));
       l += sum2.x + sum2.y;
       tmem_st_wait();
       tc_fence_before();
@@ -729,7 +765,6 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
     if (n > 0) add_tile();
 
     // ---------------------------------------------------------------- output
-    const long long unit = (long long)tile * c.kv_heads + g;
     const bool row_in = tl < ntok && work && !(ps >= 0 && seg < 0);  // rows left out write nothing
     float of[DH];
 #pragma unroll
@@ -755,23 +790,12 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
         plain_row<D>(p, sg, max(tbeg, sg.first) - sg.first, min(tend, end) - sg.first, t0 + tl, head, g, ps, hf * DH, m, l, of);
       }
     }
-    if (row_in) {
-      if (nsplit == 1) {
-        const float f = l != 0.f ? 1.f / l : 0.f;
+    // The split's partial (relative to m) into shared memory, in the place of Q and K, which
+    // all products are done with: rows of D + 4 floats, so that rows 8 apart share a bank.
+    float* po = reinterpret_cast<float*>(smem) + r * kPitch + hf * DH;
 #pragma unroll
-        for (int d = 0; d < DH; d += 8) {
-          float v[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = of[d + j] * f;
-          emit<8>(p, t0 + tl, head * D + hf * DH + d, width, v);
-        }
-      } else {
-        float* part = p.part + ((unit * p.splits + split_i) * kRows + r) * kPart;
-#pragma unroll
-        for (int d = 0; d < DH; d += 2) __stcg(reinterpret_cast<float2*>(part + hf * DH + d), make_float2(of[d], of[d + 1]));
-        if (hf == 0) __stcg(reinterpret_cast<float2*>(part + D), make_float2(m, l));
-      }
-    }
+    for (int d = 0; d < DH; d += 4) *reinterpret_cast<float4*>(po + d) = make_float4(of[d], of[d + 1], of[d + 2], of[d + 3]);
+    if (hf == 0) X.ml[r] = make_float2(m, l);
     tc_fence_before();
     __syncthreads();
   }
@@ -779,27 +803,44 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
     tc_fence_after();
     tmem_dealloc(tmem, H::kCols);
   }
-  if (nsplit == 1 || !work) return;
-  // the last split of the tile merges them all, in split order, and leaves the counter zero
-  const long long unit = (long long)tile * c.kv_heads + g;
-  if (tid == 0) X.last = atomic_add_acq_rel(p.counters + unit, 1u) == (unsigned)(nsplit - 1);
-  __syncthreads();
-  if (!X.last) return;
-  const float* parts = p.part + unit * p.splits * (long long)(kRows * kPart);
-  for (int e = tid; e < ntok * G * (D / 2); e += kThreads) {
-    const int r = e / (D / 2), d = 2 * (e - r * (D / 2)), tl = r / G;
-    if (X.pos[tl] >= 0) {
+  // The splits of a tile are one cluster: each takes a share of the rows, sums the partials
+  // in split order out of the others' shared memory, and writes them out.
+  const int C = p.splits;
+  if (C > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  const int rows_in = ntok * G, r0 = rows_in * split_i / C, r1 = rows_in * (split_i + 1) / C;
+  for (int e = tid; e < (r1 - r0) * (D / 8); e += kThreads) {
+    const int rr = r0 + e / (D / 8), d = e % (D / 8) * 8, tt = rr / G;
+    if (X.pos[tt] >= 0) {  // a row that was left out
       bool in = false;
-      for (int s = 0; s < X.nseg; ++s) in |= X.segs[s].row == X.row[tl];
+      for (int s = 0; s < X.nseg; ++s) in |= X.segs[s].row == X.row[tt];
       if (!in) continue;
     }
-    float mm, ll, a, b;
-    merge2<D>([&](int w, int i) { return __ldcg(parts + ((long long)w * kRows + r) * kPart + i); }, nsplit, d, mm, ll, a, b);
+    float mx = -INFINITY;
+    for (int w = 0; w < nsplit; ++w) mx = fmaxf(mx, peer(&X.ml[rr].x, w, C));
+    float ll = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < nsplit; ++w) {
+      const float mw = peer(&X.ml[rr].x, w, C), lw = peer(&X.ml[rr].y, w, C);
+      // a partial without keys (maximum -inf, sum 0) has nothing to add; a NaN sum stays one
+      const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2(mw - mx);
+      ll = fmaf(f, lw, ll);
+      const float* po = reinterpret_cast<const float*>(smem) + rr * kPitch + d;
+      const float4 a = peer4(po, w, C), b = peer4(po + 4, w, C);
+      v[0] = fmaf(f, a.x, v[0]), v[1] = fmaf(f, a.y, v[1]), v[2] = fmaf(f, a.z, v[2]), v[3] = fmaf(f, a.w, v[3]);
+      v[4] = fmaf(f, b.x, v[4]), v[5] = fmaf(f, b.y, v[5]), v[6] = fmaf(f, b.z, v[6]), v[7] = fmaf(f, b.w, v[7]);
+    }
     const float inv = ll != 0.f ? 1.f / ll : 0.f;
-    const float v[2] = {a * inv, b * inv};
-    emit<2>(p, t0 + tl, (g * G + r - tl * G) * D + d, width, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= inv;
+    emit<8>(p, t0 + tt, (g * G + rr - tt * G) * D + d, width, v);
   }
-  if (tid == 0) p.counters[unit] = 0u;
+  if (C > 1) {  // the others are done with this CTA's shared memory
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
 }
 
 template <int FMT, int D, int PARTS>
@@ -823,11 +864,20 @@ cudaError_t launch(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (pdl) {
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (p.splits > 1) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = (unsigned)p.splits;
+    attr[na].val.clusterDim.y = 1;
+    attr[na++].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = na;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 

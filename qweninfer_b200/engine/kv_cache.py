@@ -130,7 +130,7 @@ class KVCache:
         `check()` and gives a zero output). `query_run`: the longest run of consecutive
         tokens of one row (a prompt's length), 1 for a decode step, 0 if unknown; it only
         picks the kernel. Returns (M, heads, head_dim) of q's dtype (`out`, if given:
-        contiguous and apart from q), enqueued on the current stream.
+        contiguous, 16-byte aligned and apart from q), enqueued on the current stream.
 
         Scores, softmax and sums are fp32; q and the probabilities keep at least 22 bits for
         an 8-bit cache, 24 (16 for 16-bit q) for a bf16 one."""
@@ -148,6 +148,8 @@ class KVCache:
             out = torch.empty((M, heads, D), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {q.device}")
+        elif out.data_ptr() % 16:
+            raise ValueError("out must be 16-byte aligned")
         elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
             raise ValueError("out must not share q's storage")
         if M == 0:

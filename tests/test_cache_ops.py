@@ -40,7 +40,7 @@ def append(lib, d, k=1, v=1, dt=0, rows=1, pos=1, M=1):
     return lib.qi_kv8_append(d if d is None else C.byref(d), k, 128, 64, v, 128, 64, dt, rows, pos, M, None, None)
 
 
-def attend(lib, d, q=1, dt=0, heads=14, rows=1, pos=1, M=1, window=0, sinks=0, run=0, out=1, part=8):
+def attend(lib, d, q=1, dt=0, heads=14, rows=1, pos=1, M=1, window=0, sinks=0, run=0, out=16, part=8):
     return lib.qi_cache_attention(d if d is None else C.byref(d), q, 896, 64, dt, heads, rows, pos, M, window, sinks, run,
                                   out, part, 0, 1, 0, None, None)
 
@@ -62,7 +62,7 @@ def test_bad_calls(lib):
     for kw in (dict(k=None), dict(v=None), dict(dt=3), dict(rows=None), dict(pos=None), dict(M=0)):
         assert append(lib, d, **kw) == E, kw
     for kw in (dict(q=None), dict(dt=-1), dict(heads=0), dict(heads=15), dict(heads=18), dict(rows=None),
-               dict(pos=None), dict(M=0), dict(window=-1), dict(sinks=-1), dict(run=-1), dict(out=None),
+               dict(pos=None), dict(M=0), dict(window=-1), dict(sinks=-1), dict(run=-1), dict(out=None), dict(out=8),
                dict(M=2**31 - 1), dict(part=4)):
         assert attend(lib, d, **kw) == E, kw
     assert lib.qi_kv8_values(C.byref(d), 16, 8, None) == E
