@@ -2,23 +2,24 @@
 // keys on the 5th-generation tensor cores (the formula is in cache_attention.cu).
 //
 // A CTA takes the query rows of 128 / group consecutive tokens and one KV head (row = token
-// x head of the group) and a share of the 128-key tiles that any of them sees:
+// x head of the group), at head_dim 64 two such tiles, and a share of the 128-key tiles that
+// any of them sees:
 //   S = Q K^T     M 128 x N 128 x K D, fp32 in TMEM; Q in shared memory
 //   T = P V       M 128 x N D x K 128, fp32 in TMEM; P in TMEM, where it takes the place of S
 // Threads r and r + 128 of the softmax warps share query row r (TMEM lane r), 64 keys and
 // half of the output dims each: two passes over their scores (maximum, then exponentials),
 // and O += T of the tile before in registers: the tensor cores' own accumulation truncates,
 // so it stays within a tile and sums over tiles are rounded fp32 additions. The passes are
-// chains of dependent instructions; two threads a row and two CTAs an SM hide each other's
-// latencies. Four producer warps bring keys and values into
-// the K-major layout of UMMA descriptors as fp16; V in the same layout is the MN-major
-// operand of the second product, so nothing is transposed. One warp issues the MMAs. Two
-// CTAs share an SM at head_dim 64: one's softmax runs during the other's products.
+// chains of dependent instructions; the two threads of a row hide each other's latencies,
+// as do the two tiles of a CTA, which share the keys that four producer warps
+// bring into the K-major layout of UMMA descriptors as fp16 (the widening costs about as
+// much as a tile's softmax). V in the same layout is the MN-major operand of the second
+// product, so nothing is transposed. One warp issues the MMAs.
 //
 // Every format is multiplied in fp16 with a scale for 16 keys: 8-bit codes are exact and
 // have their block's scale; bf16 values get a power of two that puts the largest of 16 keys
-// in [2^14, 2^15), which leaves all within 2^-28 of it exact and errors of 2^-40 of it
-// otherwise. q is scaled per row to a maximum in [1, 2). fp32 callers: q and p in two fp16
+// in [2^14, 2^15), which leaves all within 2^-28 of it exact and the others off by less than
+// that. q is scaled per row to a maximum in [1, 2). fp32 callers: q and p in two fp16
 // parts (22 bits), each part one UMMA chain into the same accumulator, the small ones first.
 // 16-bit callers: one part, exact for q (to 2^-25 of the row's largest) and good to 2^-12 for
 // p, below the output's own rounding.
@@ -51,11 +52,8 @@ using namespace tc;
 
 constexpr int kRows = 128;   // query rows of a tile
 constexpr int kKeys = 128;   // keys of a tile
-// warpgroups: two of softmax, producers, and one whose first warp issues the MMAs
-constexpr int kSoftWarps = 8, kLoadWarp = 8, kLoadWarps = 4, kMmaWarp = 12;
-constexpr int kThreads = 512;
-constexpr int kLoadThreads = 32 * kLoadWarps;
 constexpr float kLift = 14.f;
+constexpr uint32_t kMag = 0x7fff7fffu;  // magnitudes of a bf16 pair
 constexpr unsigned kAll = 0xffffffffu;
 
 struct True {
@@ -67,34 +65,41 @@ struct False {
 
 template <int FMT, int D, int PARTS>
 struct Shape {
-  static constexpr uint32_t kQ = kRows * D * 2;   // one part of Q
-  static constexpr uint32_t kT = kKeys * D * 2;   // K or V tile
-  static constexpr uint32_t kOffK = PARTS * kQ, kOffV = kOffK + 2 * kT, kOffMisc = kOffV + 2 * kT;
-  static constexpr uint32_t kColT = 128, kCols = 256;  // TMEM: S (P in its place), T
+  static constexpr int kTiles = D == 64 ? 2 : 1;  // query tiles of a CTA
+  // warpgroups: two of softmax for each tile, producers, and one whose first warp issues MMAs
+  static constexpr int kSoftWarps = 8 * kTiles, kLoadWarp = kSoftWarps, kLoadWarps = 4, kMmaWarp = kLoadWarp + kLoadWarps;
+  static constexpr int kThreads = 32 * (kMmaWarp + 4);
+  static constexpr uint32_t kQ = kRows * D * 2;   // one part of a tile's Q
+  static constexpr uint32_t kT = kKeys * D * 2;   // K or V tile, two stages each
+  static constexpr uint32_t kOffK = kTiles * PARTS * kQ, kOffV = kOffK + 2 * kT, kOffMisc = kOffV + 2 * kT;
+  // TMEM columns: S of the tiles (P in its place), then T
+  static constexpr uint32_t kColT = kTiles * 128, kCols = kTiles == 2 ? 512 : 256;
+  static_assert(kColT + kTiles * D <= kCols, "tensor memory");
   // Registers of a thread: of the launch, and of the warpgroups, which together have no more.
-  static constexpr int kCtas = D == 64 ? 2 : 1;
-  static constexpr int kRegLaunch = D == 64 ? 64 : 128;
-  static constexpr int kRegSoft = D == 64 ? 80 : 152, kRegLoad = D == 64 ? 64 : 160, kRegMma = D == 64 ? 32 : 48;
-  static_assert(2 * kRegSoft + kRegLoad + kRegMma <= 4 * kRegLaunch, "the increase must be covered");
+  static constexpr int kRegLaunch = D == 64 ? 80 : 128;
+  static constexpr int kRegSoft = D == 64 ? 88 : 152, kRegLoad = D == 64 ? 88 : 160, kRegMma = D == 64 ? 40 : 48;
+  static_assert(2 * kTiles * kRegSoft + kRegLoad + kRegMma <= (2 * kTiles + 2) * kRegLaunch, "the increase must be covered");
 };
 
-// the part of a tile's tokens that lies in one cache row
+constexpr int kMaxTok = 2 * kRows;  // tokens of a CTA
+
+// the part of a CTA's tokens that lies in one cache row
 struct Seg {
   int row, lo, hi, sinks, first;  // positions lo..hi and 0..sinks-1 seen; first tile in the list
 };
 
 struct Misc {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, p_full, t_full;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], t_full[2];
   uint32_t tmem;
   int nseg, ntiles;
   int abort;  // a wait of this CTA gave up: the others do not wait any more
-  int pos[kRows], row[kRows], seg[kRows];  // per token
-  Seg segs[kRows];
+  int pos[kMaxTok], row[kMaxTok], seg[kMaxTok];  // per token
+  Seg segs[kMaxTok];
   // of 16 keys, by stage: K scale, exponent and significand of the V scale (s = 2^e * f; a
   // scale that is not finite has f = NaN)
   float ks[2][8], ve[2][8], vf[2][8];
-  float2 pair[2][kRows];                   // what the two threads of a row tell each other
-  float2 ml[kRows];                        // maximum and sum of the rows' partials
+  float2 pair[2][2 * kRows];  // what the two threads of a row tell each other
+  float2 ml[2 * kRows];       // maximum and sum of the rows' partials
 };
 constexpr uint32_t kMiscBytes = (sizeof(Misc) + 15) / 16 * 16;
 
@@ -200,11 +205,25 @@ __device__ __forceinline__ uint32_t core(int r, int c) {
   return (uint32_t)((r >> 3) * (D * 16) + c * 128 + (r & 7) * 16);
 }
 
-// Bounded wait (mbar_wait) that ends at once when another wait of the CTA has given up.
+// Bounded wait that ends at once when another wait of the CTA has given up. The thread is
+// suspended for up to kNap ns at a time: polling warps would take issue slots from the
+// others.
+constexpr uint32_t kNap = 20000;
+__device__ __forceinline__ bool nap(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(kNap)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, Misc& X, int* err) {
-  if (mbar_try_wait(bar, parity)) return;
+  if (nap(bar, parity)) return;
   const uint64_t t0 = global_timer_ns();
-  while (!mbar_try_wait(bar, parity)) {
+  while (!nap(bar, parity)) {
     if (*reinterpret_cast<volatile int*>(&X.abort)) return;
     if (global_timer_ns() - t0 > kWaitLimitNs) {
       *reinterpret_cast<volatile int*>(&X.abort) = 1;
@@ -311,7 +330,7 @@ __device__ __forceinline__ void fewer_regs() {
 }
 
 template <int FMT, int D, int PARTS>
-__global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kernel(const CacheAttnParams p) {
   using H = Shape<FMT, D, PARTS>;
   constexpr bool BF = FMT == QI_KV_BF16;
   constexpr int kPitch = D + 4;  // floats of a row of partial outputs
@@ -319,39 +338,44 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
   Misc& X = *reinterpret_cast<Misc*>(smem + H::kOffMisc);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const qi_kv_layer& c = p.c;
-  const int G = p.group, TT = kRows / G, width = p.heads * D;
-  const int tiles_m = (p.M + TT - 1) / TT;
+  const int G = p.group, TT = kRows / G, width = p.heads * D;  // TT: tokens of a tile
+  const int CT = H::kTiles * TT;
+  const int ctas_m = (p.M + CT - 1) / CT;
   // the last tokens see most: they start first
-  const int split_i = blockIdx.x % p.splits, tile = tiles_m - 1 - (int)(blockIdx.x / p.splits), g = blockIdx.y;
-  const int t0 = tile * TT, ntok = min(TT, p.M - t0);
+  const int split_i = blockIdx.x % p.splits, g = blockIdx.y;
+  const int t0 = (ctas_m - 1 - (int)(blockIdx.x / p.splits)) * CT, ntok = min(CT, p.M - t0);
+  const int ntl = ntok > TT ? 2 : 1;  // tiles with tokens
 
   grid_dep_wait();
-  if (warp == kMmaWarp) {
+  if (warp == H::kMmaWarp) {
     tmem_alloc(&X.tmem, H::kCols);
     tmem_relinquish();
   }
   grid_dep_launch();
-  // Threads r and r + 128 of the softmax warps: query row r = (token, head), half of its
-  // dims (and 64 of a tile's keys). The loads overlap the setup.
+  // Threads r and r + 128 of a tile's softmax warps: query row r = (token, head), half of
+  // its dims (and 64 of a tile's keys). The loads overlap the setup.
   constexpr int DH = D / 2, kRaw = DH / (PARTS == 2 ? 4 : 8);
-  const int r = tid & (kRows - 1), hf = tid >> 7;
-  const int tl = r / G, head = g * G + r - tl * G;
+  const int qt = tid >> 8, r = tid & (kRows - 1), hf = (tid >> 7) & 1;
+  const int rr = qt * kRows + r;  // row of the CTA
+  // its token of the CTA, none (ntok) for rows past the tile's last whole token
+  const int tl = r / G < TT ? min(qt * TT + r / G, ntok) : ntok, head = g * G + r % G;
   uint4 raw[kRaw];
-  if (warp < kSoftWarps) load_row<kRaw, PARTS == 2>(p, (long long)(t0 + min(tl, ntok - 1)) * p.q_st + (long long)head * p.q_sh + hf * DH, raw);
+  if (warp < H::kSoftWarps)
+    load_row<kRaw, PARTS == 2>(p, (long long)(t0 + min(tl, ntok - 1)) * p.q_st + (long long)head * p.q_sh + hf * DH, raw);
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&X.k_full[s], kLoadWarps);
-      mbar_init(&X.v_full[s], kLoadWarps);
+      mbar_init(&X.k_full[s], H::kLoadWarps);
+      mbar_init(&X.v_full[s], H::kLoadWarps);
       mbar_init(&X.k_empty[s], 1);
       mbar_init(&X.v_empty[s], 1);
+      mbar_init(&X.s_full[s], 1);
+      mbar_init(&X.p_full[s], 8);
+      mbar_init(&X.t_full[s], 1);
     }
-    mbar_init(&X.s_full, 1);
-    mbar_init(&X.p_full, kSoftWarps);
-    mbar_init(&X.t_full, 1);
     X.abort = 0;
     fence_barrier_init();
   }
-  if (tid < kRows) {
+  if (tid < kMaxTok) {
     int ps = -1, rw = -1;
     if (tid < ntok) {
       ps = p.pos[t0 + tid], rw = p.rows[t0 + tid];
@@ -365,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
   }
   __syncthreads();
   // segments: the first token of each cache row gathers what its tokens see
-  if (tid < kRows) {
+  if (tid < ntok) {
     int first = -1;
     Seg s = {0, 0x7fffffff, -1, 0, 0};
     if (X.pos[tid] >= 0) {
@@ -409,53 +433,67 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
   const int tbeg = work ? (int)((long long)X.ntiles * split_i / nsplit) : 0;
   const int tend = work ? (int)((long long)X.ntiles * (split_i + 1) / nsplit) : 0;
   const int n = tend - tbeg;
-  if (warp >= kMmaWarp) {
+  if (warp >= H::kMmaWarp) {
     // ------------------------------------------------------------------- MMA
     fewer_regs<H::kRegMma>();
-    if (warp == kMmaWarp) {
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");  // Q is in place
+    if (warp == H::kMmaWarp) {
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * (H::kSoftWarps + 1)) : "memory");  // Q is in place
       const uint32_t sb = smem_u32(smem), lead = lane == 0;
       const uint32_t id_s = idesc_f16(false, kKeys), id_t = idesc_f16(true, D);
-      const uint64_t qd = desc(sb, 128, D * 16);
-      for (int i = 0; i < n; ++i) {
-        const int st = i & 1;
-        const uint32_t ph = (uint32_t)(i >> 1) & 1u;
-        wait(&X.k_full[st], ph, X, p.err);
-        tc_fence_after();
-        // S(i) takes the place of P(i - 1): the product that reads it was issued before
-        const uint64_t kd = desc(sb + H::kOffK + st * H::kT, 128, D * 16);
+      // S(i) of tile t; it takes the place of P(i - 1), whose product was issued before
+      auto scores = [&](int i, int t) {
+        const uint64_t qd = desc(sb + t * PARTS * H::kQ, 128, D * 16);
+        const uint64_t kd = desc(sb + H::kOffK + (i & 1) * H::kT, 128, D * 16);
 #pragma unroll
         for (int q = PARTS - 1; q >= 0; --q)
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma_ss(lead, tmem, qd + (uint64_t)(q * (H::kQ >> 4) + k * 16), kd + (uint64_t)(k * 16), id_s,
+            umma_ss(lead, tmem + 128 * t, qd + (uint64_t)(q * (H::kQ >> 4) + k * 16), kd + (uint64_t)(k * 16), id_s,
                     q < PARTS - 1 || k > 0 ? 1u : 0u);
-        commit(lead, &X.s_full);
-        commit(lead, &X.k_empty[st]);
-        const uint64_t vd = desc(sb + H::kOffV + st * H::kT, D * 16, 128);
-        wait(&X.v_full[st], ph, X, p.err);
-        wait(&X.p_full, (uint32_t)i & 1u, X, p.err);
+        commit(lead, &X.s_full[t]);
+        if (t == ntl - 1) commit(lead, &X.k_empty[i & 1]);
+      };
+      if (n > 0) {
+        wait(&X.k_full[0], 0u, X, p.err);
         tc_fence_after();
-#pragma unroll
-        for (int q = PARTS - 1; q >= 0; --q)
-#pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            // 16 keys: 8 columns of P for each part; 2 key groups of V
-            umma_ts(lead, tmem + H::kColT, tmem + 16 * k + 8 * q, vd + (uint64_t)(k * 2 * D), id_t,
-                    q < PARTS - 1 || k > 0 ? 1u : 0u);
-        commit(lead, &X.v_empty[st]);
+        for (int t = 0; t < ntl; ++t) scores(0, t);
       }
-      commit(lead, &X.t_full);
+      for (int i = 0; i < n; ++i) {
+        const int st = i & 1;
+        for (int t = 0; t < ntl; ++t) {
+          if (t == 0) wait(&X.v_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);
+          wait(&X.p_full[t], (uint32_t)i & 1u, X, p.err);
+          tc_fence_after();
+          const uint64_t vd = desc(sb + H::kOffV + st * H::kT, D * 16, 128);
+#pragma unroll
+          for (int q = PARTS - 1; q >= 0; --q)
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              // 16 keys: 8 columns of P for each part; 2 key groups of V
+              umma_ts(lead, tmem + H::kColT + D * t, tmem + 128 * t + 16 * k + 8 * q, vd + (uint64_t)(k * 2 * D), id_t,
+                      q < PARTS - 1 || k > 0 ? 1u : 0u);
+          if (t == ntl - 1) commit(lead, &X.v_empty[st]);
+          if (i + 1 < n) {
+            if (t == 0) {
+              wait(&X.k_full[st ^ 1], (uint32_t)((i + 1) >> 1) & 1u, X, p.err);
+              tc_fence_after();
+            }
+            scores(i + 1, t);
+          } else {
+            commit(lead, &X.t_full[t]);
+          }
+        }
+      }
       __syncwarp();
     }
     __syncthreads();
-  } else if (warp >= kLoadWarp) {
+  } else if (warp >= H::kLoadWarp) {
     // ------------------------------------------------------------- producers
     if constexpr (H::kRegLoad > H::kRegLaunch) more_regs<H::kRegLoad>();
     else fewer_regs<H::kRegLoad>();
-    const int lt = tid - 32 * kLoadWarp, lw = warp - kLoadWarp;
+    const int lt = tid - 32 * H::kLoadWarp, lw = warp - H::kLoadWarp;
     constexpr int kCh = D * (BF ? 2 : 1) / 16;        // 16-byte chunks of a key
-    constexpr int kN = kKeys * kCh / kLoadThreads;    // of a thread
+    constexpr int kN = kKeys * kCh / (32 * H::kLoadWarps);    // of a thread
     // a warp takes 32 keys; one of its loads is 8 keys x 4 chunks: whole lines, and the
     // lanes of a store phase hold 8 keys
     auto place = [&](int j, int& r, int& ch) {
@@ -516,44 +554,54 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       constexpr int kB = kN / 2;  // chunks of a block
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        uint32_t mx = 0u;
+        uint32_t m2 = 0u;  // largest magnitudes of the low and the high halves
 #pragma unroll
-        for (int j = b * kB; j < (b + 1) * kB; ++j) {
-          const uint32_t w[4] = {regs[j].x, regs[j].y, regs[j].z, regs[j].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            mx = max(mx, max((w[e] << 16) & 0x7fff0000u, w[e] & 0x7fff0000u));
-        }
-        mx = __reduce_max_sync(kAll, mx);
-        if (mx >= 0x7f800000u) {  // the largest of the finite values
+        for (int j = b * kB; j < (b + 1) * kB; ++j)
+          m2 = __vmaxu2(__vmaxu2(m2, __vmaxu2(regs[j].x & kMag, regs[j].y & kMag)),
+                        __vmaxu2(regs[j].z & kMag, regs[j].w & kMag));
+        uint32_t mx = __reduce_max_sync(kAll, max(m2 >> 16, m2 & 0xffffu));
+        const bool odd = mx >= 0x7f80u;  // infinities or NaN: the scale goes by the finite values
+        if (odd) {
           mx = 0u;
 #pragma unroll
           for (int j = b * kB; j < (b + 1) * kB; ++j) {
             const uint32_t w[4] = {regs[j].x, regs[j].y, regs[j].z, regs[j].w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t lo = (w[e] << 16) & 0x7fff0000u, hi = w[e] & 0x7fff0000u;
-              mx = max(mx, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+            for (int x = 0; x < 4; ++x) {
+              const uint32_t lo = w[x] & 0x7fffu, hi = (w[x] >> 16) & 0x7fffu;
+              mx = max(mx, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
             }
           }
           mx = __reduce_max_sync(kAll, mx);
         }
         // largest value 2^(e - 127) * [1, 2): scale 2^(e - 127 - 14), for e in 15..253 (the
         // scale and its reciprocal are normal); tiny blocks are left with a smaller maximum
-        const uint32_t e = min(max(mx >> 23, 15u), 253u);
-        const float inv = __uint_as_float((268u - e) << 23);
+        const uint32_t e = min(max(mx >> 7, 15u), 253u);
         if (lane == 0) {
           if (k_side) X.ks[st][lw * 2 + b] = __uint_as_float((e - 14u) << 23);
           else X.ve[st][lw * 2 + b] = (float)((int)e - 141), X.vf[st][lw * 2 + b] = 1.f;
         }
+        // bf16 to fp16 at that scale: the exponent field moves by e - 29 (from e to 29, that
+        // of 2^14) and the significand gains three zeros; values below fp16's normal range, 2^-28
+        // of the largest, come out off by less than that. Both halves at once: neither borrows
+        // nor overflows. (Blocks with infinities or NaN, and tiny ones, whose exponent is below
+        // 29, go through fp32.)
+        const uint32_t off2 = ((e - 29u) << 7) * 0x10001u;
+        auto half2_of = [&](uint32_t w) -> uint32_t { return ((__vmaxu2(w & kMag, off2) - off2) << 3) | (w & ~kMag); };
 #pragma unroll
         for (int j = b * kB; j < (b + 1) * kB; ++j) {
           int r, ch;
           place(j, r, ch);
           const uint32_t w[4] = {regs[j].x, regs[j].y, regs[j].z, regs[j].w};
           uint32_t h[4];
+          if (odd || e < 29u) {
+            const float inv = __uint_as_float((268u - e) << 23);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) h[x] = f16x2(bf16lo(w[x]) * inv, bf16hi(w[x]) * inv);
+            for (int x = 0; x < 4; ++x) h[x] = f16x2(bf16lo(w[x]) * inv, bf16hi(w[x]) * inv);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) h[x] = half2_of(w[x]);
+          }
           *reinterpret_cast<uint4*>(t + core<D>(r, ch)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
       }
@@ -598,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
   } else {
     // --------------------------------------------------------------- softmax
     more_regs<H::kRegSoft>();
-    auto pair_bar = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };
+    auto pair_bar = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * qt + (warp & 3)) : "memory"); };
     const int ps = tl < ntok ? X.pos[tl] : -1;
     // the row's segment, by cache row (segments left out have no entry)
     int seg = -1;
@@ -613,9 +661,9 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
         const float2 x = row_pair<PARTS == 2>(raw, i, p.dtype);
         am = fmaxf(am, fmaxf(fabsf(x.x), fabsf(x.y)));
       }
-      X.pair[hf][r].x = am;
+      X.pair[hf][rr].x = am;
       pair_bar();
-      am = fmaxf(am, X.pair[hf ^ 1][r].x);
+      am = fmaxf(am, X.pair[hf ^ 1][rr].x);
       float inv = live ? 1.f : 0.f;
       const uint32_t e = __float_as_uint(am) >> 23;
       if (live && e > 0 && e < 253) {
@@ -632,14 +680,16 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
         }
 #pragma unroll
         for (int q = 0; q < PARTS; ++q)
-          *reinterpret_cast<uint4*>(smem + q * H::kQ + core<D>(r, hf * (DH / 8) + ch)) =
+          *reinterpret_cast<uint4*>(smem + (qt * PARTS + q) * H::kQ + core<D>(r, hf * (DH / 8) + ch)) =
               make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
       }
       fence_async_smem();
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * (H::kSoftWarps + 1)) : "memory");
     const Seen<kKeys> mine = seen_range<kKeys>(live ? ps : 0, live ? window_start(ps, p.window) : 0, p.sinks);
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t srow = trow + 128 * qt + 64 * hf;          // this half's scores
+    const uint32_t orow = trow + H::kColT + D * qt + DH * hf;  // and dims
 
     float m = -INFINITY, l = 0.f;  // maximum of the scores (log2 units), sum of 2^(x - m)
     f2 o[DH / 2];                  // sum of 2^(x - m) v (this half's dims; l: this half's keys)
@@ -654,14 +704,15 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
         for (int d = 0; d < DH / 2; ++d) o[d] = mul2(o[d], f);
       }
       const f2 f = pack2(ob, ob);
-      tmem_each16<DH / 16>(trow + H::kColT + hf * DH, [&](int c, const uint32_t(&t)[16]) {
+      tmem_each16<DH / 16>(orow, [&](int c, const uint32_t(&t)[16]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           o[8 * c + j] = fma2(pack2(__uint_as_float(t[2 * j]), __uint_as_float(t[2 * j + 1])), f, o[8 * c + j]);
       });
     };
     int si = 0;
-    for (int i = 0; i < n; ++i) {
+    const int n_mine = qt < ntl ? n : 0;
+    for (int i = 0; i < n_mine; ++i) {
       const int at = tbeg + i, st = i & 1;
       while (si + 1 < X.nseg && at >= X.segs[si + 1].first) ++si;
       const Seen<kKeys> list = seen_range<kKeys>(X.segs[si].hi, X.segs[si].lo, X.segs[si].sinks);
@@ -681,14 +732,13 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       float ks[4], ve[4];  // of this half's 4 blocks
 #pragma unroll
       for (int c = 0; c < 4; ++c) ks[c] = qs * X.ks[st][4 * hf + c], ve[c] = X.ve[st][4 * hf + c];
-      wait(&X.s_full, (uint32_t)i & 1u, X, p.err);  // S(i), and T(i - 1) before it
+      wait(&X.s_full[qt], (uint32_t)i & 1u, X, p.err);  // S(i), and T(i - 1) before it
       tc_fence_after();
       if (i > 0) add_tile();
-      const uint32_t tcol = trow + 64 * hf;  // this half's scores
       // pass 1: the maxima of the scores and of score + log2(V scale)
       float mx = -INFINITY, R = -INFINITY;
       auto maxima = [&](auto some_masked) {
-        tmem_each16<4>(tcol, [&](int c, const uint32_t(&s)[16]) {
+        tmem_each16<4>(srow, [&](int c, const uint32_t(&s)[16]) {
           float a4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           const uint32_t mk = decltype(some_masked)::value ? mask16(64 * hf + 16 * c) : 0u;
 #pragma unroll
@@ -706,9 +756,9 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       };
       if (masked) maxima(True{});
       else maxima(False{});
-      X.pair[hf][r] = make_float2(mx, R);
+      X.pair[hf][rr] = make_float2(mx, R);
       pair_bar();  // (the next tile's values are written after both halves' weights of this one)
-      const float2 other = X.pair[hf ^ 1][r];
+      const float2 other = X.pair[hf ^ 1][rr];
       R = fmaxf(R, other.y);
       const float mn = fmaxf(m, fmaxf(mx, other.x));
       oa = m == -INFINITY ? 1.f : ex2(m - mn);  // nothing summed yet: nothing to rescale
@@ -720,7 +770,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       // pass 2: weights and their parts
       f2 sum[2] = {0ull, 0ull};
       auto weights = [&](auto some_masked) {
-        tmem_each16<4>(tcol, [&](int c, const uint32_t(&s)[16]) {
+        tmem_each16<4>(srow, [&](int c, const uint32_t(&s)[16]) {
           // 2^(x - m) * fv = 2^(x + log2(V scale) - R + lift)
           const float fv = X.vf[st][4 * hf + c] * ex2(fminf(ve[c] + rest, 126.f));
           const f2 fk2 = pack2(ks[c], ks[c]), fv2 = pack2(fv, fv), mr2 = pack2(-mr, -mr);
@@ -748,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
           }
           // the block's 16 columns of S are read: its P takes them
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) tmem_put8(tcol + 16 * c + 8 * q, part[q]);
+          for (int q = 0; q < PARTS; ++q) tmem_put8(srow + 16 * c + 8 * q, part[q]);
         });
       };
       if (masked) weights(True{});
@@ -758,11 +808,13 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&X.p_full);
+      if (lane == 0) mbar_arrive(&X.p_full[qt]);
     }
-    wait(&X.t_full, 0u, X, p.err);
-    tc_fence_after();
-    if (n > 0) add_tile();
+    if (n_mine > 0) {
+      wait(&X.t_full[qt], 0u, X, p.err);
+      tc_fence_after();
+      add_tile();
+    }
 
     // ---------------------------------------------------------------- output
     const bool row_in = tl < ntok && work && !(ps >= 0 && seg < 0);  // rows left out write nothing
@@ -779,9 +831,9 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
       for (int d = 0; d < DH; ++d) bad |= !(fabsf(of[d]) <= 3.402823466e38f);
     }
     pair_bar();
-    X.pair[hf][r] = make_float2(l, bad ? 1.f : 0.f);
+    X.pair[hf][rr] = make_float2(l, bad ? 1.f : 0.f);
     pair_bar();
-    const float2 other = X.pair[hf ^ 1][r];
+    const float2 other = X.pair[hf ^ 1][rr];
     l = hf ? other.x + l : l + other.x;
     if constexpr (BF) {
       if (row_in && live && (bad || other.y != 0.f)) {
@@ -792,14 +844,16 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
     }
     // The split's partial (relative to m) into shared memory, in the place of Q and K, which
     // all products are done with: rows of D + 4 floats, so that rows 8 apart share a bank.
-    float* po = reinterpret_cast<float*>(smem) + r * kPitch + hf * DH;
+    if (n > 0)
+      for (int t = 0; t < ntl; ++t) wait(&X.t_full[t], 0u, X, p.err);
+    float* po = reinterpret_cast<float*>(smem) + rr * kPitch + hf * DH;
 #pragma unroll
     for (int d = 0; d < DH; d += 4) *reinterpret_cast<float4*>(po + d) = make_float4(of[d], of[d + 1], of[d + 2], of[d + 3]);
-    if (hf == 0) X.ml[r] = make_float2(m, l);
+    if (hf == 0) X.ml[rr] = make_float2(m, l);
     tc_fence_before();
     __syncthreads();
   }
-  if (warp == kMmaWarp) {
+  if (warp == H::kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, H::kCols);
   }
@@ -811,8 +865,9 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
     cluster_wait();
   }
   const int rows_in = ntok * G, r0 = rows_in * split_i / C, r1 = rows_in * (split_i + 1) / C;
-  for (int e = tid; e < (r1 - r0) * (D / 8); e += kThreads) {
-    const int rr = r0 + e / (D / 8), d = e % (D / 8) * 8, tt = rr / G;
+  for (int e = tid; e < (r1 - r0) * (D / 8); e += H::kThreads) {
+    const int x = r0 + e / (D / 8), d = e % (D / 8) * 8, tt = x / G, hh = x - tt * G;
+    const int rr = tt < TT ? x : kRows + x - TT * G;  // its row of the CTA
     if (X.pos[tt] >= 0) {  // a row that was left out
       bool in = false;
       for (int s = 0; s < X.nseg; ++s) in |= X.segs[s].row == X.row[tt];
@@ -834,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D, PARTS>::kCtas) prompt_
     const float inv = ll != 0.f ? 1.f / ll : 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= inv;
-    emit<8>(p, t0 + tt, (g * G + rr - tt * G) * D + d, width, v);
+    emit<8>(p, t0 + tt, (g * G + hh) * D + d, width, v);
   }
   if (C > 1) {  // the others are done with this CTA's shared memory
     __syncwarp();
@@ -858,10 +913,10 @@ cudaError_t launch(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
     return r != cudaSuccess ? r : a.numRegs < H::kRegLaunch ? cudaErrorInvalidConfiguration : cudaSuccess;
   }();
   if (regs != cudaSuccess) return regs;
-  const int TT = kRows / p.group;
+  const int CT = H::kTiles * (kRows / p.group);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.M + TT - 1) / TT * p.splits), p.c.kv_heads, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.gridDim = dim3((unsigned)((p.M + CT - 1) / CT * p.splits), p.c.kv_heads, 1);
+  cfg.blockDim = dim3(H::kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
