@@ -78,10 +78,11 @@ class KVCache:
                               self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1], None, 0, 0, 0)
 
     def _errors(self) -> torch.Tensor:
-        err = self.__dict__.get("_err")
-        if err is None:
-            err = self._err = torch.zeros(1, dtype=torch.int32, device=self.k.device)
-        return err
+        try:
+            return self._err
+        except AttributeError:
+            self._err = torch.zeros(1, dtype=torch.int32, device=self.k.device)
+            return self._err
 
     def check(self) -> None:
         """Raise if an `attend` or `append` of this cache met a position, cache row or page
@@ -93,6 +94,11 @@ class KVCache:
     def _tokens(self, M: int, rows: torch.Tensor, pos: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """Rows and positions of M tokens as int32 on the device; those given on the host are
         checked there."""
+        dev = self.k.device
+        if (rows.dtype is torch.int32 and pos.dtype is torch.int32 and rows.shape == pos.shape == (M,)
+                and rows.device == dev and pos.device == dev and rows.is_contiguous() and pos.is_contiguous()
+                and dev.type == "cuda"):
+            return rows, pos
         out = []
         for name, t, lo, hi in (("rows", rows, 0, self.max_batch), ("pos", pos, -1, self.max_len)):
             if t.dim() != 1 or t.shape[0] != M:
@@ -116,7 +122,6 @@ class KVCache:
         if t.stride(2) != 1:
             raise ValueError(f"the last dimension of {name} must be contiguous")
 
-    @torch.no_grad()
     def attend(self, layer: int, q: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor, window: int = 0,
                sinks: int = 0, query_run: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
         """Grouped-query attention of M query tokens over layer `layer` (qi_cache_attention).
@@ -134,6 +139,45 @@ class KVCache:
 
         Scores, softmax and sums are fp32; q and the probabilities keep at least 22 bits for
         an 8-bit cache, 24 (16 for 16-bit q) for a bf16 one."""
+        # what the shapes alone decide is checked once for each kind of call
+        key = (layer, q.shape, q.stride(), q.dtype, window, sinks, query_run)
+        try:
+            plan = self._plans.get(key)
+        except AttributeError:
+            self._plans, plan = {}, None
+        if plan is None:
+            plan = self._attend_plan(*key[:1], q, *key[4:])
+            if len(self._plans) >= 4096:
+                self._plans.clear()
+            self._plans[key] = plan
+        dev = self.k.device
+        if q.device != dev:
+            _require(q, "q", dev)
+        M = q.shape[0]
+        rows, pos = self._tokens(M, rows, pos)
+        if out is None:
+            out = q.new_empty(q.shape)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {q.device}")
+        elif out.data_ptr() % 16:
+            raise ValueError("out must be 16-byte aligned")
+        elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+            raise ValueError("out must not share q's storage")
+        if M == 0:
+            return out
+        d, st, sh, dtype, heads, window, sinks, query_run, part_floats, n_counters = plan
+        with _lib.on_device(dev):
+            stream = torch._C._cuda_getCurrentRawStream(dev.index)
+            part, counters, _keep = _lib.scratch(dev, stream, 4 * part_floats, n_counters) if n_counters else (0, 0, None)
+            code = _lib.lib().qi_cache_attention(
+                d, q.data_ptr(), st, sh, dtype, heads, rows.data_ptr(), pos.data_ptr(), M, window, sinks, query_run,
+                out.data_ptr(), part, part_floats, counters, n_counters, self._errors().data_ptr(), stream)
+        if code:
+            _lib.check(code, "qi_cache_attention")
+        return out
+
+    def _attend_plan(self, layer: int, q: torch.Tensor, window: int, sinks: int, query_run: int) -> tuple:
+        """The arguments of an `attend` call that its shapes decide, checked, and its scratch."""
         d = self.layer(layer)
         self._operand("q", q, None)
         M, heads, D = q.shape
@@ -143,38 +187,15 @@ class KVCache:
             raise ValueError(f"{heads} query heads are not 1 to 8 for each of {d.kv_heads} KV heads")
         if window < 0 or sinks < 0 or query_run < 0:
             raise ValueError("window, sinks and query_run must not be negative")
-        rows, pos = self._tokens(M, rows, pos)
-        if out is None:
-            out = torch.empty((M, heads, D), dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {q.device}")
-        elif out.data_ptr() % 16:
-            raise ValueError("out must be 16-byte aligned")
-        elif out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
-            raise ValueError("out must not share q's storage")
-        if M == 0:
-            return out
         lim = 2**31 - 1
         window, sinks, query_run = min(window, lim), min(sinks, lim), min(query_run, lim)
-        with _lib.on_device(self.k.device):
-            L = _lib.lib()
-            plan = self.__dict__.setdefault("_plans", {})
-            key = (M, heads, window, sinks, query_run)
-            need = plan.get(key)
-            if need is None:
-                a, b = C.c_longlong(), C.c_longlong()
-                _lib.check(L.qi_cache_attention_scratch(C.byref(d), heads, M, window, sinks, query_run, C.byref(a),
-                                                        C.byref(b)), "qi_cache_attention_scratch")
-                if len(plan) >= 4096:
-                    plan.clear()
-                need = plan[key] = (a.value, b.value)
-            stream = _lib.stream_ptr(self.k.device)
-            part, counters, _keep = _lib.scratch(self.k.device, stream, 4 * need[0], need[1])
-            _lib.check(L.qi_cache_attention(
-                C.byref(d), q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPES[q.dtype], heads, rows.data_ptr(),
-                pos.data_ptr(), M, window, sinks, query_run, out.data_ptr(), part, need[0], counters, need[1],
-                self._errors().data_ptr(), stream), "qi_cache_attention")
-        return out
+        a, b = C.c_longlong(), C.c_longlong()
+        if M:
+            with _lib.on_device(self.k.device):
+                _lib.check(_lib.lib().qi_cache_attention_scratch(C.byref(d), heads, M, window, sinks, query_run,
+                                                                 C.byref(a), C.byref(b)), "qi_cache_attention_scratch")
+        return (C.byref(d), q.stride(0), q.stride(1), _lib.DTYPES[q.dtype], heads, window, sinks, query_run, a.value,
+                b.value)
 
     # storage management hooks of the paged cache (every slot of a packed row exists)
     def reserve(self, row: int, length: int) -> None:
@@ -360,7 +381,6 @@ class Kv8Cache(KVCache):
                               self.v_scale[i].data_ptr(), self.FORMATS[self.format][0], self.block_tokens,
                               self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1], None, 0, 0, 0)
 
-    @torch.no_grad()
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor) -> None:
         """Write M tokens' keys and values into layer `layer` (qi_kv8_append): token t at
         position pos[t] of cache row rows[t]; pos[t] = -1 skips it.
@@ -374,25 +394,39 @@ class Kv8Cache(KVCache):
         the same row and position the later one is kept. A value that is not finite makes
         its block's scale NaN, and so the outputs that read the block. rows and pos as in
         `attend`."""
-        d = self.layer(layer)
-        self._operand("k", k, d.kv_heads)
-        self._operand("v", v, d.kv_heads)
-        if v.dtype != k.dtype or v.shape != k.shape:
-            raise ValueError(f"k and v must have one shape and dtype, got {tuple(k.shape)} {k.dtype} and "
-                             f"{tuple(v.shape)} {v.dtype}")
-        if d.head_dim not in (64, 128):
-            raise ValueError(f"head_dim must be 64 or 128, got {d.head_dim}")
+        key = (layer, k.shape, k.stride(), v.shape, v.stride(), k.dtype, v.dtype)
+        try:
+            d = self._append_plans.get(key)
+        except AttributeError:
+            self._append_plans, d = {}, None
+        if d is None:
+            layer_ = self.layer(layer)
+            self._operand("k", k, layer_.kv_heads)
+            self._operand("v", v, layer_.kv_heads)
+            if v.dtype != k.dtype or v.shape != k.shape:
+                raise ValueError(f"k and v must have one shape and dtype, got {tuple(k.shape)} {k.dtype} and "
+                                 f"{tuple(v.shape)} {v.dtype}")
+            if layer_.head_dim not in (64, 128):
+                raise ValueError(f"head_dim must be 64 or 128, got {layer_.head_dim}")
+            if len(self._append_plans) >= 4096:
+                self._append_plans.clear()
+            d = self._append_plans[key] = C.byref(layer_)
+        dev = self.k.device
+        if k.device != dev or v.device != dev:
+            _require(k, "k", dev)
+            _require(v, "v", dev)
         M = k.shape[0]
         rows, pos = self._tokens(M, rows, pos)
         if M == 0:
             return
-        with _lib.on_device(self.k.device):
-            _lib.check(_lib.lib().qi_kv8_append(
-                C.byref(d), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        with _lib.on_device(dev):
+            code = _lib.lib().qi_kv8_append(
+                d, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
                 _lib.DTYPES[k.dtype], rows.data_ptr(), pos.data_ptr(), M, self._errors().data_ptr(),
-                _lib.stream_ptr(self.k.device)), "qi_kv8_append")
+                torch._C._cuda_getCurrentRawStream(dev.index))
+        if code:
+            _lib.check(code, "qi_kv8_append")
 
-    @torch.no_grad()
     def values(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
         """What layer `layer` stands for: K and V (max_batch, kv_heads, max_len, head_dim)
         fp32 (qi_kv8_values). Dead positions give whatever their codes say."""
@@ -400,7 +434,7 @@ class Kv8Cache(KVCache):
         _require(self.k_scale, "values", self.k.device)
         if d.head_dim not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {d.head_dim}")
-        k = torch.empty(self.k.shape[1:], dtype=torch.float32, device=self.k.device)
+        k = self.k_scale.new_empty(self.k.shape[1:])
         v = torch.empty_like(k)
         with _lib.on_device(self.k.device):
             _lib.check(_lib.lib().qi_kv8_values(C.byref(d), k.data_ptr(), v.data_ptr(),

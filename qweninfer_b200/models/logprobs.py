@@ -26,7 +26,6 @@ class TokenLogprobs:
     top_logprobs: torch.Tensor | None
 
 
-@torch.no_grad()
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0) -> TokenLogprobs:
     """Per row of `logits` (M, V) (float32, bfloat16 or float16; rows may be strided):
     log softmax at targets[t], the entropy of the distribution, and its `top` (0..32, at
@@ -59,17 +58,21 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
             raise ValueError(f"targets on {targets.device}, logits on {logits.device}")
         targets = targets.contiguous()
     dev = logits.device
-    f32 = dict(dtype=torch.float32, device=dev)
-    r = TokenLogprobs(torch.empty(M, **f32) if targets is not None else None, torch.empty(M, **f32),
-                      torch.empty(M, top, dtype=torch.int32, device=dev) if top else None,
-                      torch.empty(M, top, **f32) if top else None)
+    # the outputs share one allocation
+    buf = torch.empty(2 * M * (1 + top), dtype=torch.float32, device=dev)
+    if top:
+        lp, ent, ids, lps = buf.split((M, M, M * top, M * top))
+        r = TokenLogprobs(lp if targets is not None else None, ent, ids.view(torch.int32).view(M, top), lps.view(M, top))
+    else:
+        lp, ent = buf.split(M) if M else (buf, buf)
+        r = TokenLogprobs(lp if targets is not None else None, ent, None, None)
     if M == 0:
         return r
     with _lib.on_device(dev):
         L = _lib.lib()
         stream = _lib.stream_ptr(dev)
         nbytes = L.qi_token_logprobs_scratch(M, V)
-        data, counters, _keep = _lib.scratch(dev, stream, nbytes, M if nbytes else 0)
+        data, counters, _keep = _lib.scratch(dev, stream, nbytes, M) if nbytes else (0, 0, None)
         _lib.check(L.qi_token_logprobs(
             logits.data_ptr(), _lib.DTYPES[logits.dtype], logits.stride(0) if M > 1 else V, _lib.ptr(targets),
             int(targets is not None and targets.dtype == torch.int64), M, V, top, _lib.ptr(r.logprob),
