@@ -12,7 +12,7 @@
 // zero-filled, so what dead positions hold (NaN included) never enters a product.
 //
 // Each warp streams its own granules through a private ring of shared memory with cp.async
-// and never waits for another warp before the merge. A call is bound by the cache's bytes,
+// and never waits for another warp before the sums. A call is bound by the cache's bytes,
 // so what counts is bytes in flight: 16 warps of an SM with two granules each requested.
 //
 // The group's query heads (at most 8) are rows of m16n8k16 MMAs. Row h holds the high part
@@ -89,8 +89,16 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Granules a split has at least, so that its warps have two each.
-constexpr int kMinSplit = 2 * kWarps;
+// Granules a split has at least: one for each warp.
+constexpr int kMinSplit = kWarps;
+constexpr int kMaxCluster = 8;
+
+// shared memory of CTA w of the cluster
+__device__ __forceinline__ float peer(const float* x, int w) {
+  float r;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r) : "r"(map_rank(x, (uint32_t)w)) : "memory");
+  return r;
+}
 
 // F16 products for 8-bit codes, bf16 for a bf16 cache; P3: three parts of q and p (bf16).
 template <int FMT, int D, bool P3>
@@ -125,8 +133,9 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
   }
   const Seen<kGran> seen = seen_range<kGran>(ps, window_start(ps, p.window), p.sinks);
   const int nsplit = min(p.splits, (seen.n + kMinSplit - 1) / kMinSplit);
-  if (split_i >= nsplit) return;
-  const int gbeg = (int)((long long)seen.n * split_i / nsplit), gend = (int)((long long)seen.n * (split_i + 1) / nsplit);
+  if (nsplit == 1 ? split_i > 0 : split_i / p.cluster * p.cluster >= nsplit) return;  // clusters without keys
+  // (a split without keys in a cluster that has some gets an empty run)
+  const int gbeg = (int)((long long)seen.n * split_i / nsplit), gend = split_i < nsplit ? (int)((long long)seen.n * (split_i + 1) / nsplit) : gbeg;
 
   const uint32_t ring = smem_u32(smem) + (uint32_t)(warp * S::kStages * S::kStage);
   // granule i (its place in the list) into ring stage st; nothing for i >= gend
@@ -340,10 +349,17 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
     if (qd == 0) w[D] = m, w[D + 1] = l;
   }
   __syncthreads();
+  // The splits of a unit are clusters of p.cluster CTAs: they exchange their sums through
+  // distributed shared memory, each CTA adding up a share of the outputs in split order. Over
+  // more than one cluster, the clusters' sums go through global memory to the last to arrive.
   const long long unit = (long long)tok * c.kv_heads + g;
-  float* part = p.part + (unit * p.splits + split_i) * (long long)(G * kPart);
-    for (int e = tid; e < G * D / 2; e += kThreads) {
-    const int h = e / (D / 2), d = 2 * (e - h * (D / 2));
+  const int C = p.cluster, rank = split_i % C, first = split_i - rank;
+  const int here = min(C, nsplit - first);                // splits of this cluster with keys
+  const int clusters = (nsplit + C - 1) / C;
+  float* sums = wp + kWarps * G * kPart;                  // this split's: [head][D values, m, l]
+  constexpr int kPairs = D / 2;
+  for (int e = tid; e < G * kPairs; e += kThreads) {
+    const int h = e / kPairs, d = 2 * (e - h * kPairs);
     float mm, ll, a, b;
     merge2<D>([&](int w, int i) { return wp[(w * G + h) * kPart + i]; }, kWarps, d, mm, ll, a, b);
     if (nsplit == 1) {
@@ -351,32 +367,52 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
       const float v[2] = {a * inv, b * inv};
       emit<2>(p, tok, g * G * D + h * D + d, width, v);
     } else {
-      __stcg(reinterpret_cast<float2*>(part + h * kPart + d), make_float2(a, b));
-      if (d == 0) __stcg(reinterpret_cast<float2*>(part + h * kPart + D), make_float2(mm, ll));
+      sums[h * kPart + d] = a, sums[h * kPart + d + 1] = b;
+      if (d == 0) sums[h * kPart + D] = mm, sums[h * kPart + D + 1] = ll;
     }
   }
   if (nsplit == 1) return;
-  // the last split of the unit merges them all, in split order, and leaves the counter zero
-  __syncthreads();
-  if (tid == 0) last = atomic_add_acq_rel(p.counters + unit, 1u) == (unsigned)(nsplit - 1);
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  float* part = p.part + unit * (p.splits / C) * (long long)(G * kPart);  // [cluster][head][D + 2]
+  const int e0 = G * kPairs * rank / C, e1 = G * kPairs * (rank + 1) / C;
+  for (int e = e0 + tid; e < e1; e += kThreads) {
+    const int h = e / kPairs, d = 2 * (e - h * kPairs);
+    float mm, ll, a, b;
+    merge2<D>([&](int w, int i) { return peer(sums + h * kPart + i, w); }, here, d, mm, ll, a, b);
+    if (clusters == 1) {
+      const float inv = ll != 0.f ? 1.f / ll : 0.f;
+      const float v[2] = {a * inv, b * inv};
+      emit<2>(p, tok, g * G * D + h * D + d, width, v);
+    } else {
+      float* x = part + (long long)(first / C) * (G * kPart) + h * kPart;
+      __stcg(reinterpret_cast<float2*>(x + d), make_float2(a, b));
+      if (d == 0) __stcg(reinterpret_cast<float2*>(x + D), make_float2(mm, ll));
+    }
+  }
+  __syncwarp();
+  cluster_arrive();  // sums read, and the cluster's share of part written
+  cluster_wait();
+  if (clusters == 1 || rank != 0) return;
+  if (tid == 0) last = atomic_add_acq_rel(p.counters + unit, 1u) == (unsigned)(clusters - 1);
   __syncthreads();
   if (!last) return;
-  const float* parts = p.part + unit * p.splits * (long long)(G * kPart);
-    for (int e = tid; e < G * D / 2; e += kThreads) {
-    const int h = e / (D / 2), d = 2 * (e - h * (D / 2));
+  for (int e = tid; e < G * kPairs; e += kThreads) {
+    const int h = e / kPairs, d = 2 * (e - h * kPairs);
     float mm, ll, a, b;
-    merge2<D>([&](int w, int i) { return __ldcg(parts + ((long long)w * G + h) * kPart + i); }, nsplit, d, mm, ll, a, b);
+    merge2<D>([&](int w, int i) { return __ldcg(part + ((long long)w * G + h) * kPart + i); }, clusters, d, mm, ll, a, b);
     const float inv = ll != 0.f ? 1.f / ll : 0.f;
     const float v[2] = {a * inv, b * inv};
     emit<2>(p, tok, g * G * D + h * D + d, width, v);
   }
-  if (tid == 0) p.counters[unit] = 0u;
+  if (tid == 0) p.counters[unit] = 0u;  // as the next call expects it
 }
 
 template <int FMT, int D, bool P3>
 cudaError_t launch_token(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
   auto kernel = cache_attention_kernel<FMT, D, P3>;
-  constexpr size_t merge = sizeof(float) * kWarps * kMaxGroup * (D + 2);
+  constexpr size_t merge = sizeof(float) * (kWarps + 1) * kMaxGroup * (D + 2);
   constexpr size_t smem = Shape<FMT, D>::kRing > merge ? Shape<FMT, D>::kRing : merge;
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), (int)smem);
   if (e != cudaSuccess) return e;
@@ -385,11 +421,20 @@ cudaError_t launch_token(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (p.cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)p.cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -411,14 +456,16 @@ long long seen_at_most(const qi_kv_layer& c, int window, int sinks) {
   return window > 0 && w < c.max_len ? w : c.max_len;
 }
 
-// Key splits of the per-token kernel: four CTAs for every SM, as far as rows are long
-// enough to give each split kMinSplit granules.
+// Key splits of the per-token kernel: four CTAs for every SM (what its shared memory
+// admits), as far as rows are long enough to give each split kMinSplit granules; whole
+// clusters when there are more than fit one.
 int token_splits(const qi_kv_layer& c, int M, int window, int sinks) {
   const long long gran = seen_at_most(c, window, sinks) / kGran + 2, units = (long long)M * c.kv_heads;
   const long long most = (gran + kMinSplit - 1) / kMinSplit;
-  long long want = (4LL * sm_count() + units - 1) / units;
+  long long want = 4LL * sm_count() / units;
   want = want > most ? most : want;
-  return (int)(want > kMaxAttnSplits ? kMaxAttnSplits : want < 1 ? 1 : want);
+  want = want > kMaxAttnSplits ? kMaxAttnSplits : want < 1 ? 1 : want;
+  return (int)(want > kMaxCluster ? want / kMaxCluster * kMaxCluster : want);
 }
 
 // Key splits of the prompt kernel, the CTAs of a cluster: as many as fill the CTAs that are
@@ -435,8 +482,8 @@ int prompt_tiles(int M, int group) { return (M + kPromptRows / group - 1) / (kPr
 
 void sizes(CacheAttnPlan& r, const qi_kv_layer& c, int heads, int M) {
   r.part_floats = r.counters = 0;
-  if ((!r.prompt || r.singles) && r.token_splits > 1) {
-    r.part_floats = (long long)M * heads * r.token_splits * (c.head_dim + 2);
+  if ((!r.prompt || r.singles) && r.token_splits > kMaxCluster) {  // sums of more than one cluster
+    r.part_floats = (long long)M * heads * (r.token_splits / kMaxCluster) * (c.head_dim + 2);
     r.counters = (long long)M * c.kv_heads;
   }
 }
@@ -456,7 +503,7 @@ CacheAttnPlan cache_attention_plan(const qi_kv_layer& c, int heads, int M, int w
 void cache_attention_fit(CacheAttnPlan& r, const qi_kv_layer& c, int heads, int M, long long part_floats,
                          long long counters) {
   while (r.part_floats > part_floats || r.counters > counters) {
-    if (r.token_splits > 1) --r.token_splits;
+    r.token_splits -= kMaxCluster;  // (with one cluster there is no scratch)
     sizes(r, c, heads, M);
   }
 }
@@ -475,6 +522,7 @@ cudaError_t launch_cache_attention(const CacheAttnParams& args, const CacheAttnP
     p.only_single = 1;
   }
   p.splits = plan.token_splits;
+  p.cluster = p.splits > kMaxCluster ? kMaxCluster : p.splits;
   return p.c.head_dim == 64 ? launch_dim<64>(p, s, pdl) : launch_dim<128>(p, s, pdl);
 }
 

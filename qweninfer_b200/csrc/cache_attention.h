@@ -21,9 +21,10 @@ struct CacheAttnParams {
   void* out;              // (M, heads, head_dim), may be null
   uint16_t* out_act;      // activation tiles of token tile out_nt for the o projection, may be null
   int out_nt;
-  float* part;            // partials of the splits, fp32
+  float* part;            // sums of the per-token kernel's clusters, fp32
   unsigned int* counters; // one per unit, zero between calls
   int splits;             // key splits of the kernel that runs
+  int cluster;            // per-token kernel: CTAs of a cluster, which divides splits
   int* err;
   // prompts (cache_attention_prompt.cu)
   int min_tiles;          // key tiles that a split has at least

@@ -81,6 +81,8 @@ def test_scratch_sizes(lib):
     assert (a.value, b.value) == (0, 0)  # short rows: one split
     assert lib.qi_cache_attention_scratch(C.byref(layer(max_len=100000)), 14, 1, 0, 0, 1, C.byref(a), C.byref(b)) == 0
     assert a.value % (14 * 66) == 0 and a.value >= 2 * 14 * 66 and b.value == 2
+    assert lib.qi_cache_attention_scratch(C.byref(layer(max_len=100000)), 14, 1, 64, 4, 1, C.byref(a), C.byref(b)) == 0
+    assert (a.value, b.value) == (0, 0)  # short windows too
     assert lib.qi_token_logprobs_scratch(1, 151936) > 0 and lib.qi_token_logprobs_scratch(4000, 151936) == 0
 
 
