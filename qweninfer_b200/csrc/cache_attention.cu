@@ -71,24 +71,23 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
   return r;
 }
-__device__ __forceinline__ float lds32(uint32_t addr) {
-  float r;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(addr) : "memory");
-  return r;
-}
+// d = a b + c of m16n8k16
 template <bool F16>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   if constexpr (F16)
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, "
+        "%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   else
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, "
+        "%12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
+
 // Granules a split has at least: one for each warp.
 constexpr int kMinSplit = kWarps;
 constexpr int kMaxCluster = 8;
@@ -138,33 +137,68 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
   const int gbeg = (int)((long long)seen.n * split_i / nsplit), gend = split_i < nsplit ? (int)((long long)seen.n * (split_i + 1) / nsplit) : gbeg;
 
   const uint32_t ring = smem_u32(smem) + (uint32_t)(warp * S::kStages * S::kStage);
+  // The row's keys and values of this head, in bytes, and its scales (of a packed layer; a
+  // paged one looks every granule's page up). Lanes 0..3 take the granule's scales, of K in
+  // its two halves and of V.
+  const bool paged = c.page_table != nullptr;
+  const uint8_t* krow = static_cast<const uint8_t*>(c.k);
+  const uint8_t* vrow = static_cast<const uint8_t*>(c.v);
+  const float* srow = lane < 2 ? c.k_scale : c.v_scale;
+  const int lg_block = F16 ? __ffs(c.block) - 1 : 0;
+  if (!paged) {
+    const long long rg = (long long)row * c.kv_heads + g;
+    krow += rg * c.max_len * S::kRow;
+    vrow += rg * c.max_len * S::kRow;
+    if constexpr (F16) srow += rg * ((c.max_len + c.block - 1) >> lg_block);
+  }
+  // Chunk x = lane + 32 j of a granule is chunk x % kChunks of key x / kChunks.
+  auto place = [&](int j) -> uint32_t {
+    constexpr int kStep = 32 / S::kChunks;  // keys of 32 chunks: the next j is 512 bytes on
+    const int r0 = lane / S::kChunks, ch = lane % S::kChunks;
+    if constexpr (S::kChunks == 4) return r0 * S::kRow + swizzle<4>(r0, ch) * 16 + j * 512;  // swizzled alike
+    else if constexpr (S::kChunks == 8) return ((r0 * S::kRow + swizzle<8>(r0, ch) * 16) ^ ((j & 1) * 32)) + j * 512;
+    else return (r0 + j * kStep) * S::kRow + swizzle<S::kChunks>(r0 + j * kStep, ch) * 16;
+  };
   // granule i (its place in the list) into ring stage st; nothing for i >= gend
   auto issue = [&](int i, int st) {
     if (i < gend) {
       const int k0 = seen.granule(i) * kGran;
-      long long o = layer_offset(c, D, row, g, k0);
-      if (o < 0) {  // an unmapped page: reported, read as zeros
-        if (lane == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
-      }
-      const bool mapped = o >= 0;
-      const uint8_t* kb = static_cast<const uint8_t*>(c.k) + (mapped ? o : 0) * (S::kRow / D);
-      const uint8_t* vb = static_cast<const uint8_t*>(c.v) + (mapped ? o : 0) * (S::kRow / D);
       const uint32_t dst = ring + (uint32_t)(st * S::kStage);
-#pragma unroll
-      for (int j = 0; j < S::kChunks; ++j) {
-        const int x = lane + 32 * j, r = x / S::kChunks, ch = x % S::kChunks;
-        const uint32_t n = mapped && seen.sees(k0 + r) ? 16u : 0u;
-        const uint32_t at = dst + (uint32_t)(r * S::kRow + swizzle<S::kChunks>(r, ch) * 16);
-        // a key that is not seen reads nothing; its address stays at the granule's first key
-        cp16(at, kb + (n ? x * 16 : 0), n);
-        cp16(at + S::kTensor, vb + (n ? x * 16 : 0), n);
+      long long ko = (long long)k0 * S::kRow, so = k0;  // of the first key: bytes, and position
+      bool mapped = true;
+      if (paged) {
+        const long long o = layer_offset(c, D, row, g, k0);
+        mapped = o >= 0;
+        ko = (mapped ? o : 0) * (S::kRow / D);
+        if constexpr (F16) so = mapped ? scale_index(c, row, g, k0) << lg_block | (k0 & (c.block - 1)) : 0;
+        // an unmapped page: reported, read as zeros
+        if (!mapped && lane == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
       }
-      if constexpr (F16) {
-        if (lane < 4) {  // scales of the granule's halves: K, K, V, V
-          const int h0 = k0 + 16 * (lane & 1);
-          const bool any = mapped && seen.sees16(h0);
-          const long long si = any ? scale_index(c, row, g, h0) : 0;
-          cp4(dst + 2 * S::kTensor + 4 * lane, (lane < 2 ? c.k_scale : c.v_scale) + si, any ? 4u : 0u);
+      const uint8_t* kp = krow + ko + lane * 16;
+      const uint8_t* vp = vrow + ko + lane * 16;
+      if (mapped && k0 + kGran - 1 <= seen.p && (k0 >= seen.lo || k0 + kGran <= seen.sinks)) {
+#pragma unroll
+        for (int j = 0; j < S::kChunks; ++j) {
+          cp16(dst + place(j), kp + j * 512);
+          cp16(dst + S::kTensor + place(j), vp + j * 512);
+        }
+        if constexpr (F16) {
+          if (lane < 4) cp4(dst + 2 * S::kTensor + 4 * lane, srow + ((so + 16 * (lane & 1)) >> lg_block), 4u);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < S::kChunks; ++j) {
+          // a key that is not seen reads nothing; its address stays in the granule's page
+          const uint32_t n = mapped && seen.sees(k0 + (lane + 32 * j) / S::kChunks) ? 16u : 0u;
+          cp16(dst + place(j), n ? kp + j * 512 : krow + ko, n);
+          cp16(dst + S::kTensor + place(j), n ? vp + j * 512 : vrow + ko, n);
+        }
+        if constexpr (F16) {
+          if (lane < 4) {
+            const int h0 = k0 + 16 * (lane & 1);
+            const bool any = mapped && seen.sees16(h0);
+            cp4(dst + 2 * S::kTensor + 4 * lane, srow + (any ? (so + 16 * (lane & 1)) >> lg_block : 0), any ? 4u : 0u);
+          }
         }
       }
     }
@@ -236,11 +270,12 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
     st = st + 1 == S::kStages ? 0 : st + 1;
     const int k0 = seen.granule(i) * kGran;
 
-    // scores of head gq for keys 8 t + 2 qd + e
-    float sc[4][2];
+    // scores of head gq for keys 8 t + 2 qd + e, without the factor f[t] > 0
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    float sc[4][2], f[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      float acc[4];
 #pragma unroll
       for (int h = 0; h < S::kChunks / 4; ++h) {
         const uint4 w = lds128(kt + (uint32_t)((8 * t + gq) * S::kRow + swizzle<S::kChunks>(8 * t + gq, 4 * h + qd) * 16));
@@ -250,24 +285,36 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
           uint32_t b0, b1;
           if constexpr (F16) widen<FMT, 0>(ws[j], b0, b1);
           else b0 = ws[2 * j], b1 = ws[2 * j + 1];
-          mma<F16>(acc, qa[0][kPer * h + j], b0, b1);
-          if constexpr (P3) mma<F16>(acc, qa[1][kPer * h + j], b0, b1);
+          if (h + j == 0) mma<F16>(acc, qa[0][0], b0, b1, zero);
+          else mma<F16>(acc, qa[0][kPer * h + j], b0, b1, acc);
+          if constexpr (P3) mma<F16>(acc, qa[1][kPer * h + j], b0, b1, acc);
         }
       }
-      float f = qscale;
-      if constexpr (F16) f *= lds32(kt + 2 * S::kTensor + 4 * (t >> 1));
-      sc[t][0] = (acc[0] + acc[2]) * f;
-      sc[t][1] = (acc[1] + acc[3]) * f;
+      sc[t][0] = acc[0] + acc[2];
+      sc[t][1] = acc[1] + acc[3];
+    }
+    float2 sv = make_float2(1.f, 1.f);  // V scales of the halves
+    if constexpr (F16) {
+      const uint4 w = lds128(kt + 2 * S::kTensor);
+      f[0] = f[1] = qscale * __uint_as_float(w.x);
+      f[2] = f[3] = qscale * __uint_as_float(w.y);
+      sv = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
+    } else {
+      f[0] = f[1] = f[2] = f[3] = qscale;
     }
     if (k0 + kGran - 1 > seen.p || (k0 < seen.lo && k0 + kGran > seen.sinks)) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (!seen.sees(k0 + 8 * t + 2 * qd + e)) sc[t][e] = -INFINITY;
+        for (int e = 0; e < 2; ++e) {
+          // (0 * f would be NaN for a scale that is not finite)
+          const bool in = seen.sees(k0 + 8 * t + 2 * qd + e);
+          sc[t][e] = in ? sc[t][e] * f[t] : -INFINITY;
+        }
+      f[0] = f[1] = f[2] = f[3] = 1.f;
     }
-    float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])),
-                     fmaxf(fmaxf(sc[2][0], sc[2][1]), fmaxf(sc[3][0], sc[3][1])));
+    float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])) * f[0],
+                     fmaxf(fmaxf(sc[2][0], sc[2][1]), fmaxf(sc[3][0], sc[3][1])) * f[2]);
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     if (__any_sync(0xffffffffu, mx > m)) {  // a new maximum: rescale what is summed so far
@@ -280,11 +327,11 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
     }
     // probabilities relative to the running maximum (8-bit: times 2^12, which keeps the
     // second fp16 part of small ones above the subnormal range)
-    const float mref = (m == -INFINITY ? 0.f : m) - (F16 ? 12.f : 0.f);
+    const float mref = (F16 ? 12.f : 0.f) - (m == -INFINITY ? 0.f : m);
     uint32_t pa[2][kA][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const float p0 = ex2(sc[t][0] - mref), p1 = ex2(sc[t][1] - mref);
+      const float p0 = ex2(fmaf(sc[t][0], f[t], mref)), p1 = ex2(fmaf(sc[t][1], f[t], mref));
       l += p0 + p1;
       uint32_t r[kParts];
       split<F16, kParts>(p0, p1, r);
@@ -292,41 +339,58 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
       pa[t >> 1][0][2 * (t & 1) + 1] = r[1];
       if constexpr (P3) pa[t >> 1][1][2 * (t & 1)] = r[2], pa[t >> 1][1][2 * (t & 1) + 1] = 0u;
     }
-    // O += P V, 16 keys at a time (one block scale each)
+    // O += P V: 16 keys have one V scale; where the two halves share it (blocks of 32 and
+    // more), or have none, both go into one sum before it is multiplied
+    const bool one = !F16 || sv.x == sv.y;
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      float sv = 1.f;
-      if constexpr (F16) sv = lds32(kt + 2 * S::kTensor + 8 + 4 * hf);
+    for (int h = 0; h < S::kChunks / 2; ++h) {
+      // matrices: keys 16 hf + 8 (j & 1) .., chunk 2 h + (j >> 1)
+      uint32_t b[2][4];
 #pragma unroll
-      for (int h = 0; h < S::kChunks / 2; ++h) {
-        // matrices: keys 16 hf + 8 (j & 1) .., chunk 2 h + (j >> 1)
+      for (int hf = 0; hf < 2; ++hf) {
         const int lj = lane >> 3, r = 16 * hf + 8 * (lj & 1) + (lane & 7), ch = 2 * h + (lj >> 1);
-        uint32_t b[4];
-        ldsm4t(vt + (uint32_t)(r * S::kRow + swizzle<S::kChunks>(r, ch) * 16), b);
+        ldsm4t(vt + (uint32_t)(r * S::kRow + swizzle<S::kChunks>(r, ch) * 16), b[hf]);
+      }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          if constexpr (F16) {
-            // chunk of 16 dims: this thread's columns are dims 4 qd + {0, 2} of the even and
-            // {1, 3} of the odd n-tile
-            uint32_t e0, e1, d0, d1;
-            widen<FMT, 1>(b[2 * u], e0, d0);
-            widen<FMT, 1>(b[2 * u + 1], e1, d1);
-            mma<F16>(acc, pa[hf][0], e0, e1);
-            float* oo = o + 4 * (2 * h + u);
-            oo[0] = fmaf(sv, acc[0] + acc[2], oo[0]);
-            oo[2] = fmaf(sv, acc[1] + acc[3], oo[2]);
-            float ac2[4] = {0.f, 0.f, 0.f, 0.f};
-            mma<F16>(ac2, pa[hf][0], d0, d1);
-            oo[1] = fmaf(sv, ac2[0] + ac2[2], oo[1]);
-            oo[3] = fmaf(sv, ac2[1] + ac2[3], oo[3]);
-          } else {
-            mma<F16>(acc, pa[hf][0], b[2 * u], b[2 * u + 1]);
-            if constexpr (P3) mma<F16>(acc, pa[hf][1], b[2 * u], b[2 * u + 1]);
-            float* oo = o + 2 * (2 * h + u);
-            oo[0] += acc[0] + acc[2];
-            oo[1] += acc[1] + acc[3];
+      for (int u = 0; u < 2; ++u) {
+        if constexpr (F16) {
+          // chunk of 16 dims: this thread's columns are dims 4 qd + {0, 2} of the even and
+          // {1, 3} of the odd n-tile
+          float* oo = o + 4 * (2 * h + u);
+          uint32_t e[2][2], d[2][2];
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            widen<FMT, 1>(b[hf][2 * u], e[hf][0], d[hf][0]);
+            widen<FMT, 1>(b[hf][2 * u + 1], e[hf][1], d[hf][1]);
           }
+          float ae[4], ad[4];
+          mma<F16>(ae, pa[0][0], e[0][0], e[0][1], zero);
+          mma<F16>(ad, pa[0][0], d[0][0], d[0][1], zero);
+          if (one) {
+            mma<F16>(ae, pa[1][0], e[1][0], e[1][1], ae);
+            mma<F16>(ad, pa[1][0], d[1][0], d[1][1], ad);
+          } else {
+            float be[4], bd[4];
+            mma<F16>(be, pa[1][0], e[1][0], e[1][1], zero);
+            mma<F16>(bd, pa[1][0], d[1][0], d[1][1], zero);
+            oo[0] = fmaf(sv.y, be[0] + be[2], oo[0]);
+            oo[1] = fmaf(sv.y, bd[0] + bd[2], oo[1]);
+            oo[2] = fmaf(sv.y, be[1] + be[3], oo[2]);
+            oo[3] = fmaf(sv.y, bd[1] + bd[3], oo[3]);
+          }
+          oo[0] = fmaf(sv.x, ae[0] + ae[2], oo[0]);
+          oo[1] = fmaf(sv.x, ad[0] + ad[2], oo[1]);
+          oo[2] = fmaf(sv.x, ae[1] + ae[3], oo[2]);
+          oo[3] = fmaf(sv.x, ad[1] + ad[3], oo[3]);
+        } else {
+          float acc[4];
+          mma<F16>(acc, pa[0][0], b[0][2 * u], b[0][2 * u + 1], zero);
+          if constexpr (P3) mma<F16>(acc, pa[0][1], b[0][2 * u], b[0][2 * u + 1], acc);
+          mma<F16>(acc, pa[1][0], b[1][2 * u], b[1][2 * u + 1], acc);
+          if constexpr (P3) mma<F16>(acc, pa[1][1], b[1][2 * u], b[1][2 * u + 1], acc);
+          float* oo = o + 2 * (2 * h + u);
+          oo[0] += acc[0] + acc[2];
+          oo[1] += acc[1] + acc[3];
         }
       }
     }
