@@ -391,7 +391,7 @@ int grid_for(int n_tiles, int KB, int max_contrib) {
 
 bool bad_attention(const qi_kv_layer* c, int heads, int M, int window, int sinks, int query_run) {
   return bad_layer(c) || heads <= 0 || heads % c->kv_heads != 0 || heads / c->kv_heads > 8 || M <= 0 || window < 0 ||
-         sinks < 0 || query_run < 0 || c->kv_heads > 65535 || (long long)M * kMaxAttnSplits > 0x7fffffffLL;
+         sinks < 0 || query_run < 0 || c->kv_heads > 65535 || (long long)M * 256 > 0x7fffffffLL;
 }
 
 // qi_forward on the tensor-core path: every projection is a tc_proj launch whose

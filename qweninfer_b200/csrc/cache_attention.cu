@@ -48,8 +48,11 @@ struct Shape {
   static constexpr int kChunks = kRow / 16;
   static constexpr int kTensor = kGran * kRow;                   // K or V of a granule
   static constexpr int kStage = 2 * kTensor + 16;                // + 2 K scales, 2 V scales
-  static constexpr int kStages = kStage > 9000 ? 2 : 3;
+  static constexpr int kStages = 2;
   static constexpr size_t kRing = (size_t)kWarps * kStages * kStage;
+  // CTAs of an SM: by registers for 8-bit codes, by shared memory otherwise
+  static constexpr int kCtas = FMT == QI_KV_BF16 ? (D == 64 ? 3 : 1) : (D == 64 ? 5 : 3);
+  static_assert((kRing + 6 * 1024) * kCtas <= 228 * 1024, "shared memory of an SM");
 };
 
 // physical 16-byte chunk c of key r: 8 keys at one chunk (ldmatrix) and 2 keys at 4
@@ -92,16 +95,21 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
 constexpr int kMinSplit = kWarps;
 constexpr int kMaxCluster = 8;
 
-// shared memory of CTA w of the cluster
-__device__ __forceinline__ float peer(const float* x, int w) {
-  float r;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r) : "r"(map_rank(x, (uint32_t)w)) : "memory");
-  return r;
+// What the CTAs of a cluster push to each other, apart from the rings that are still in use:
+// maximum and sum of the heads, and a share of the outputs as pairs of dims.
+template <int D>
+struct Inbox {
+  float2 ml[kMaxCluster][kMaxGroup];
+  float2 pairs[kMaxGroup * D / 2 + kMaxCluster];  // [split][the share]
+};
+// into the shared memory of CTA w of the cluster
+__device__ __forceinline__ void put2(float2* to, int w, float a, float b) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(map_rank(to, (uint32_t)w)), "f"(a), "f"(b) : "memory");
 }
 
 // F16 products for 8-bit codes, bf16 for a bf16 cache; P3: three parts of q and p (bf16).
 template <int FMT, int D, bool P3>
-__global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(kThreads, Shape<FMT, D>::kCtas) cache_attention_kernel(const CacheAttnParams p) {
   using S = Shape<FMT, D>;
   constexpr bool F16 = FMT != QI_KV_BF16;
   constexpr int kParts = P3 ? 3 : 2, kA = P3 ? 2 : 1;  // parts, A operands
@@ -110,29 +118,52 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
   constexpr int kOut = D / 4;                          // output dims of a thread
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int last;
+  __shared__ Inbox<D> in;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, qd = lane & 3;
   const int tok = blockIdx.x / p.splits, split_i = blockIdx.x - tok * p.splits, g = blockIdx.y;
   const qi_kv_layer& c = p.c;
   const int G = p.group, width = p.heads * D;
   grid_dep_wait();
   grid_dep_launch();
+  if (p.cluster > 1) cluster_arrive();  // this CTA's shared memory may be written by the others
   const int ps = p.pos[tok], row = p.rows[tok];
+  // the query of head gq: dims 16 bytes apart per quad, in the keys' chunk order (loaded
+  // before the keys, whose addresses wait for the position)
+  float x[D / 4];
+  {
+    const long long qo = (long long)tok * p.q_st + (long long)(g * G + (gq < G ? gq : 0)) * p.q_sh;
+#pragma unroll
+    for (int i = 0; i < D / 4; i += 4) {
+      // i-th value of this thread: k-step i / 4 lies in chunk 4 * (i / 4 / kPer) + qd
+      const int d = (4 * (i / 4 / kPer) + qd) * 4 * kPer + (i / 4 % kPer) * 4;
+      if (p.dtype == QI_F32) load4<QI_F32>(p.q, qo + d, p.q_vec, *reinterpret_cast<float(*)[4]>(x + i));
+      else if (p.dtype == QI_BF16) load4<QI_BF16>(p.q, qo + d, p.q_vec, *reinterpret_cast<float(*)[4]>(x + i));
+      else load4<QI_F16>(p.q, qo + d, p.q_vec, *reinterpret_cast<float(*)[4]>(x + i));
+    }
+    if (gq >= G) {
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+    }
+  }
+  auto leave = [&] {  // nothing to do: the cluster's first barrier is still to be met
+    if (p.cluster > 1) cluster_wait();
+  };
   if (!token_ok(p, ps, row)) {  // nothing seen: zeros; a position or row outside the cache is reported
     if (split_i == 0 && !p.only_single) {
       if (ps != -1 && tid == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
       const float z[2] = {0.f, 0.f};
       for (int e = tid; e < G * D / 2; e += kThreads) emit<2>(p, tok, g * G * D + 2 * e, width, z);
     }
-    return;
+    return leave();
   }
   if (p.only_single) {  // the tokens that the prompt kernel left out
     const int n = kPromptRows / G, t = tok / n * n + tid;
     const bool same = tid < n && t < p.M && p.rows[t] == row && token_ok(p, p.pos[t], row);
-    if (__syncthreads_count(same) != 1) return;
+    if (__syncthreads_count(same) != 1) return leave();
   }
   const Seen<kGran> seen = seen_range<kGran>(ps, window_start(ps, p.window), p.sinks);
   const int nsplit = min(p.splits, (seen.n + kMinSplit - 1) / kMinSplit);
-  if (nsplit == 1 ? split_i > 0 : split_i / p.cluster * p.cluster >= nsplit) return;  // clusters without keys
+  if (nsplit == 1 ? split_i > 0 : split_i / p.cluster * p.cluster >= nsplit) return leave();  // without keys
   // (a split without keys in a cluster that has some gets an empty run)
   const int gbeg = (int)((long long)seen.n * split_i / nsplit), gend = split_i < nsplit ? (int)((long long)seen.n * (split_i + 1) / nsplit) : gbeg;
 
@@ -207,31 +238,9 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
 #pragma unroll
   for (int s = 0; s < S::kStages - 1; ++s) issue(gbeg + warp + s * kWarps, s);
 
-  // the query fragments: dims 16 bytes apart per quad, in the keys' chunk order
   uint32_t qa[kA][kSteps][4];
   float qscale = p.scale_log2;
   {
-    float x[D / 4];
-    const long long qo = (long long)tok * p.q_st + (long long)(g * G + (gq < G ? gq : 0)) * p.q_sh;
-#pragma unroll
-    for (int i = 0; i < D / 4; i += 4) {
-      // i-th value of this thread: k-step i / 4 lies in chunk 4 * (i / 4 / kPer) + qd
-      const int d = (4 * (i / 4 / kPer) + qd) * 4 * kPer + (i / 4 % kPer) * 4;
-      if (p.q_vec && p.dtype == QI_F32) {
-        const float4 f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + qo + d));
-        x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[i + e] = p.dtype == QI_F32    ? load_elem<QI_F32>(p.q, qo + d + e)
-                     : p.dtype == QI_BF16 ? load_elem<QI_BF16>(p.q, qo + d + e)
-                                          : load_elem<QI_F16>(p.q, qo + d + e);
-      }
-    }
-    if (gq >= G) {
-#pragma unroll
-      for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
-    }
     if constexpr (F16) {
       // q * 2^-e in [1, 2) at its largest: fp16 parts keep 22 bits of every head's scale
       float am = 0.f;
@@ -413,16 +422,18 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
     if (qd == 0) w[D] = m, w[D + 1] = l;
   }
   __syncthreads();
-  // The splits of a unit are clusters of p.cluster CTAs: they exchange their sums through
-  // distributed shared memory, each CTA adding up a share of the outputs in split order. Over
-  // more than one cluster, the clusters' sums go through global memory to the last to arrive.
+  // The splits of a unit are clusters of p.cluster CTAs. Every CTA adds up a share of the
+  // outputs: the others push theirs into its shared memory, and it sums them in split order.
+  // Over more than one cluster the clusters' sums go through global memory to the CTA that
+  // arrives last.
   const long long unit = (long long)tok * c.kv_heads + g;
   const int C = p.cluster, rank = split_i % C, first = split_i - rank;
-  const int here = min(C, nsplit - first);                // splits of this cluster with keys
+  const int here = min(C, nsplit - first);  // splits of this cluster with keys
   const int clusters = (nsplit + C - 1) / C;
-  float* sums = wp + kWarps * G * kPart;                  // this split's: [head][D values, m, l]
   constexpr int kPairs = D / 2;
-  for (int e = tid; e < G * kPairs; e += kThreads) {
+  const int E = G * kPairs, per = (E + C - 1) / C;  // pairs of outputs, and a CTA's share of them
+  if (nsplit > 1) cluster_wait();                   // every CTA of the cluster has started
+  for (int e = tid; e < E; e += kThreads) {
     const int h = e / kPairs, d = 2 * (e - h * kPairs);
     float mm, ll, a, b;
     merge2<D>([&](int w, int i) { return wp[(w * G + h) * kPart + i]; }, kWarps, d, mm, ll, a, b);
@@ -430,39 +441,40 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const CacheAt
       const float inv = ll != 0.f ? 1.f / ll : 0.f;
       const float v[2] = {a * inv, b * inv};
       emit<2>(p, tok, g * G * D + h * D + d, width, v);
-    } else {
-      sums[h * kPart + d] = a, sums[h * kPart + d + 1] = b;
-      if (d == 0) sums[h * kPart + D] = mm, sums[h * kPart + D + 1] = ll;
+    } else if (rank < here) {
+      const int to = e / per;
+      put2(&in.pairs[rank * per + e - to * per], to, a, b);
+      // maximum and sum of the head, for the first pair of it in each share
+      if (d == 0 || e % per == 0) put2(&in.ml[rank][h], to, mm, ll);
     }
   }
-  if (nsplit == 1) return;
+  if (nsplit == 1) return leave();
   __syncwarp();
   cluster_arrive();
   cluster_wait();
   float* part = p.part + unit * (p.splits / C) * (long long)(G * kPart);  // [cluster][head][D + 2]
-  const int e0 = G * kPairs * rank / C, e1 = G * kPairs * (rank + 1) / C;
-  for (int e = e0 + tid; e < e1; e += kThreads) {
+  for (int e = rank * per + tid; e < min(E, (rank + 1) * per); e += kThreads) {
     const int h = e / kPairs, d = 2 * (e - h * kPairs);
     float mm, ll, a, b;
-    merge2<D>([&](int w, int i) { return peer(sums + h * kPart + i, w); }, here, d, mm, ll, a, b);
+    merge2<0>([&](int w, int i) { return i < 2 ? (i ? in.ml[w][h].y : in.ml[w][h].x)
+                                               : (i == 2 ? in.pairs[(w - rank) * per + e].x : in.pairs[(w - rank) * per + e].y); },
+              here, 2, mm, ll, a, b);
     if (clusters == 1) {
       const float inv = ll != 0.f ? 1.f / ll : 0.f;
       const float v[2] = {a * inv, b * inv};
       emit<2>(p, tok, g * G * D + h * D + d, width, v);
     } else {
-      float* x = part + (long long)(first / C) * (G * kPart) + h * kPart;
-      __stcg(reinterpret_cast<float2*>(x + d), make_float2(a, b));
-      if (d == 0) __stcg(reinterpret_cast<float2*>(x + D), make_float2(mm, ll));
+      float* y = part + (long long)(first / C) * (G * kPart) + h * kPart;
+      __stcg(reinterpret_cast<float2*>(y + d), make_float2(a, b));
+      if (d == 0) __stcg(reinterpret_cast<float2*>(y + D), make_float2(mm, ll));
     }
   }
-  __syncwarp();
-  cluster_arrive();  // sums read, and the cluster's share of part written
-  cluster_wait();
-  if (clusters == 1 || rank != 0) return;
-  if (tid == 0) last = atomic_add_acq_rel(p.counters + unit, 1u) == (unsigned)(clusters - 1);
+  if (clusters == 1) return;
+  __syncthreads();
+  if (tid == 0) last = atomic_add_acq_rel(p.counters + unit, 1u) == (unsigned)(C * clusters - 1);
   __syncthreads();
   if (!last) return;
-  for (int e = tid; e < G * kPairs; e += kThreads) {
+  for (int e = tid; e < E; e += kThreads) {
     const int h = e / kPairs, d = 2 * (e - h * kPairs);
     float mm, ll, a, b;
     merge2<D>([&](int w, int i) { return __ldcg(part + ((long long)w * G + h) * kPart + i); }, clusters, d, mm, ll, a, b);
@@ -520,15 +532,20 @@ long long seen_at_most(const qi_kv_layer& c, int window, int sinks) {
   return window > 0 && w < c.max_len ? w : c.max_len;
 }
 
-// Key splits of the per-token kernel: four CTAs for every SM (what its shared memory
-// admits), as far as rows are long enough to give each split kMinSplit granules; whole
-// clusters when there are more than fit one.
+constexpr int kMaxTokenSplits = 256;
+
+// Key splits of the per-token kernel: as many CTAs as are resident at once, as far as rows
+// are long enough to give each split kMinSplit granules; whole clusters when there are more
+// than fit one.
 int token_splits(const qi_kv_layer& c, int M, int window, int sinks) {
+  const int ctas = c.format == QI_KV_BF16 ? (c.head_dim == 64 ? Shape<QI_KV_BF16, 64>::kCtas : Shape<QI_KV_BF16, 128>::kCtas)
+                                          : (c.head_dim == 64 ? Shape<QI_KV_INT8, 64>::kCtas : Shape<QI_KV_INT8, 128>::kCtas);
   const long long gran = seen_at_most(c, window, sinks) / kGran + 2, units = (long long)M * c.kv_heads;
   const long long most = (gran + kMinSplit - 1) / kMinSplit;
-  long long want = 4LL * sm_count() / units;
+  // (nine tenths of them: clusters do not fill every GPC)
+  long long want = (long long)ctas * sm_count() * 9 / 10 / units;
   want = want > most ? most : want;
-  want = want > kMaxAttnSplits ? kMaxAttnSplits : want < 1 ? 1 : want;
+  want = want > kMaxTokenSplits ? kMaxTokenSplits : want < 1 ? 1 : want;
   return (int)(want > kMaxCluster ? want / kMaxCluster * kMaxCluster : want);
 }
 

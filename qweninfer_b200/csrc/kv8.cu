@@ -28,29 +28,6 @@ struct Kv8AppendParams {
   int* err;
 };
 
-// 4 consecutive elements; `vec`: the address is aligned for one load
-template <int DT>
-__device__ __forceinline__ void load4(const void* p, long long i, bool vec, float (&x)[4]) {
-  if (vec) {
-    if constexpr (DT == QI_F32) {
-      const float4 f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
-      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-    } else {
-      const uint2 u = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i));
-      if constexpr (DT == QI_BF16) {
-        x[0] = bf16lo(u.x), x[1] = bf16hi(u.x), x[2] = bf16lo(u.y), x[3] = bf16hi(u.y);
-      } else {
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = load_elem<DT>(p, i + e);
-  }
-}
-
 // CTA (token t, head g). The tokens of one call may come in any order, so one of a block's
 // tokens takes all of them: the one with the lowest position. A token right behind its
 // predecessor in the same block ends at once; the others (run starts: one for each block
