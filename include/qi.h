@@ -249,14 +249,16 @@ int qi_cache_attention_scratch(const qi_kv_layer* layer, int heads, int M, int w
  * targets: int32 (targets_64 = 0) or int64, or NULL; a negative target gives 0, one >= V
  * NaN. logprob, entropy may be NULL. A logit of -inf has probability 0; a row with a NaN or
  * +inf logit, or of -inf alone, has NaN results (NaN logits are no alternatives: missing
- * ones have id -1). scratch: scratch_bytes bytes, 16-byte aligned, and counters (M uint32,
- * zero before the first call and left zero); qi_token_logprobs_scratch gives the bytes that
- * use the whole GPU for few rows, with less a row is cut into fewer slices. No reference
- * counterpart: the reference takes the argmax (qweninfer/engine/engine.py:129,155). */
+ * ones have id -1). scratch: scratch_bytes bytes, 16-byte aligned, and counters
+ * (QI_LOGPROBS_COUNTERS uint32, zero before the first call and left zero);
+ * qi_token_logprobs_scratch gives the bytes that use the whole GPU (a few hundred KB at
+ * most), with less (or NULL) no row is shared by CTAs. No reference counterpart: the
+ * reference takes the argmax (qweninfer/engine/engine.py:129,155). */
+#define QI_LOGPROBS_COUNTERS 1024
 int qi_token_logprobs(const void* logits, int dtype, long long ld, const void* targets, int targets_64, int M, int V,
                       int top, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, void* scratch,
                       long long scratch_bytes, unsigned int* counters, qi_stream_t stream);
-long long qi_token_logprobs_scratch(int M, int V);
+long long qi_token_logprobs_scratch(int M, int V, int dtype);
 
 /* ------------------------------------------------------------- whole forward */
 

@@ -22,6 +22,7 @@ QI_ERR_DEVICE = 1003
 QI_ERR_TOO_LARGE = 1004
 QI_ERR_INDEX = 1005
 QI_KV_BF16, QI_KV_INT8, QI_KV_E4M3 = 0, 1, 2
+LOGPROBS_COUNTERS = 1024
 # element types of activations (QI_F32, QI_BF16, QI_F16)
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # launch kinds of qi_forward_launch_times
@@ -90,7 +91,7 @@ SIGNATURES = {
     "qi_cache_attention_scratch": (i32, [C.POINTER(QiKvLayer), i32, i32, i32, i32, i32, C.POINTER(i64),
                                          C.POINTER(i64)]),
     "qi_token_logprobs": (i32, [vp, i32, i64, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, i64, vp, vp]),
-    "qi_token_logprobs_scratch": (i64, [i32, i32]),
+    "qi_token_logprobs_scratch": (i64, [i32, i32, i32]),
     "qi_act_tiles": (i32, [vp, vp, i32, i32, i32, vp, vp, i32, vp]),
     "qi_tc_linear": (i32, [vp, i32, i32, vp, i32, i32, vp, i32, f32, vp, i32, vp, i64, vp, i32, i32, vp, vp]),
     "qi_tc_gate_up_swiglu": (i32, [vp, vp, i32, i32, vp, i32, f32, vp, vp, i64, vp, i32, i32, vp, vp]),

@@ -760,19 +760,21 @@ int qi_cache_attention(const qi_kv_layer* layer, const void* q, long long q_toke
   return rc(launch_cache_attention(p, plan, as_stream(stream), false));
 }
 
-long long qi_token_logprobs_scratch(int M, int V) {
-  if (M <= 0 || V <= 0) return 0;
-  const int n = logprob_slices(M, V);
-  return n > 1 ? (long long)M * n * (16 + 32 * 8) : 0;
+long long qi_token_logprobs_scratch(int M, int V, int dtype) {
+  if (M <= 0 || V <= 0 || bad_dtype(dtype)) return 0;
+  return logprob_plan(M, V, dtype).scratch;
 }
 
 int qi_token_logprobs(const void* logits, int dtype, long long ld, const void* targets, int targets_64, int M, int V,
                       int top, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, void* scratch,
                       long long scratch_bytes, unsigned int* counters, qi_stream_t stream) {
   if (bad_ptr(logits) || bad_dtype(dtype) || M <= 0 || V <= 0 || ld < V || top < 0 || top > 32 || top > V ||
-      (top > 0 && (bad_ptr(top_ids) || bad_ptr(top_logprobs))) || (long long)M * kMaxLogprobSlices > 0x7fffffffLL ||
-      ((uintptr_t)scratch & 15))
+      (top > 0 && (bad_ptr(top_ids) || bad_ptr(top_logprobs))) || ((uintptr_t)scratch & 15))
     return QI_ERR_ARG;
+  LogprobPlan plan = logprob_plan(M, V, dtype);
+  if ((long long)M * plan.chunks > 0x7fffffffLL) return QI_ERR_ARG;
+  // without scratch for shared rows every CTA takes whole ones
+  if (!scratch || !counters || scratch_bytes < plan.scratch || plan.ctas > QI_LOGPROBS_COUNTERS) plan.ctas = M;
   LogprobParams p = {};
   p.logits = logits;
   p.ld = ld;
@@ -785,12 +787,10 @@ int qi_token_logprobs(const void* logits, int dtype, long long ld, const void* t
   p.entropy = entropy;
   p.top_ids = top_ids;
   p.top_logprobs = top_logprobs;
-  p.slices = scratch && counters ? logprob_slices(M, V) : 1;
-  while (p.slices > 1 && (long long)M * p.slices * (16 + 32 * 8) > scratch_bytes) --p.slices;
   p.part_stats = static_cast<float*>(scratch);
-  p.part_list = reinterpret_cast<unsigned long long*>(static_cast<char*>(scratch) + (size_t)M * p.slices * 16);
+  p.part_list = reinterpret_cast<unsigned long long*>(static_cast<char*>(scratch) + (size_t)plan.ctas * 2 * 16);
   p.counters = counters;
-  return rc(launch_token_logprobs(p, dtype, as_stream(stream), false));
+  return rc(launch_token_logprobs(p, plan, dtype, as_stream(stream)));
 }
 
 int qi_act_tiles(const float* x, const float* norm_w, int M, int K, int NT, uint16_t* act, float* ss, int ss_ld,

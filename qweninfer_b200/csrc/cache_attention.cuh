@@ -25,11 +25,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 
 // ---- parts of fp32 pairs as 16-bit pairs (a in the low half)
 __device__ __forceinline__ uint32_t f16x2(float a, float b) {

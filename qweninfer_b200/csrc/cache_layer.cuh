@@ -1,6 +1,7 @@
 // One layer of a KV cache as the cached-attention and 8-bit kernels address it: bf16 values,
 // or 8-bit codes with a power-of-two scale per block of positions and KV head; packed rows
-// or pages.
+// or pages. Also the element types and fp32 helpers that these kernels and the log
+// probabilities share.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -94,6 +95,40 @@ template <int FMT>
 __device__ __forceinline__ float decode(uint8_t c) {
   if constexpr (FMT == QI_KV_INT8) return (float)(int8_t)c;
   else return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+}
+
+// ---- pairs of fp32 values in 64 bits: one instruction for two operations
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(f2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // Host-side checks of a layer descriptor shared by the entry points.

@@ -6,8 +6,6 @@
 
 namespace qi {
 
-constexpr int kMaxLogprobSlices = 64;
-
 struct LogprobParams {
   const void* logits;
   long long ld;
@@ -18,13 +16,18 @@ struct LogprobParams {
   float* entropy;
   int32_t* top_ids;
   float* top_logprobs;
-  float* part_stats;              // M * slices * 4
-  unsigned long long* part_list;  // M * slices * 32
-  unsigned int* counters;         // M, zero between calls
-  int slices;
+  // of rows that several CTAs share, two parts for each CTA: sums (4 floats) and lists (32 words)
+  float* part_stats;
+  unsigned long long* part_list;
+  unsigned int* counters;  // one for each CTA, zero between calls
+  int chunks;              // of a row (set by the launch)
 };
 
-int logprob_slices(int M, int V);
-cudaError_t launch_token_logprobs(const LogprobParams& p, int dtype, cudaStream_t s, bool pdl);
+struct LogprobPlan {
+  int ctas, chunks;
+  long long scratch;  // bytes
+};
+LogprobPlan logprob_plan(int M, int V, int dtype);
+cudaError_t launch_token_logprobs(const LogprobParams& p, const LogprobPlan& plan, int dtype, cudaStream_t s);
 
 }  // namespace qi

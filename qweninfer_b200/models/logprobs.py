@@ -71,8 +71,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     with _lib.on_device(dev):
         L = _lib.lib()
         stream = _lib.stream_ptr(dev)
-        nbytes = L.qi_token_logprobs_scratch(M, V)
-        data, counters, _keep = _lib.scratch(dev, stream, nbytes, M) if nbytes else (0, 0, None)
+        nbytes = L.qi_token_logprobs_scratch(M, V, _lib.DTYPES[logits.dtype])
+        data, counters, _keep = _lib.scratch(dev, stream, nbytes, _lib.LOGPROBS_COUNTERS)
         _lib.check(L.qi_token_logprobs(
             logits.data_ptr(), _lib.DTYPES[logits.dtype], logits.stride(0) if M > 1 else V, _lib.ptr(targets),
             int(targets is not None and targets.dtype == torch.int64), M, V, top, _lib.ptr(r.logprob),
