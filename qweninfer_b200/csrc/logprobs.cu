@@ -1,18 +1,21 @@
 // Log probabilities of given tokens, the entropy and the top alternatives of each row of
 // logits, in one pass over the logits.
 //
-//   m = max x,  Z = sum e^(x - m),  A = sum e^(x - m) (x - m):
-//   log p(target) = x_target - m - log Z,  entropy = log Z - A / Z.
+// with m = max x and y = (x - m) log2(e):
+//   Z = sum 2^y,  A = sum 2^y y,  log p(target) = x_target - m - log Z,
+//   entropy = log 2 (log2 Z - A / Z).
 //
 // Every lane keeps (m, Z, A) of its own elements and rescales them when its maximum grows:
-// with f = e^(m - m'), Z' = f Z and A' = f (A + Z (m - m')). A logit of -inf has weight 0.
-// The top alternatives: each warp keeps its best 32 as (order of the value, inverted index)
-// words, lane i the i-th best, so that equal values go to the lower index. An element that
-// reaches the top-th best so far goes into a buffer; 32 of them are sorted and merged into
-// the list at once (15 and 6 exchange steps). The first threshold comes from the lanes' own
-// maxima, so that few elements do.
-//
-// A call reads its logits once and is bound by those bytes. They are cut into chunks of 16 KB
+// with d = (m - m') log2(e) and f = 2^d, Z' = f Z and A' = f (A + Z d). A logit of -inf has
+// weight 0.
+// The top alternatives are words (order of the value, inverted index), so that equal values
+// go to the lower index. While a row streams by, a lane only keeps its largest logit, and
+// which of its steps reached the top-th largest of the lanes' first ones. Of the lanes'
+// largest, the top-th is then a bound that hardly more than top elements reach: the steps of
+// the lanes that reach it are read again, their elements above it sorted. (More than 64, as
+// in a row of equal values: every warp keeps a list of its best 32 instead, 32 candidates
+// sorted and merged into it at a time.)
+// A call reads its logits once and is bound by those bytes. They are cut into chunks of 32 KB
 // and the chunks of all rows are shared out evenly, in order, over the CTAs that are
 // resident at once, so that all SMs load until the end whatever the number of rows. A
 // producer thread keeps a ring of chunks under way with bulk copies, over row ends too: the
@@ -27,12 +30,13 @@ namespace {
 
 constexpr int kWarps = 8;                     // that compute; one more copies
 constexpr int kThreads = 32 * (kWarps + 1);
-constexpr int kStages = 4;
-constexpr int kChunk = 16384;                 // bytes; a warp's share is 4 vectors of every lane
+constexpr int kStages = 2;
+constexpr int kChunk = 32768;                 // bytes; a warp's share is 8 vectors of every lane
 constexpr int kCtas = 3;                      // of an SM
 constexpr int kList = 32;
 constexpr float kLog2e = 1.4426950408889634f;
-// e^kFar is 0 in fp32, and a sum of weights times kFar is finite: distances of masked logits
+constexpr float kLn2 = 0.6931471805599453f;
+// 2^kFar is 0 in fp32, and a sum of weights times kFar is finite: distances of masked logits
 // (-inf, or a type's lowest value) stop there
 constexpr float kFar = -1e4f;
 constexpr unsigned kAll = 0xffffffffu;
@@ -44,14 +48,26 @@ __device__ __forceinline__ float key_value(u64 key) {
   return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 struct Stats {
   float m, z, a;
 };
 __device__ __forceinline__ void merge(Stats& s, const Stats& t) {
   const float m = fmaxf(s.m, t.m);
   // an empty side (maximum -inf, sum 0) adds nothing; a NaN sum stays one
-  const float ds = s.m == -INFINITY ? 0.f : fmaxf(s.m - m, kFar), dt = t.m == -INFINITY ? 0.f : fmaxf(t.m - m, kFar);
-  const float fs = ex2(ds * kLog2e), ft = ex2(dt * kLog2e);
+  const float ds = s.m == -INFINITY ? 0.f : fmaxf((s.m - m) * kLog2e, kFar);
+  const float dt = t.m == -INFINITY ? 0.f : fmaxf((t.m - m) * kLog2e, kFar);
+  const float fs = ex2(ds), ft = ex2(dt);
   const float a = fs * fmaf(s.z, ds, s.a) + ft * fmaf(t.z, dt, t.a);
   s.z = fs * s.z + ft * t.z;
   s.a = a;
@@ -59,7 +75,7 @@ __device__ __forceinline__ void merge(Stats& s, const Stats& t) {
 }
 __device__ __forceinline__ Stats warp_stats(Stats s) {
   const float m = warp_max(s.m);
-  const float d = s.m == -INFINITY ? 0.f : fmaxf(s.m - m, kFar), f = ex2(d * kLog2e);
+  const float d = s.m == -INFINITY ? 0.f : fmaxf((s.m - m) * kLog2e, kFar), f = ex2(d);
   const float a = f * fmaf(s.z, d, s.a);
   return Stats{m, warp_sum(f * s.z), warp_sum(a)};
 }
@@ -88,8 +104,8 @@ __device__ __forceinline__ u64 sort_lanes(u64 v, int lane) {
     }
   return v;
 }
-// the k-th largest of the lanes' values (1 <= k <= 32)
-__device__ __forceinline__ float kth_of_lanes(float v, int k, int lane) {
+// the lanes' values in descending order
+__device__ __forceinline__ float sort_lanes(float v, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -98,7 +114,17 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k, int lane) {
       const bool down = (lane & size) == 0 || size == 32;
       v = ((lane & o) == 0) == down ? fmaxf(v, x) : fminf(v, x);
     }
-  return __shfl_sync(kAll, v, k - 1);
+  return v;
+}
+// the 32 largest of two descending sequences, descending
+__device__ __forceinline__ float merge_lists(float list, float other, int lane) {
+  list = fmaxf(list, __shfl_sync(kAll, other, 31 - lane));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float x = __shfl_xor_sync(kAll, list, o);
+    list = (lane & o) == 0 ? fmaxf(list, x) : fminf(list, x);
+  }
+  return list;
 }
 
 template <int DT>
@@ -123,7 +149,7 @@ __device__ __forceinline__ void unpack(const uint4& u, float* x) {
   }
 }
 
-// A warp's candidates for the top alternatives: its best 32 so far, and words that may enter.
+// A warp's list of its best 32 so far, and words that may enter.
 struct Best {
   u64 list;    // lane i: the i-th best
   float thr;   // nothing below it can enter
@@ -153,6 +179,21 @@ struct Best {
 __device__ __forceinline__ int share(int c, long long T, int G) { return (int)(c * T / G); }
 __device__ __forceinline__ int owner(long long u, long long T, int G) { return (int)(((u + 1) * G - 1) / T); }
 
+// element i of a vector array in shared memory
+template <int DT>
+__device__ __forceinline__ float elem(const uint4* v, int i) {
+  if constexpr (DT == QI_F32) return reinterpret_cast<const float*>(v)[i];
+  else if constexpr (DT == QI_BF16) return bf16_to_f32(reinterpret_cast<const uint16_t*>(v)[i]);
+  else return __half2float(reinterpret_cast<const __half*>(v)[i]);
+}
+
+struct Yes {
+  static constexpr bool value = true;
+};
+struct No {
+  static constexpr bool value = false;
+};
+
 struct Ring {
   uint64_t full[kStages], empty[kStages];
 };
@@ -160,14 +201,16 @@ struct Ring {
 template <int DT, bool TOP>
 __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const LogprobParams p) {
   constexpr int VN = Vec<DT>::N, ES = DT == QI_F32 ? 4 : 2;
-  constexpr int U = DT == QI_F32 ? 4 : 2, N = U * VN;  // vectors and elements of a lane's step
+  constexpr int U = DT == QI_F32 ? 8 : 4, N = U * VN;  // vectors and elements of a lane's step
   constexpr int kVecs = kChunk / 16, kSteps = kVecs / (32 * kWarps * U);
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Ring ring;
   __shared__ Stats wstats[kWarps];
   __shared__ u64 wlist[kWarps][kList];
+  __shared__ float wmax[kWarps][kList];
   __shared__ u64 wbuf[TOP ? kWarps : 1][2 * kList];
-  __shared__ int last;
+  __shared__ int last, found;
+  __shared__ float bound;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = gridDim.x;
   // chunks of a row: its whole 16-byte vectors, from the first aligned element on
   const int cpr = p.chunks;
@@ -207,104 +250,166 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
     const int head = head_of(row), nvec = (p.V - head) / VN;
     Stats s = {-INFINITY, 0.f, 0.f};
     f2 z = 0ull, a = 0ull;  // this lane's sums in pairs
-    Best best = {0ull, -INFINITY, 0, wbuf[TOP ? warp : 0]};
-    bool primed = false;
+    uint32_t hot = 0u;      // TOP: bit i: a step i, i + 32, .. of this lane may have a candidate
+    float first_bound = -INFINITY;
     auto rescale = [&](float m) {  // the sums relative to a new maximum
-      const float d = s.m == -INFINITY ? 0.f : fmaxf(s.m - m, kFar), f = ex2(d * kLog2e);
+      const float d = s.m == -INFINITY ? 0.f : fmaxf((s.m - m) * kLog2e, kFar), f = ex2(d);
       const f2 f_2 = pack2(f, f);
       a = mul2(f_2, fma2(z, pack2(d, d), a));
       z = mul2(f_2, z);
       s.m = m;
     };
-    auto add = [&](float x0, float x1, f2 mr) {
-      const f2 d = add2(pack2(x0, x1), mr);
-      const float2 y = unpack2(mul2(d, pack2(kLog2e, kLog2e))), dd = unpack2(d);
-      const f2 e = pack2(ex2(y.x), ex2(y.y));
+    auto add = [&](f2 y) {  // y not below kFar, or 2^y without -inf
+      const float2 v = unpack2(y);
+      const f2 e = pack2(ex2(v.x), ex2(v.y));
       z = add2(z, e);
-      a = fma2(e, pack2(fmaxf(dd.x, kFar), fmaxf(dd.y, kFar)), a);
+      a = fma2(e, y, a);
     };
+    auto add_far = [&](f2 y) {
+      const float2 v = unpack2(y);
+      const f2 e = pack2(ex2(v.x), ex2(v.y));  // (a NaN stays one)
+      z = add2(z, e);
+      a = fma2(e, pack2(fmaxf(v.x, kFar), fmaxf(v.y, kFar)), a);
+    };
+    const f2 log2e = pack2(kLog2e, kLog2e);
     for (int k = k0; k < k1; ++k, ++u) {
       const int i = u - u0, st = i % kStages, n = vecs_in(nvec, k);
       mbar_wait(&ring.full[st], (uint32_t)((i / kStages) & 1), nullptr);
-      const uint4* c = reinterpret_cast<const uint4*>(smem + st * kChunk) + warp * (kVecs / kWarps) + lane;
       const int v0 = warp * (kVecs / kWarps) + lane;  // this lane's first vector of the chunk
+      const uint4* c = reinterpret_cast<const uint4*>(smem + st * kChunk) + v0;
+      auto chunk = [&](auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
+#pragma unroll 1
+        for (int j0 = 0; j0 < kSteps; ++j0) {
+          float x[N];
+          const int v = v0 + j0 * 32 * U;
 #pragma unroll
-      for (int j0 = 0; j0 < kSteps; ++j0) {
-        float x[N];
-        const int v = v0 + j0 * 32 * U;
+          for (int w = 0; w < U; ++w) {
+            if (kWhole || v + w * 32 < n) {
+              unpack<DT>(c[j0 * 32 * U + w * 32], x + w * VN);
+            } else {
 #pragma unroll
-        for (int w = 0; w < U; ++w) {
-          if (v + w * 32 < n) {
-            unpack<DT>(c[j0 * 32 * U + w * 32], x + w * VN);
+              for (int j = 0; j < VN; ++j) x[w * VN + j] = -INFINITY;
+            }
+          }
+          float m = x[0], lo = x[0];
+#pragma unroll
+          for (int j = 1; j + 1 < N; j += 2) m = max3(m, x[j], x[j + 1]), lo = min3(lo, x[j], x[j + 1]);
+          m = fmaxf(m, x[N - 1]), lo = fminf(lo, x[N - 1]);
+          if (m > s.m) rescale(m);
+          const float mr = s.m == -INFINITY ? 0.f : -s.m;
+          const f2 mr2 = pack2(mr, mr);
+          if ((lo + mr) * kLog2e >= kFar) {
+#pragma unroll
+            for (int j = 0; j < N; j += 2) add(mul2(add2(pack2(x[j], x[j + 1]), mr2), log2e));
           } else {
 #pragma unroll
-            for (int j = 0; j < VN; ++j) x[w * VN + j] = -INFINITY;
+            for (int j = 0; j < N; j += 2) add_far(mul2(add2(pack2(x[j], x[j + 1]), mr2), log2e));
+          }
+          if constexpr (TOP) {
+            const int step = (k - k0) * kSteps + j0;
+            if (step == 0) first_bound = __shfl_sync(kAll, sort_lanes(m, lane), p.top - 1);
+            hot |= (m >= first_bound ? 1u : 0u) << (step & 31);
           }
         }
-        if (j0 == kSteps - 1) {  // the chunk is read
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ring.empty[st]);
-        }
-        float m4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int j = 4; j < N; ++j) m4[j & 3] = fmaxf(m4[j & 3], x[j]);
-        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        if (m > s.m) rescale(m);
-        const float mr = s.m == -INFINITY ? 0.f : -s.m;
-        const f2 mr2 = pack2(mr, mr);
-#pragma unroll
-        for (int j = 0; j < N; j += 2) add(x[j], x[j + 1], mr2);
-        if constexpr (TOP) {
-          if (!primed) {  // the lanes' largest of the first step give a first threshold
-            best.thr = kth_of_lanes(m, p.top, lane);
-            primed = true;
-          }
-          if (__any_sync(kAll, m >= best.thr)) {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-              best.offer(v + (j / VN) * 32 < n, x[j], head + (k * kVecs + v + (j / VN) * 32) * VN + j % VN, p.top, lane);
-          }
-        }
-      }
+      };
+      if (n == kVecs) chunk(Yes{});
+      else chunk(No{});
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring.empty[st]);  // the chunk is read
     }
-    if (warp == 0 && (k0 == 0 || k1 == cpr)) {  // at most 2 * 15 loose elements, before and after the vectors
+    // at most 2 * 15 loose elements, before and after the vectors
+    int loose = -1;
+    float xl = -INFINITY;
+    if (warp == 0) {
       const int tail = head + nvec * VN;
-      int i = -1;
       if (lane < 16) {
-        if (k0 == 0 && lane < head) i = lane;
+        if (k0 == 0 && lane < head) loose = lane;
       } else if (k1 == cpr && tail + lane - 16 < p.V) {
-        i = tail + lane - 16;
+        loose = tail + lane - 16;
       }
-      const float x = i >= 0 ? load_elem<DT>(row, i) : -INFINITY;
-      if (x > s.m) rescale(x);
+      if (loose >= 0) xl = load_elem<DT>(row, loose);
+      if (xl > s.m) rescale(xl);
       const float mr = s.m == -INFINITY ? 0.f : -s.m;
-      add(x, -INFINITY, pack2(mr, mr));
-      if constexpr (TOP) best.offer(i >= 0, x, i, p.top, lane);
+      add_far(mul2(add2(pack2(xl, -INFINITY), pack2(mr, mr)), log2e));
     }
     const float2 z2 = unpack2(z), a2 = unpack2(a);
     s.z = z2.x + z2.y, s.a = a2.x + a2.y;
-    u64 list = 0ull;
-    if constexpr (TOP) {
-      if (best.n > 0) best.flush(p.top, lane);
-      list = best.list;
-    }
 
-    // the warps (halves of them onto the others), then the parts of the row
-    auto join = [&] {
+    // lists and statistics of the warps onto warp 0, halves of them onto the others
+    auto join_lists = [&](u64& list) {
       for (int half = kWarps / 2; half > 0; half >>= 1) {
-        if (warp >= half && warp < 2 * half) {
-          if (lane == 0) wstats[warp] = s;
-          if constexpr (TOP) wlist[warp][lane] = list;
-        }
+        if (warp >= half && warp < 2 * half) wlist[warp][lane] = list;
         bar();
-        if (warp < half) {
-          merge(s, wstats[warp + half]);
-          if constexpr (TOP) list = merge_lists(list, wlist[warp + half][lane], lane);
-        }
+        if (warp < half) list = merge_lists(list, wlist[warp + half][lane], lane);
       }
     };
+    auto join_stats = [&](Stats& x) {  // x of the warps' lanes 0, which warp 0 has after it
+      if (lane == 0) wstats[warp] = x;
+      bar();
+      if (warp == 0) {
+        x = wstats[lane & (kWarps - 1)];
+#pragma unroll
+        for (int o = kWarps / 2; o > 0; o >>= 1) {
+          const Stats y = {__shfl_xor_sync(kAll, x.m, o), __shfl_xor_sync(kAll, x.z, o), __shfl_xor_sync(kAll, x.a, o)};
+          if ((lane & o) == 0) merge(x, y);  // the upper lane's onto the lower one's
+        }
+        x = {__shfl_sync(kAll, x.m, 0), __shfl_sync(kAll, x.z, 0), __shfl_sync(kAll, x.a, 0)};
+      }
+    };
+    u64 list = 0ull;
+    if constexpr (TOP) {
+      float top = sort_lanes(s.m, lane);
+      for (int half = kWarps / 2; half > 0; half >>= 1) {
+        if (warp >= half && warp < 2 * half) wmax[warp][lane] = top;
+        bar();
+        if (warp < half) top = merge_lists(top, wmax[warp + half][lane], lane);
+      }
+      if (tid == p.top - 1) bound = top;
+      if (tid == 0) found = 0;
+      bar();
+      const float least = bound;
+      const int steps = (k1 - k0) * kSteps;
+      // every element of this warp that may reach the bound: f(whether it does, value, index)
+      auto candidates = [&](auto f) {
+        if (warp == 0) f(loose >= 0 && xl >= least, xl, loose);
+        for (unsigned go = __ballot_sync(kAll, s.m >= least); go; go &= go - 1) {
+          const int from = __ffs(go) - 1;
+          for (uint32_t h = __shfl_sync(kAll, hot, from); h; h &= h - 1)
+            for (int st = __ffs(h) - 1; st < steps; st += 32) {  // a step's 32 elements, one for each lane
+              const int k = k0 + st / kSteps, v = warp * (kVecs / kWarps) + (st % kSteps) * 32 * U + from + lane / VN * 32;
+              const int i = head + (k * kVecs + v) * VN + lane % VN;
+              const bool in = v < vecs_in(nvec, k);
+              const float x = in ? load_elem<DT>(row, i) : 0.f;
+              f(in && x >= least, x, i);
+            }
+        }
+      };
+      candidates([&](bool in, float x, int i) {
+        const unsigned go = __ballot_sync(kAll, in);
+        if (!go) return;
+        int at = lane == 0 ? atomicAdd(&found, __popc(go)) : 0;
+        at = __shfl_sync(kAll, at, 0) + __popc(go & ((1u << lane) - 1u));
+        if (in && at < 2 * kList) wbuf[0][at] = argmax_pack(x, i);
+      });
+      bar();
+      const int n = found;
+      if (n <= 2 * kList) {
+        if (warp == 0) {
+          list = sort_lanes(lane < n ? wbuf[0][lane] : 0ull, lane);
+          if (n > kList) list = merge_lists(list, sort_lanes(lane + kList < n ? wbuf[0][lane + kList] : 0ull, lane), lane);
+        }
+      } else {
+        bar();  // (warp 0's buffer is the one just counted)
+        Best best = {0ull, least, 0, wbuf[warp]};
+        candidates([&](bool in, float x, int i) { best.offer(in, x, i, p.top, lane); });
+        if (best.n > 0) best.flush(p.top, lane);
+        list = best.list;
+        join_lists(list);
+      }
+    }
     s = warp_stats(s);
-    join();
+    join_stats(s);
     const int c0 = owner((long long)t * cpr, T, G), parts = owner((long long)(t + 1) * cpr - 1, T, G) - c0 + 1;
     // a CTA has at most two parts of rows: of the row that its share begins in, and of the last
     auto place = [&](int c) { return 2 * c + (share(c, T, G) >= (long long)t * cpr ? 0 : 1); };
@@ -331,25 +436,28 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
           merge(s, Stats{f.x, f.y, f.z});
           if constexpr (TOP) list = merge_lists(list, other, lane);
         }
-        join();
+        if constexpr (TOP) join_lists(list);
+        bar();  // (what the statistics of this CTA's part were joined in)
+        join_stats(s);
         if (tid == 0) p.counters[c0] = 0u;  // as the next call expects it
       }
     }
     if (mine && warp == 0) {
-      const float lz = logf(s.z);
+      const float lz = log2f(s.z);
+      auto logprob = [&](float x) { return fmaf(-lz, kLn2, x - s.m); };
       if (lane == 0) {
-        if (p.entropy) p.entropy[t] = lz - s.a / s.z;
+        if (p.entropy) p.entropy[t] = (lz - s.a / s.z) * kLn2;
         if (p.logprob) {
           const long long y = !p.targets    ? -1
                               : p.targets64 ? static_cast<const long long*>(p.targets)[t]
                                             : (long long)static_cast<const int32_t*>(p.targets)[t];
-          p.logprob[t] = y < 0 ? 0.f : y >= p.V ? __uint_as_float(0x7fc00000u) : load_elem<DT>(row, y) - s.m - lz;
+          p.logprob[t] = y < 0 ? 0.f : y >= p.V ? __uint_as_float(0x7fc00000u) : logprob(load_elem<DT>(row, y));
         }
       }
       if constexpr (TOP) {
         if (lane < p.top) {
           p.top_ids[(long long)t * p.top + lane] = list ? (int)(0xffffffffu - (uint32_t)list) : -1;
-          p.top_logprobs[(long long)t * p.top + lane] = list ? key_value(list) - s.m - lz : -INFINITY;
+          p.top_logprobs[(long long)t * p.top + lane] = list ? logprob(key_value(list)) : -INFINITY;
         }
       }
     }
