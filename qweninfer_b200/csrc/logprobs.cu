@@ -12,8 +12,8 @@
 // go to the lower index. While a row streams by, a lane only keeps its largest logit, and
 // which of its steps reached the top-th largest of the lanes' first ones. Of the lanes'
 // largest, the top-th is then a bound that hardly more than top elements reach: the steps of
-// the lanes that reach it are read again, their elements above it sorted. (More than 64, as
-// in a row of equal values: every warp keeps a list of its best 32 instead, 32 candidates
+// the lanes that reach it are read again, their elements above it sorted. (More than 64 of
+// them or 128 steps, as in a row of equal values: every warp keeps a list of its best 32 instead, 32 candidates
 // sorted and merged into it at a time.)
 // A call reads its logits once and is bound by those bytes. They are cut into chunks of 32 KB
 // and the chunks of all rows are shared out evenly, in order, over the CTAs that are
@@ -34,6 +34,7 @@ constexpr int kStages = 2;
 constexpr int kChunk = 32768;                 // bytes; a warp's share is 8 vectors of every lane
 constexpr int kCtas = 3;                      // of an SM
 constexpr int kList = 32;
+constexpr int kPairs = 128;                   // steps that are read again
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // 2^kFar is 0 in fp32, and a sum of weights times kFar is finite: distances of masked logits
@@ -209,7 +210,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
   __shared__ u64 wlist[kWarps][kList];
   __shared__ float wmax[kWarps][kList];
   __shared__ u64 wbuf[TOP ? kWarps : 1][2 * kList];
-  __shared__ int last, found;
+  __shared__ int last, found, pairs;
+  __shared__ int2 again[TOP ? kPairs : 1];
   __shared__ float bound;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = gridDim.x;
   // chunks of a row: its whole 16-byte vectors, from the first aligned element on
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
         if (warp < half) top = merge_lists(top, wmax[warp + half][lane], lane);
       }
       if (tid == p.top - 1) bound = top;
-      if (tid == 0) found = 0;
+      if (tid == 0) found = pairs = 0;
       bar();
       const float least = bound;
       const int steps = (k1 - k0) * kSteps;
@@ -385,15 +387,48 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
             }
         }
       };
-      candidates([&](bool in, float x, int i) {
+      // Steps to read again, as (warp and lane, step), shared out over the warps; their elements
+      // that reach the bound go into one buffer.
+      if (s.m >= least)
+        for (uint32_t h = hot; h; h &= h - 1)
+          for (int st = __ffs(h) - 1; st < steps; st += 32) {
+            const int at = atomicAdd(&pairs, 1);
+            if (at < kPairs) again[at] = make_int2(tid, st);
+          }
+      bar();
+      const int np = pairs;
+      auto push = [&](bool in, float x, int i) {
         const unsigned go = __ballot_sync(kAll, in);
         if (!go) return;
         int at = lane == 0 ? atomicAdd(&found, __popc(go)) : 0;
         at = __shfl_sync(kAll, at, 0) + __popc(go & ((1u << lane) - 1u));
         if (in && at < 2 * kList) wbuf[0][at] = argmax_pack(x, i);
-      });
+      };
+      if (np <= kPairs) {
+        if (warp == 0) push(loose >= 0 && xl >= least, xl, loose);
+        constexpr int B = 4;  // loads under way together
+        for (int q = warp; q < np; q += B * kWarps) {
+          float x[B];
+          int i[B];
+#pragma unroll
+          for (int b = 0; b < B; ++b) {
+            const int2 pr = again[min(q + b * kWarps, kPairs - 1)];
+            i[b] = -1, x[b] = 0.f;
+            if (q + b * kWarps < np) {
+              const int k = k0 + pr.y / kSteps;
+              const int v = (pr.x >> 5) * (kVecs / kWarps) + (pr.y % kSteps) * 32 * U + (pr.x & 31) + lane / VN * 32;
+              if (v < vecs_in(nvec, k)) {
+                i[b] = head + (k * kVecs + v) * VN + lane % VN;
+                x[b] = load_elem<DT>(row, i[b]);
+              }
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < B; ++b) push(i[b] >= 0 && x[b] >= least, x[b], i[b]);
+        }
+      }
       bar();
-      const int n = found;
+      const int n = np <= kPairs ? found : 2 * kList + 1;
       if (n <= 2 * kList) {
         if (warp == 0) {
           list = sort_lanes(lane < n ? wbuf[0][lane] : 0ull, lane);
@@ -485,7 +520,10 @@ LogprobPlan logprob_plan(int M, int V, int dtype) {
   r.chunks = (V / vn + kv - 1) / kv;
   if (r.chunks < 1) r.chunks = 1;
   const long long T = (long long)M * r.chunks, most = (long long)kCtas * sm_count();
-  r.ctas = (int)(T < most ? T : most);
+  // as many chunks for each as the resident CTAs need, then no more CTAs than that takes: an
+  // uneven share would only give some CTAs the ends of two rows
+  const long long per = (T + most - 1) / most;
+  r.ctas = (int)((T + per - 1) / per);
   r.scratch = (long long)r.ctas * 2 * (16 + kList * 8);
   return r;
 }

@@ -36,6 +36,47 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     vocabulary NaN. A logit of -inf has probability 0. A row with a NaN or +inf logit, or of
     -inf alone, has NaN results. Exponentials and sums are fp32. Enqueued on the current
     stream."""
+    key = (logits.shape, logits.stride(), logits.dtype, logits.device, top)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _plan(logits, top)
+        if len(_plans) >= 4096:
+            _plans.clear()
+        _plans[key] = plan
+    M, V, dtype, ld, nbytes = plan
+    dev = logits.device
+    if targets is not None and not (targets.shape == (M,) and targets.dtype in _INTS and targets.device == dev
+                                    and targets.is_contiguous()):
+        targets = _targets(targets, M, V, dev)
+    # the outputs share one allocation
+    buf = torch.empty(2 * M * (1 + top), dtype=torch.float32, device=dev)
+    if top:
+        lp, ent, ids, lps = buf.split((M, M, M * top, M * top))
+        r = TokenLogprobs(lp if targets is not None else None, ent, ids.view(torch.int32).view(M, top), lps.view(M, top))
+    else:
+        lp, ent = buf.split(M) if M else (buf, buf)
+        r = TokenLogprobs(lp if targets is not None else None, ent, None, None)
+    if M == 0:
+        return r
+    base = buf.data_ptr()
+    with _lib.on_device(dev):
+        stream = _lib.stream_ptr(dev)
+        data, counters, _keep = _lib.scratch(dev, stream, nbytes, _lib.LOGPROBS_COUNTERS)
+        code = _lib.lib().qi_token_logprobs(
+            logits.data_ptr(), dtype, ld, None if targets is None else targets.data_ptr(),
+            targets is not None and targets.dtype == torch.int64, M, V, top, None if targets is None else base,
+            base + 4 * M, base + 8 * M, base + 8 * M + 4 * M * top, data, nbytes, counters, stream)
+    if code:
+        _lib.check(code, "qi_token_logprobs")
+    return r
+
+
+_INTS = (torch.int32, torch.int64)
+_plans: dict[tuple, tuple] = {}
+
+
+def _plan(logits: torch.Tensor, top: int) -> tuple:
+    """What the shapes of a call decide, checked: (M, V, element type, row stride, scratch)."""
     if logits.device.type != "cuda":
         raise _lib.QiError(f"token_logprobs: qweninfer_b200 computes on CUDA (sm_100) tensors only, got {logits.device}")
     if logits.dim() != 2 or logits.shape[1] == 0:
@@ -47,35 +88,20 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
         raise ValueError("a row of logits must be contiguous and rows must not overlap")
     if not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"top must be 0..{min(MAX_TOP, V)}, got {top}")
-    if targets is not None:
-        if targets.dim() != 1 or targets.shape[0] != M or targets.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"targets must be ({M},) int32 or int64, got {tuple(targets.shape)} {targets.dtype}")
-        if targets.device.type == "cpu":
-            if M and int(targets.max()) >= V:
-                raise IndexError("target outside the vocabulary")
-            targets = targets.to(logits.device)
-        elif targets.device != logits.device:
-            raise ValueError(f"targets on {targets.device}, logits on {logits.device}")
-        targets = targets.contiguous()
-    dev = logits.device
-    # the outputs share one allocation
-    buf = torch.empty(2 * M * (1 + top), dtype=torch.float32, device=dev)
-    if top:
-        lp, ent, ids, lps = buf.split((M, M, M * top, M * top))
-        r = TokenLogprobs(lp if targets is not None else None, ent, ids.view(torch.int32).view(M, top), lps.view(M, top))
-    else:
-        lp, ent = buf.split(M) if M else (buf, buf)
-        r = TokenLogprobs(lp if targets is not None else None, ent, None, None)
-    if M == 0:
-        return r
-    with _lib.on_device(dev):
-        L = _lib.lib()
-        stream = _lib.stream_ptr(dev)
-        nbytes = L.qi_token_logprobs_scratch(M, V, _lib.DTYPES[logits.dtype])
-        data, counters, _keep = _lib.scratch(dev, stream, nbytes, _lib.LOGPROBS_COUNTERS)
-        _lib.check(L.qi_token_logprobs(
-            logits.data_ptr(), _lib.DTYPES[logits.dtype], logits.stride(0) if M > 1 else V, _lib.ptr(targets),
-            int(targets is not None and targets.dtype == torch.int64), M, V, top, _lib.ptr(r.logprob),
-            r.entropy.data_ptr(), _lib.ptr(r.top_ids), _lib.ptr(r.top_logprobs), data, nbytes, counters, stream),
-            "qi_token_logprobs")
-    return r
+    dtype = _lib.DTYPES[logits.dtype]
+    with _lib.on_device(logits.device):
+        nbytes = _lib.lib().qi_token_logprobs_scratch(M, V, dtype)
+    return M, V, dtype, logits.stride(0) if M > 1 else V, nbytes
+
+
+def _targets(targets: torch.Tensor, M: int, V: int, dev: torch.device) -> torch.Tensor:
+    """Targets as (M,) integers on the logits' device; those given on the host are checked."""
+    if targets.dim() != 1 or targets.shape[0] != M or targets.dtype not in _INTS:
+        raise ValueError(f"targets must be ({M},) int32 or int64, got {tuple(targets.shape)} {targets.dtype}")
+    if targets.device.type == "cpu":
+        if M and int(targets.max()) >= V:
+            raise IndexError("target outside the vocabulary")
+        targets = targets.to(dev)
+    elif targets.device != dev:
+        raise ValueError(f"targets on {targets.device}, logits on {dev}")
+    return targets.contiguous()
