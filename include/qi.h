@@ -299,6 +299,16 @@ typedef struct {
   int page_size;
   int pages_per_row;
   int n_pages;
+  /* 8-bit cache (qi_kv_layer, with its formats, blocks and scales; k and v then point to
+   * codes, every layer's after the other, and so do the scales), and the window and first
+   * tokens that attention sees (qi_cache_attention; window 0: all keys). All zero for a bf16
+   * cache without a window. Only qi_forward with ws->use_tc reads them. */
+  int format;               /* QI_KV_*                                            */
+  int block;
+  float* k_scale;
+  float* v_scale;
+  int window;
+  int sinks;
 } qi_cache;
 
 typedef struct {
@@ -337,6 +347,8 @@ typedef struct {
                                of its row and the row's keys below its position are
                                in the cache before the call, so attention copies
                                them while the previous launch still runs          */
+  float* kv_stage;          /* (max_tokens, 4, 64): keys and values of the forward's
+                               tokens on their way into an 8-bit cache (else unused) */
 } qi_workspace;
 
 /* Full Qwen2 forward of M tokens (qweninfer/models/qwen2.py:263-292 with a cache):
@@ -362,6 +374,7 @@ int qi_forward(const qi_model* model, const qi_cache* cache, const qi_workspace*
 #define QI_LAUNCH_GATE_UP 4   /* RMSNorm + gate/up + SwiGLU                      */
 #define QI_LAUNCH_DOWN 5      /* down + residual                                 */
 #define QI_LAUNCH_HEAD 6      /* final RMSNorm + tied head + argmax              */
+#define QI_LAUNCH_APPEND 7    /* keys and values into an 8-bit cache             */
 
 /* qi_forward (tensor-core projections, ws->use_tc != 0) with a CUDA event recorded before
  * the first launch and after every launch: kinds[i] (QI_LAUNCH_*) and us[i] (microseconds

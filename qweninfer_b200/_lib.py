@@ -26,7 +26,7 @@ LOGPROBS_COUNTERS = 1024
 # element types of activations (QI_F32, QI_BF16, QI_F16)
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # launch kinds of qi_forward_launch_times
-LAUNCH_KINDS = ("embed", "qkv", "attention", "o_proj", "gate_up", "down", "head")
+LAUNCH_KINDS = ("embed", "qkv", "attention", "o_proj", "gate_up", "down", "head", "kv_append")
 
 vp = C.c_void_p
 i32 = C.c_int
@@ -47,7 +47,8 @@ class QiModel(C.Structure):
 
 class QiCache(C.Structure):
     _fields_ = [("k", vp), ("v", vp), ("cache_rows", i32), ("max_len", i32), ("page_table", vp),
-                ("page_size", i32), ("pages_per_row", i32), ("n_pages", i32)]
+                ("page_size", i32), ("pages_per_row", i32), ("n_pages", i32), ("format", i32), ("block", i32),
+                ("k_scale", vp), ("v_scale", vp), ("window", i32), ("sinks", i32)]
 
 
 class QiKvLayer(C.Structure):
@@ -61,7 +62,7 @@ class QiWorkspace(C.Structure):
                 ("attn_counters", vp), ("max_tokens", i32), ("max_splits", i32),
                 ("split_keys", i32), ("err", vp), ("use_tc", i32), ("act_x", vp), ("act_attn", vp),
                 ("act_h", vp), ("ss", vp), ("ss_ld", i32), ("tc_scratch", vp), ("tc_scratch_floats", i64),
-                ("tc_counters", vp), ("tc_counters_len", i32), ("query_run", i32)]
+                ("tc_counters", vp), ("tc_counters_len", i32), ("query_run", i32), ("kv_stage", vp)]
 
 
 # name -> (restype, argtypes), exactly the declarations of include/qi.h

@@ -408,6 +408,73 @@ KvLayout kv_layout(const qi_cache* c) {
   }
   return kv;
 }
+// Layer li of a cache for the kernels of cache layers (8-bit formats, windows).
+qi_kv_layer cache_layer(const qi_cache* c, int li) {
+  qi_kv_layer l = {};
+  const long long cells = c->page_table ? (long long)c->n_pages * kKvHeads * c->page_size
+                                        : (long long)c->cache_rows * kKvHeads * c->max_len;
+  const long long bytes = cells * kHeadDim * (c->format == QI_KV_BF16 ? 2 : 1);
+  l.k = reinterpret_cast<uint8_t*>(c->k) + li * bytes;
+  l.v = reinterpret_cast<uint8_t*>(c->v) + li * bytes;
+  l.format = c->format;
+  l.block = c->block;
+  l.cache_rows = c->cache_rows;
+  l.kv_heads = kKvHeads;
+  l.max_len = c->max_len;
+  l.head_dim = kHeadDim;
+  l.page_table = c->page_table;
+  l.page_size = c->page_size;
+  l.pages_per_row = c->pages_per_row;
+  l.n_pages = c->n_pages;
+  if (c->format != QI_KV_BF16) {
+    const long long blocks = c->page_table ? (long long)c->n_pages * kKvHeads * (c->page_size / c->block)
+                                           : (long long)c->cache_rows * kKvHeads * ((c->max_len + c->block - 1) / c->block);
+    l.k_scale = c->k_scale + li * blocks;
+    l.v_scale = c->v_scale + li * blocks;
+  }
+  return l;
+}
+// Formats and windows that the forward takes (bad_layer does the rest).
+bool plain_cache(const qi_cache* c) { return c->format == QI_KV_BF16 && c->window == 0; }
+bool bad_format(const qi_cache* c, const qi_workspace* ws) {
+  if (c->window < 0 || c->sinks < 0) return true;
+  if (plain_cache(c)) return false;
+  if (!ws->use_tc) return true;
+  if (c->format != QI_KV_BF16) {
+    if (c->format != QI_KV_INT8 && c->format != QI_KV_E4M3) return true;
+    if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128) return true;
+    if (!c->k_scale || !c->v_scale || !ws->kv_stage) return true;
+  }
+  const qi_kv_layer l = cache_layer(c, 0);
+  return bad_layer(&l);
+}
+// Attention over layer `l` within a forward, into the o projection's activation tiles.
+int attention_over(const qi_kv_layer& l, const qi_cache* c, const qi_workspace* ws, const int32_t* pos,
+                   const int32_t* rows, int M, int out_nt, cudaStream_t s) {
+  CacheAttnParams p = {};
+  p.c = l;
+  p.q = ws->q;
+  p.dtype = QI_F32;
+  p.q_st = kHidden;
+  p.q_sh = kHeadDim;
+  p.heads = kHeads;
+  p.group = kGqa;
+  p.rows = rows;
+  p.pos = pos;
+  p.M = M;
+  p.window = c->window;
+  p.sinks = c->sinks;
+  p.out_act = ws->act_attn;
+  p.out_nt = out_nt;
+  p.part = ws->attn_part;
+  p.counters = ws->attn_counters;
+  p.err = ws->err;
+  CacheAttnPlan plan = cache_attention_plan(l, kHeads, M, c->window, c->sinks, ws->query_run);
+  const bool scratch = ws->attn_part && ws->attn_counters && ws->max_splits > 1;
+  cache_attention_fit(plan, l, kHeads, M, scratch ? (long long)M * kKvHeads * ws->max_splits * kGqa * (kHeadDim + 2) : 0,
+                      scratch ? (long long)M * kKvHeads : 0);
+  return rc(launch_cache_attention(p, plan, s, true));
+}
 long long layer_kv_elems(const qi_cache* c) {
   return c->page_table ? (long long)c->n_pages * kKvHeads * c->page_size * kHeadDim
                        : (long long)c->cache_rows * kKvHeads * c->max_len * kHeadDim;
@@ -512,7 +579,9 @@ int forward_tc(const qi_model* model, const qi_cache* cache, const qi_workspace*
     p.n_mtiles = kQkvRows / 128;
     p.act_in = ws->act_x;
     p.ss_in = ws->ss;
-    p.epi = cache->page_table ? kTcQkvRopePaged : kTcQkvRope;
+    const bool kv8 = cache->format != QI_KV_BF16;
+    p.epi = kv8 ? kTcQkvRopeStage : cache->page_table ? kTcQkvRopePaged : kTcQkvRope;
+    p.kv_stage = ws->kv_stage;
     p.bias = L.b_qkv;
     p.rope_cos = model->rope_cos;
     p.rope_sin = model->rope_sin;
@@ -525,9 +594,20 @@ int forward_tc(const qi_model* model, const qi_cache* cache, const qi_workspace*
     p.cache_rows = cache->cache_rows;
     prefetch(p, 4 * li);
     if ((r = launch(p, 0)) != QI_OK) return r;
-    r = attention(ws->q, kl, vl, pos, rows, M, cache->max_len, ws->split_keys, ws->max_splits, nullptr,
-                  ws->attn_part, ws->attn_counters, ws->err, s, pdl, ws->act_attn, tiles[1], cache->cache_rows,
-                  ws->query_run, kv);
+    if (plain_cache(cache)) {
+      r = attention(ws->q, kl, vl, pos, rows, M, cache->max_len, ws->split_keys, ws->max_splits, nullptr,
+                    ws->attn_part, ws->attn_counters, ws->err, s, pdl, ws->act_attn, tiles[1], cache->cache_rows,
+                    ws->query_run, kv);
+    } else {
+      const qi_kv_layer layer = cache_layer(cache, li);
+      if (kv8) {
+        r = rc(launch_kv8_append(layer, ws->kv_stage, ws->kv_stage + kKvHeads * kHeadDim, QI_F32,
+                                 2 * kKvHeads * kHeadDim, kHeadDim, 2 * kKvHeads * kHeadDim, kHeadDim, rows, pos, M,
+                                 ws->err, s, pdl));
+        if (r != QI_OK || (r = mark(QI_LAUNCH_APPEND)) != QI_OK) return r;
+      }
+      r = attention_over(layer, cache, ws, pos, rows, M, tiles[1], s);
+    }
     if (r != QI_OK || (r = mark(QI_LAUNCH_ATTENTION)) != QI_OK) return r;
     p = params(1, tiles[2]);  // o_proj + residual; emits RMSNorm(post_attention) inputs
     p.w = L.w_o;
@@ -860,7 +940,7 @@ int qi_forward(const qi_model* model, const qi_cache* cache, const qi_workspace*
                qi_stream_t stream) {
   if (bad_forward_args(model, cache, ws, ids, pos, rows, M, head_lo, head_stride, n_head, logits, logits_ld,
                        argmax_slots) ||
-      bad_paging(cache) || (cache->page_table && !ws->use_tc))
+      bad_paging(cache) || (cache->page_table && !ws->use_tc) || bad_format(cache, ws))
     return QI_ERR_ARG;
   if (ws->use_tc) return forward_tc(model, cache, ws, ids, pos, rows, M, head_lo, head_stride, n_head, logits,
                                     logits_bf16, logits_ld, argmax_slots, as_stream(stream));
@@ -900,7 +980,7 @@ int qi_forward_launch_times(const qi_model* model, const qi_cache* cache, const 
                             int max_launches, int* n_launches) {
   if (bad_forward_args(model, cache, ws, ids, pos, rows, M, head_lo, head_stride, n_head, logits, logits_ld,
                        argmax_slots) ||
-      bad_paging(cache) || !ws->use_tc || !kinds || !us || !n_launches || max_launches <= 0)
+      bad_paging(cache) || !ws->use_tc || bad_format(cache, ws) || !kinds || !us || !n_launches || max_launches <= 0)
     return QI_ERR_ARG;
   LaunchTimer lt;
   lt.s = as_stream(stream);

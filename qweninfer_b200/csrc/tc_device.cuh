@@ -246,6 +246,8 @@ struct ChunkPre<kTcQkvRope, CT> {
 template <int CT>
 struct ChunkPre<kTcQkvRopePaged, CT> : ChunkPre<kTcQkvRope, CT> {};
 template <int CT>
+struct ChunkPre<kTcQkvRopeStage, CT> : ChunkPre<kTcQkvRope, CT> {};
+template <int CT>
 struct ChunkPre<kTcResidual, CT> {
   float xo[CT], wn;
 };
@@ -307,6 +309,8 @@ __device__ __forceinline__ void finish_rows(const TcParams& p, int n, int tbase,
         const int t = tbase + i;
         if (head < kHeads) {
           p.q[(long long)t * kHidden + head * kHeadDim + d] = x[i];
+        } else if constexpr (EPI == kTcQkvRopeStage) {
+          p.kv_stage[(long long)t * (2 * kKvHeads * kHeadDim) + (head - kHeads) * kHeadDim + d] = x[i];
         } else if constexpr (EPI == kTcQkvRopePaged) {
           const long long o = kv_slot_ok(p, tpos[i], trow[i]) ? kv_offset(p.kv, p.max_len, trow[i], kvh, tpos[i]) : -1;
           if (o >= 0) kvbase[o + d] = f32_to_bf16_rn(x[i]);

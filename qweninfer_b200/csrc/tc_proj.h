@@ -15,11 +15,12 @@ enum TcEpilogue : int {
   kTcSwiglu = 3,    // h = silu(gate) * up -> activation tiles of the down projection
   kTcLogits = 4,    // optional logits + packed argmax of the head tokens
   kTcQkvRopePaged = 5,  // kTcQkvRope into a paged cache (TcParams::kv)
+  kTcQkvRopeStage = 6,  // kTcQkvRope with k/v as fp32 rows (TcParams::kv_stage), for an 8-bit cache
 };
 
-// the QKV epilogue kinds (packed or paged KV append)
+// the QKV epilogue kinds (packed or paged KV append, or staged keys and values)
 template <int EPI>
-constexpr bool kIsQkv = EPI == kTcQkvRope || EPI == kTcQkvRopePaged;
+constexpr bool kIsQkv = EPI == kTcQkvRope || EPI == kTcQkvRopePaged || EPI == kTcQkvRopeStage;
 
 // Activation tiles: for inner size K and token tile NT (8..128, power of two), token t,
 // column k, half `part` (0 = hi = bf16(x), 1 = lo = bf16(x - hi)):
@@ -63,6 +64,7 @@ struct TcParams {
   int max_len;
   int cache_rows;  // rows of the cache (0: rows are not checked)
   KvLayout kv;     // packed (kv.table == nullptr) or paged cache
+  float* kv_stage; // (M, 4, 64): K heads, then V heads
   // residual / swiglu
   float* x;
   const float* next_norm_w;

@@ -22,7 +22,7 @@ from dataclasses import dataclass, field
 
 import torch
 
-from qweninfer_b200.engine.kv_cache import KVCache, PagedKVCache
+from qweninfer_b200.engine.kv_cache import Kv8Cache, KVCache, PagedKv8Cache, PagedKVCache
 from qweninfer_b200.engine.runner import DecodeRunner
 
 
@@ -38,6 +38,8 @@ class Request:
     finished: float | None = None
     length: int = 0
     last: int = 0
+    # with Engine(logprobs=...): one TokenInfo (models/logprobs.py) for each output token
+    logprobs: list = field(default_factory=list)
 
     @property
     def done(self) -> bool:
@@ -53,23 +55,35 @@ class Engine:
                  static: bool = False, max_prefills_per_step: int | None = None,
                  pad_to: list[int] | None = None, cuda_graphs: bool = True,
                  record: bool = False, batch_prefill: bool = True, page_size: int = 0,
-                 kv_pages: int | None = None) -> None:
+                 kv_pages: int | None = None, kv_format: str | None = None, kv_block: int = 32,
+                 attn_window: int = 0, attn_sinks: int = 0, logprobs: int | None = None) -> None:
         """engine.py:62-98. Extra keywords: `cuda_graphs` (capture each decode batch size),
         `record` (keep a per-step trace of scheduler actions in `self.trace`),
         `batch_prefill` (prefill a step's admissions together; same decisions) and
         `page_size` (> 0: a PagedKVCache of pages of that many positions, `kv_pages` pages
-        per layer; row moves then move page-table entries; same decisions)."""
+        per layer; row moves then move page-table entries; same decisions), `kv_format`
+        ("int8" or "e4m3": an 8-bit cache with a scale for each `kv_block` positions and KV
+        head), `attn_window` and `attn_sinks` (> 0: attention sees only the last attn_window
+        positions of a row and its first attn_sinks; paged caches give back the pages in
+        between) and `logprobs` (0..32: with every output token its log probability, entropy
+        and that many alternatives in Request.logprobs)."""
         if pad_to is not None:
             if len(pad_to) <= max_slots or any(pad_to[n] < n for n in range(max_slots + 1)):
                 raise ValueError("pad_to needs an entry n -> size >= n for n = 0..max_slots")
         rows = max([max_slots] + (pad_to[: max_slots + 1] if pad_to else []))
         self.model = model
         self.device = model.norm.weight.device
+        cls, extra = self.cache_cls, {}
         if page_size:
-            self.cache = PagedKVCache(model.cfg, rows, max_len, dtype=model.dtype, device=self.device,
-                                      page_size=page_size, n_pages=kv_pages)
-        else:
-            self.cache = self.cache_cls(model.cfg, rows, max_len, dtype=model.dtype, device=self.device)
+            cls = PagedKv8Cache if kv_format else PagedKVCache
+            extra.update(page_size=page_size, n_pages=kv_pages)
+        elif kv_format:
+            cls = Kv8Cache
+        if kv_format:
+            extra.update(format=kv_format, block_tokens=kv_block)
+        if attn_window or attn_sinks:
+            extra.update(attn_window=attn_window, attn_sinks=attn_sinks)
+        self.cache = cls(model.cfg, rows, max_len, dtype=model.dtype, device=self.device, **extra)
         self.max_slots, self.max_len = max_slots, max_len
         self.eos_ids = eos_ids or set()
         self.static = static
@@ -78,7 +92,9 @@ class Engine:
         self.pad_to = pad_to
         self.waiting: deque[Request] = deque()
         self.active: list[Request] = []
-        self.runner = self.runner_cls(model, self.cache, max_batch=rows, cuda_graphs=cuda_graphs)
+        self.logprobs = logprobs
+        self.runner = self.runner_cls(model, self.cache, max_batch=rows, cuda_graphs=cuda_graphs,
+                                      **({} if logprobs is None else {"logprobs": logprobs}))
         self.trace: list[dict] | None = [] if record else None
         self._rec: dict | None = None
 
@@ -97,11 +113,13 @@ class Engine:
         if release is not None:
             release(row)
 
-    def _finish_check(self, req: Request, tok: int) -> bool:
-        """engine.py:109-113."""
+    def _finish_check(self, req: Request, tok: int, i: int) -> bool:
+        """engine.py:109-113, for token i of the runner's last call."""
         if tok in self.eos_ids:
             return True
         req.output.append(tok)
+        if self.logprobs is not None:
+            req.logprobs.append(self.runner.last_logprobs[i])
         return len(req.output) >= req.max_new_tokens
 
     def _admit(self) -> list[Request]:
@@ -131,12 +149,12 @@ class Engine:
             else:
                 toks = [self.runner.prefill(rows[0], run[0].prompt)]
             now = time.perf_counter()
-            for req, row, tok in zip(run, rows, toks):
+            for i, (req, row, tok) in enumerate(zip(run, rows, toks)):
                 req.first_token = now
                 admitted += 1
                 if self._rec is not None:
                     self._rec["admit"].append([req.rid, row, len(req.prompt), tok])
-                if self._finish_check(req, tok):
+                if self._finish_check(req, tok, i):
                     req.finished = req.first_token
                     done.append(req)
                     self._release(row)  # the next admission reuses the row
@@ -166,7 +184,7 @@ class Engine:
         for i, (req, tok) in enumerate(zip(self.active, nxt)):
             req.length += 1
             req.last = tok
-            if self._finish_check(req, tok):
+            if self._finish_check(req, tok, i):
                 req.finished = now
                 finished_rows.append(i)
         return finished_rows

@@ -39,9 +39,20 @@ def _require(t: torch.Tensor, name: str, device: torch.device) -> None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
 
 
+def _window(attn_window: int, attn_sinks: int) -> tuple[int, int]:
+    if attn_window < 0 or attn_sinks < 0:
+        raise ValueError(f"attn_window and attn_sinks must not be negative; got {attn_window} and {attn_sinks}")
+    return attn_window, attn_sinks
+
+
 class KVCache:
+    # what the model's attention sees of a row: the last `attn_window` positions (0: all) and
+    # the first `attn_sinks`
+    attn_window = attn_sinks = 0
+
     def __init__(self, cfg: Qwen2Config, max_batch: int, max_len: int,
-                 dtype: torch.dtype = torch.float16, device: str | torch.device = "cuda") -> None:
+                 dtype: torch.dtype = torch.float16, device: str | torch.device = "cuda",
+                 attn_window: int = 0, attn_sinks: int = 0) -> None:
         # The kernels read and write a bfloat16 cache (the reference's cache dtype for a
         # bf16 model). A float16 or float32 request (the reference's default is float16)
         # gets the same bfloat16 storage: `dtype` is accepted for API compatibility.
@@ -54,12 +65,14 @@ class KVCache:
         self.max_len = max_len
         self.window = 0
         self.row_start = 0
+        self.attn_window, self.attn_sinks = _window(attn_window, attn_sinks)
         self._native: _lib.QiCache | None = None
 
     def native(self) -> _lib.QiCache:
         if self._native is None:
             self._native = _lib.QiCache(self.k.data_ptr(), self.v.data_ptr(), self.max_batch, self.max_len,
-                                        None, 0, 0, 0)
+                                        None, 0, 0, 0, _lib.QI_KV_BF16, 0, None, None, self.attn_window,
+                                        self.attn_sinks)
         return self._native
 
     # ---------------------------------------------------------- operators of a layer
@@ -204,6 +217,9 @@ class KVCache:
     def release(self, row: int) -> None:
         """The row's request is gone (no-op for packed rows)."""
 
+    def trim(self, row: int, length: int) -> None:
+        """Give back what no query at position `length` or later sees (no-op for packed rows)."""
+
     def sync(self) -> None:
         """Publish storage changes to the device before a forward (no-op)."""
 
@@ -246,7 +262,8 @@ class PagedKVCache(KVCache):
 
     def __init__(self, cfg: Qwen2Config, max_batch: int, max_len: int,
                  dtype: torch.dtype = torch.float16, device: str | torch.device = "cuda",
-                 page_size: int = 128, n_pages: int | None = None) -> None:
+                 page_size: int = 128, n_pages: int | None = None,
+                 attn_window: int = 0, attn_sinks: int = 0) -> None:
         if dtype not in (torch.bfloat16, torch.float16, torch.float32):
             raise ValueError(f"KV cache dtype must be bfloat16, float16 or float32; got {dtype}")
         if page_size < 128 or page_size % 128:
@@ -256,27 +273,32 @@ class PagedKVCache(KVCache):
         self.n_pages = n_pages if n_pages is not None else max_batch * self.pages_per_row
         if self.n_pages < 1:
             raise ValueError("the pool needs at least one page")
-        shape = (cfg.num_hidden_layers, self.n_pages, cfg.num_key_value_heads, page_size, cfg.head_dim)
-        self.k = torch.zeros(shape, dtype=torch.bfloat16, device=device)
-        self.v = torch.zeros(shape, dtype=torch.bfloat16, device=device)
+        self._allocate((cfg.num_hidden_layers, self.n_pages, cfg.num_key_value_heads, page_size, cfg.head_dim), device)
         self.max_batch = max_batch
         self.max_len = max_len
         self.window = 0
         self.row_start = 0
+        self.attn_window, self.attn_sinks = _window(attn_window, attn_sinks)
         dev = torch.device(device)
         self.table_host = torch.full((max_batch, self.pages_per_row), -1, dtype=torch.int32,
                                      pin_memory=dev.type == "cuda")
         self.table = self.table_host.to(dev)
         self._t = self.table_host.numpy()
         self.mapped = np.zeros(max_batch, dtype=np.int64)   # pages mapped per row (a prefix)
+        self.trimmed = np.zeros(max_batch, dtype=np.int64)  # of them, looked at by `trim`
         self.free = list(range(self.n_pages - 1, -1, -1))   # stack of free page ids
         self.dirty = False
         self._native = None
 
+    def _allocate(self, shape: tuple, device: str | torch.device) -> None:
+        self.k = torch.zeros(shape, dtype=torch.bfloat16, device=device)
+        self.v = torch.zeros(shape, dtype=torch.bfloat16, device=device)
+
     def native(self) -> _lib.QiCache:
         if self._native is None:
             self._native = _lib.QiCache(self.k.data_ptr(), self.v.data_ptr(), self.max_batch, self.max_len,
-                                        self.table.data_ptr(), self.page_size, self.pages_per_row, self.n_pages)
+                                        self.table.data_ptr(), self.page_size, self.pages_per_row, self.n_pages,
+                                        _lib.QI_KV_BF16, 0, None, None, self.attn_window, self.attn_sinks)
         return self._native
 
     def _layer(self, i: int) -> _lib.QiKvLayer:
@@ -305,11 +327,25 @@ class PagedKVCache(KVCache):
 
     def release(self, row: int) -> None:
         for j in range(int(self.mapped[row]) - 1, -1, -1):
-            self.free.append(int(self._t[row, j]))
+            if self._t[row, j] >= 0:
+                self.free.append(int(self._t[row, j]))
             self._t[row, j] = -1
         if self.mapped[row]:
             self.dirty = True
-        self.mapped[row] = 0
+        self.mapped[row] = self.trimmed[row] = 0
+
+    def trim(self, row: int, length: int) -> None:
+        """With a window, return the pages that no query at position `length` or later sees:
+        those that end before its window and hold no first tokens."""
+        if not self.attn_window:
+            return
+        end = min(max(0, length - self.attn_window + 1) // self.page_size, int(self.mapped[row]))
+        for j in range(int(self.trimmed[row]), end):
+            if j * self.page_size >= self.attn_sinks and self._t[row, j] >= 0:
+                self.free.append(int(self._t[row, j]))
+                self._t[row, j] = -1
+                self.dirty = True
+        self.trimmed[row] = max(int(self.trimmed[row]), end)
 
     def move_row(self, src: int, dst: int, length: int) -> None:
         """Row dst takes over row src's pages (positions [0, length) and any beyond);
@@ -318,9 +354,9 @@ class PagedKVCache(KVCache):
             return
         self.release(dst)
         self._t[dst] = self._t[src]
-        self.mapped[dst] = self.mapped[src]
+        self.mapped[dst], self.trimmed[dst] = self.mapped[src], self.trimmed[src]
         self._t[src] = -1
-        self.mapped[src] = 0
+        self.mapped[src] = self.trimmed[src] = 0
         self.dirty = True
 
     def move_rows(self, moves: list[tuple[int, int, int]]) -> None:
@@ -339,47 +375,38 @@ class PagedKVCache(KVCache):
         raise NotImplementedError("the paged cache is written by the forward's kernels only")
 
 
-class Kv8Cache(KVCache):
-    """K and V as 8-bit codes with block scales: `k`, `v` (layers, max_batch, kv_heads,
-    max_len, head_dim) int8 or float8_e4m3fn and `k_scale`, `v_scale` (layers, max_batch,
-    kv_heads, ceil(max_len / block_tokens)) fp32. The scale of a block of `block_tokens`
-    (16, 32, 64 or 128) positions of one row and head is the least power of two s with
-    127 s (int8) or 448 s (e4m3) >= all its values; the codes stand for code * s. `int8`
-    is the more exact on even-sized values (a step of at most amax / 63.5), `e4m3` keeps
-    small values next to large ones (relative steps of 2^-3).
-
-    `append` writes new tokens, `attend` reads them (KVCache.attend), `values` gives back
-    what the codes stand for."""
+class _Codes:
+    """K and V as 8-bit codes with block scales: what Kv8Cache and PagedKv8Cache share."""
 
     FORMATS = {"int8": (_lib.QI_KV_INT8, torch.int8), "e4m3": (_lib.QI_KV_E4M3, torch.float8_e4m3fn)}
 
-    def __init__(self, cfg: Qwen2Config, max_batch: int, max_len: int,
-                 dtype: torch.dtype = torch.float16, device: str | torch.device = "cuda",
-                 format: str = "int8", block_tokens: int = 32) -> None:
-        if dtype not in (torch.bfloat16, torch.float16, torch.float32):
-            raise ValueError(f"KV cache dtype must be bfloat16, float16 or float32; got {dtype}")
+    def _format(self, format: str, block_tokens: int) -> None:
         if format not in self.FORMATS:
             raise ValueError(f"format must be one of {sorted(self.FORMATS)}; got {format!r}")
         if block_tokens not in (16, 32, 64, 128):
             raise ValueError(f"block_tokens must be 16, 32, 64 or 128; got {block_tokens}")
         self.format, self.block_tokens = format, block_tokens
-        shape = (cfg.num_hidden_layers, max_batch, cfg.num_key_value_heads, max_len, cfg.head_dim)
-        blocks = shape[:3] + (-(-max_len // block_tokens),)
-        code = self.FORMATS[format][1]
+
+    def _allocate(self, shape: tuple, device: str | torch.device) -> None:
+        blocks = shape[:3] + (-(-shape[3] // self.block_tokens),)
+        code = self.FORMATS[self.format][1]
         self.k = torch.zeros(shape, dtype=torch.int8, device=device).view(code)
         self.v = torch.zeros(shape, dtype=torch.int8, device=device).view(code)
         self.k_scale = torch.zeros(blocks, dtype=torch.float32, device=device)
         self.v_scale = torch.zeros(blocks, dtype=torch.float32, device=device)
-        self.max_batch = max_batch
-        self.max_len = max_len
-        self.window = 0
-        self.row_start = 0
-        self._native = None
+
+    def native(self) -> _lib.QiCache:
+        if self._native is None:
+            n = super().native()
+            n.format, n.block = self.FORMATS[self.format][0], self.block_tokens
+            n.k_scale, n.v_scale = self.k_scale.data_ptr(), self.v_scale.data_ptr()
+        return self._native
 
     def _layer(self, i: int) -> _lib.QiKvLayer:
-        return _lib.QiKvLayer(self.k[i].data_ptr(), self.v[i].data_ptr(), self.k_scale[i].data_ptr(),
-                              self.v_scale[i].data_ptr(), self.FORMATS[self.format][0], self.block_tokens,
-                              self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1], None, 0, 0, 0)
+        d = super()._layer(i)
+        d.format, d.block = self.FORMATS[self.format][0], self.block_tokens
+        d.k_scale, d.v_scale = self.k_scale[i].data_ptr(), self.v_scale[i].data_ptr()
+        return d
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor) -> None:
         """Write M tokens' keys and values into layer `layer` (qi_kv8_append): token t at
@@ -434,18 +461,47 @@ class Kv8Cache(KVCache):
         _require(self.k_scale, "values", self.k.device)
         if d.head_dim not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {d.head_dim}")
-        k = self.k_scale.new_empty(self.k.shape[1:])
+        k = self.k_scale.new_empty((self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1]))
         v = torch.empty_like(k)
         with _lib.on_device(self.k.device):
             _lib.check(_lib.lib().qi_kv8_values(C.byref(d), k.data_ptr(), v.data_ptr(),
                                                 _lib.stream_ptr(self.k.device)), "qi_kv8_values")
         return k, v
 
-    def native(self) -> _lib.QiCache:
-        raise NotImplementedError("the model's forward does not read an 8-bit cache yet")
-
     def update(self, layer: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor):
-        raise NotImplementedError("the 8-bit cache is written by append")
+        raise NotImplementedError("an 8-bit cache is written by append and by the model's forward")
+
+    def memory_bytes(self) -> int:
+        return 2 * (self.k.numel() + 4 * self.k_scale.numel())
+
+
+class Kv8Cache(_Codes, KVCache):
+    """K and V as 8-bit codes with block scales: `k`, `v` (layers, max_batch, kv_heads,
+    max_len, head_dim) int8 or float8_e4m3fn and `k_scale`, `v_scale` (layers, max_batch,
+    kv_heads, ceil(max_len / block_tokens)) fp32. The scale of a block of `block_tokens`
+    (16, 32, 64 or 128) positions of one row and head is the least power of two s with
+    127 s (int8) or 448 s (e4m3) >= all its values; the codes stand for code * s. `int8`
+    is the more exact on even-sized values (a step of at most amax / 63.5), `e4m3` keeps
+    small values next to large ones (relative steps of 2^-3).
+
+    `append` writes new tokens, `attend` reads them (KVCache.attend), `values` gives back
+    what the codes stand for; the model's forward, `generate` and `Engine(kv_format=...)`
+    use it like a bf16 cache."""
+
+    def __init__(self, cfg: Qwen2Config, max_batch: int, max_len: int,
+                 dtype: torch.dtype = torch.float16, device: str | torch.device = "cuda",
+                 format: str = "int8", block_tokens: int = 32,
+                 attn_window: int = 0, attn_sinks: int = 0) -> None:
+        if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise ValueError(f"KV cache dtype must be bfloat16, float16 or float32; got {dtype}")
+        self._format(format, block_tokens)
+        self._allocate((cfg.num_hidden_layers, max_batch, cfg.num_key_value_heads, max_len, cfg.head_dim), device)
+        self.max_batch = max_batch
+        self.max_len = max_len
+        self.window = 0
+        self.row_start = 0
+        self.attn_window, self.attn_sinks = _window(attn_window, attn_sinks)
+        self._native = None
 
     def move_rows(self, moves: list[tuple[int, int, int]]) -> None:
         """KVCache.move_rows: codes of positions [0, length) and the scales of their blocks."""
@@ -458,8 +514,29 @@ class Kv8Cache(KVCache):
             for t, n in ((self.k, length), (self.v, length), (self.k_scale, blocks), (self.v_scale, blocks)):
                 t[:, dst, :, :n] = t[:, src, :, :n]
 
-    def memory_bytes(self) -> int:
-        return 2 * (self.k.numel() + 4 * self.k_scale.numel())
+
+class PagedKv8Cache(_Codes, PagedKVCache):
+    """Kv8Cache in pages: pools of codes (layers, n_pages, kv_heads, page_size, head_dim) and
+    of scales (layers, n_pages, kv_heads, page_size / block_tokens), with PagedKVCache's
+    page table and storage management."""
+
+    def __init__(self, cfg: Qwen2Config, max_batch: int, max_len: int,
+                 dtype: torch.dtype = torch.float16, device: str | torch.device = "cuda",
+                 page_size: int = 128, n_pages: int | None = None, format: str = "int8", block_tokens: int = 32,
+                 attn_window: int = 0, attn_sinks: int = 0) -> None:
+        self._format(format, block_tokens)
+        super().__init__(cfg, max_batch, max_len, dtype, device, page_size, n_pages, attn_window, attn_sinks)
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor) -> None:
+        """Kv8Cache.append; the pages of the positions are mapped (`reserve`) by the caller and
+        table changes published first. A token without a page is recorded for `check()`."""
+        self.sync()
+        super().append(layer, k, v, rows, pos)
+
+    def values(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Kv8Cache.values by cache row and position; zeros where no page is mapped."""
+        self.sync()
+        return super().values(layer)
 
 
 def _single_layer_view(cache: KVCache, layer: int) -> tuple[torch.Tensor, torch.Tensor]:

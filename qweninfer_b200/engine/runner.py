@@ -17,7 +17,8 @@ import numpy as np
 import torch
 
 from qweninfer_b200 import _lib
-from qweninfer_b200.engine.kv_cache import KVCache, PagedKVCache
+from qweninfer_b200.engine.kv_cache import Kv8Cache, KVCache, PagedKv8Cache, PagedKVCache
+from qweninfer_b200.models.logprobs import MAX_TOP, TokenInfo, TokenLogprobs, token_logprobs
 
 
 class _Staging:
@@ -45,7 +46,10 @@ class _Staging:
 class DecodeRunner:
     """Prefill and decode of one model over one KV cache (see the module docstring)."""
 
-    def __init__(self, model, cache: KVCache, max_batch: int, cuda_graphs: bool = True) -> None:
+    def __init__(self, model, cache: KVCache, max_batch: int, cuda_graphs: bool = True,
+                 logprobs: int | None = None) -> None:
+        """`logprobs`: with each step also the tokens' log probabilities, entropies and this
+        many alternatives (0..32), in `last_logprobs`."""
         self.model = model
         self.cache = cache
         self.dev = model.device
@@ -68,9 +72,18 @@ class DecodeRunner:
         self.launches = 0
         self.h2d_bytes = 0
         self.d2h_bytes = 0
-        self.kernels_per_forward = lambda M: 1 + 5 * model.cfg.num_hidden_layers + 1
+        per_layer = 5 + isinstance(cache, (Kv8Cache, PagedKv8Cache))
+        self.kernels_per_forward = lambda M: 1 + per_layer * model.cfg.num_hidden_layers + 1 + (logprobs is not None)
         # a paged cache maps pages before each forward; packed rows need nothing
         self.paged = isinstance(cache, PagedKVCache)
+        if logprobs is not None and not 0 <= logprobs <= MAX_TOP:
+            raise ValueError(f"logprobs must be 0..{MAX_TOP}, got {logprobs}")
+        self.logprobs = logprobs
+        self.last_logprobs: list[TokenInfo] | None = None
+        self._lp: TokenLogprobs | None = None              # of the forward just enqueued
+        self._graph_lp: dict[int, TokenLogprobs] = {}      # of each graph's replays
+        if logprobs is not None:
+            self.logits = torch.empty(max_batch, model.cfg.vocab_size, dtype=torch.float32, device=self.dev)
 
     # ------------------------------------------------------------ helpers
 
@@ -80,16 +93,30 @@ class DecodeRunner:
         self.launches += self.kernels_per_forward(M)
         _lib.check(_lib.lib().qi_forward(
             C.byref(self.model.native()), C.byref(self.cache.native()), C.byref(ws.struct),
-            st.ptr(0), st.ptr(1), st.ptr(2), M, head_lo, 1, n_head, None, 0, 0,
+            st.ptr(0), st.ptr(1), st.ptr(2), M, head_lo, 1, n_head,
+            None if self.logprobs is None else self.logits.data_ptr(), 0,
+            0 if self.logprobs is None else self.logits.shape[1],
             self.d_slots.data_ptr(), _lib.stream_ptr(self.dev)), "qi_forward")
+        if self.logprobs is not None:
+            # the greedy token is the first alternative
+            self._lp = token_logprobs(self.logits[:n_head], None, max(1, self.logprobs))
 
     def _read(self, k: int) -> np.ndarray:
         self.d2h_bytes += 8 * k
         self.h_slots[:k].copy_(self.d_slots[:k], non_blocking=True)
+        lp = self._lp
+        if lp is not None:
+            host = [t[:k].to("cpu", non_blocking=True) for t in (lp.entropy, lp.top_ids, lp.top_logprobs)]
+            self.d2h_bytes += sum(t.numel() * 4 for t in host)
         self.done.record()
         self.done.synchronize()
         s = self.h_slots_np[:k]
-        return (0xFFFFFFFF - (s & 0xFFFFFFFF)).astype(np.int64)
+        toks = (0xFFFFFFFF - (s & 0xFFFFFFFF)).astype(np.int64)
+        if lp is not None:
+            ent, ids, lps = (t.tolist() for t in host)
+            self.last_logprobs = [TokenInfo(int(toks[i]), lps[i][0], ent[i], list(zip(ids[i], lps[i]))[:self.logprobs])
+                                  for i in range(k)]
+        return toks
 
     def _check_ids(self, ids) -> None:
         a = np.asarray(ids)
@@ -137,6 +164,7 @@ class DecodeRunner:
             for row, p in zip(rows, prompts):
                 self.cache.reserve(row, len(p))
         out: list[int] = []
+        infos: list[TokenInfo] = []
         i = 0
         while i < len(prompts):
             j, tot = i, 0
@@ -154,7 +182,10 @@ class DecodeRunner:
             ws = self.model.workspace(cap, cap).plan(M, max(len(p) for p in chunk))
             self._forward(self.pre, M, ws, M - n, n)
             out += [int(t) for t in self._read(n)]
+            infos += self.last_logprobs or []
             i = j
+        if self.logprobs is not None:
+            self.last_logprobs = infos
         return out
 
     @torch.inference_mode()
@@ -171,6 +202,7 @@ class DecodeRunner:
         self._check_ids(toks)
         if self.paged:
             for b, q in enumerate(pos):
+                self.cache.trim(row_start + b, int(q))
                 self.cache.reserve(row_start + b, int(q) + 1)
             # page-table changes go out before the step, graph replays included (nothing is
             # left to copy when a graph is captured, so no copy is recorded into it)
@@ -180,14 +212,18 @@ class DecodeRunner:
         g = self.graphs.get(B)
         if g is not None:
             g.replay()
+            self._lp = self._graph_lp.get(B)
         else:
             self.ws.plan(B, 1)  # one token per row: a decode step
             self._forward(self.dec, B, self.ws, 0, B)
             if self.cuda_graphs:
+                lp = self._lp
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g):
                     self._forward(self.dec, B, self.ws, 0, B)
                 self.graphs[B] = g
+                if lp is not None:
+                    self._graph_lp[B], self._lp = self._lp, lp
         self.steps += 1
         return self._read(B)
 

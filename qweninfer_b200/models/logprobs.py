@@ -26,6 +26,16 @@ class TokenLogprobs:
     top_logprobs: torch.Tensor | None
 
 
+@dataclass
+class TokenInfo:
+    """A generated token: its log probability, the entropy of the distribution it was taken
+    from, and the best alternatives as (id, log probability), itself first (greedy)."""
+    token: int
+    logprob: float
+    entropy: float
+    top: list[tuple[int, float]]
+
+
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0) -> TokenLogprobs:
     """Per row of `logits` (M, V) (float32, bfloat16 or float16; rows may be strided):
     log softmax at targets[t], the entropy of the distribution, and its `top` (0..32, at

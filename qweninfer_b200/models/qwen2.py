@@ -361,6 +361,8 @@ class Workspace:
         self.act_attn = torch.zeros(pad * HIDDEN * 2, **bf)
         self.act_h = torch.zeros(pad * INTER * 2, **bf)
         self.ss = torch.zeros(7 * pad, **f32)
+        # keys and values on their way into an 8-bit cache
+        self.kv_stage = torch.empty(max_tokens * 4 * HEAD_DIM, **f32)
         sms = torch.cuda.get_device_properties(device).multi_processor_count
         self.tc_scratch = torch.empty(sms * 2 * 128 * nt, **f32)
         n_counters = max(76 * -(-pad // 8), -(-vocab // 128), 64)  # any token tile down to 8
@@ -370,7 +372,7 @@ class Workspace:
             self.attn_part.data_ptr(), self.attn_counters.data_ptr(), max_tokens, 1, 128, self.err.data_ptr(),
             int(use_tensor_cores()), self.act_x.data_ptr(), self.act_attn.data_ptr(), self.act_h.data_ptr(),
             self.ss.data_ptr(), pad, self.tc_scratch.data_ptr(), self.tc_scratch.numel(),
-            self.tc_counters.data_ptr(), n_counters, 0)
+            self.tc_counters.data_ptr(), n_counters, 0, self.kv_stage.data_ptr())
 
     def plan(self, M: int, query_run: int = 0) -> "Workspace":
         """Attention splits for M query tokens; `query_run`: the longest prompt among them
@@ -543,6 +545,35 @@ class Qwen2(nn.Module):
             "qi_forward")
         self.last_argmax = self.decode_argmax(slots[:n_head])
         return logits.view(B, 1 if last_only else S, self.cfg.vocab_size).to(want)
+
+    def score(self, input_ids: torch.Tensor, top: int = 0, cache=None, chunk: int = 512):
+        """Log probabilities of a text under the model: for input_ids (B, S), `TokenLogprobs`
+        (models/logprobs.py) of shape (B, S - 1[, top]): entry [b, i] is of token i + 1 after
+        tokens 0..i. The text runs `chunk` tokens at a time through `cache` (a new bf16 cache
+        if None; pass an 8-bit or windowed one to see what it costs), so that logits take
+        B x chunk rows of memory. The reference has no counterpart: its callers take the
+        argmax (qweninfer/engine/generate.py:33-36)."""
+        from qweninfer_b200.engine.kv_cache import KVCache
+        from qweninfer_b200.models.logprobs import TokenLogprobs, token_logprobs
+        B, S = input_ids.shape
+        if S < 2:
+            raise ValueError("a text of at least 2 tokens has log probabilities")
+        if chunk < 1:
+            raise ValueError(f"chunk must be positive, got {chunk}")
+        if input_ids.device.type == "cpu" and (int(input_ids.min()) < 0 or int(input_ids.max()) >= self.cfg.vocab_size):
+            raise IndexError("token id outside the vocabulary")
+        if cache is None:
+            cache = KVCache(self.cfg, B, S - 1, dtype=torch.bfloat16, device=self.device)
+        ids = input_ids.to(self.device)
+        parts = []
+        for lo in range(0, S - 1, chunk):
+            hi = min(S - 1, lo + chunk)
+            logits = self.forward(input_ids[:, lo:hi], positions=torch.arange(lo, hi), cache=cache,
+                                  logits_dtype=torch.float32)
+            r = token_logprobs(logits.reshape(B * (hi - lo), -1), ids[:, lo + 1:hi + 1].reshape(-1), top)
+            parts.append([t if t is None else t.view(B, hi - lo, *t.shape[1:])
+                          for t in (r.logprob, r.entropy, r.top_ids, r.top_logprobs)])
+        return TokenLogprobs(*(None if p[0] is None else torch.cat(p, 1) for p in zip(*parts)))
 
     @torch.inference_mode()
     def residual_stream(self, input_ids: torch.Tensor, n_layers: int, positions: torch.Tensor | None = None,
