@@ -121,9 +121,10 @@ def load_library(path: Path = LIB_PATH) -> C.CDLL:
 
 def lib() -> C.CDLL:
     global _lib
-    with _lock:
-        if _lib is None:
-            _lib = load_library()
+    if _lib is None:
+        with _lock:
+            if _lib is None:
+                _lib = load_library()
     return _lib
 
 
@@ -180,6 +181,12 @@ class on_device:
         if self.other is not None:
             self.other.__exit__(*exc)
             _current[0] = -1
+
+
+def ready(idx: int) -> bool:
+    """Whether a call for device `idx` needs no `on_device`: the process sees one device, which
+    is set up and current (1 us less than entering the context)."""
+    return idx in _inited and torch._C._cuda_getDevice() == idx and torch.cuda.device_count() == 1
 
 
 class _Scratch:

@@ -178,16 +178,25 @@ class KVCache:
             raise ValueError("out must not share q's storage")
         if M == 0:
             return out
-        d, st, sh, dtype, heads, window, sinks, query_run, part_floats, n_counters = plan
-        with _lib.on_device(dev):
-            stream = torch._C._cuda_getCurrentRawStream(dev.index)
-            part, counters, _keep = _lib.scratch(dev, stream, 4 * part_floats, n_counters) if n_counters else (0, 0, None)
-            code = _lib.lib().qi_cache_attention(
-                d, q.data_ptr(), st, sh, dtype, heads, rows.data_ptr(), pos.data_ptr(), M, window, sinks, query_run,
-                out.data_ptr(), part, part_floats, counters, n_counters, self._errors().data_ptr(), stream)
+        if _lib.ready(dev.index):
+            code = self._attend(plan, q, rows, pos, out)
+        else:
+            with _lib.on_device(dev):
+                code = self._attend(plan, q, rows, pos, out)
         if code:
             _lib.check(code, "qi_cache_attention")
         return out
+
+    def _attend(self, plan: tuple, q: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor, out: torch.Tensor) -> int:
+        d, st, sh, dtype, heads, window, sinks, query_run, part_floats, n_counters = plan
+        dev = q.device
+        stream = torch._C._cuda_getCurrentRawStream(dev.index)
+        part = counters = 0
+        if n_counters:
+            part, counters, _keep = _lib.scratch(dev, stream, 4 * part_floats, n_counters)
+        return _lib.lib().qi_cache_attention(
+            d, q.data_ptr(), st, sh, dtype, heads, rows.data_ptr(), pos.data_ptr(), q.shape[0], window, sinks,
+            query_run, out.data_ptr(), part, part_floats, counters, n_counters, self._errors().data_ptr(), stream)
 
     def _attend_plan(self, layer: int, q: torch.Tensor, window: int, sinks: int, query_run: int) -> tuple:
         """The arguments of an `attend` call that its shapes decide, checked, and its scratch."""
@@ -446,11 +455,13 @@ class _Codes:
         rows, pos = self._tokens(M, rows, pos)
         if M == 0:
             return
-        with _lib.on_device(dev):
-            code = _lib.lib().qi_kv8_append(
-                d, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                _lib.DTYPES[k.dtype], rows.data_ptr(), pos.data_ptr(), M, self._errors().data_ptr(),
-                torch._C._cuda_getCurrentRawStream(dev.index))
+        args = (d, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                _lib.DTYPES[k.dtype], rows.data_ptr(), pos.data_ptr(), M, self._errors().data_ptr())
+        if _lib.ready(dev.index):
+            code = _lib.lib().qi_kv8_append(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        else:
+            with _lib.on_device(dev):
+                code = _lib.lib().qi_kv8_append(*args, torch._C._cuda_getCurrentRawStream(dev.index))
         if code:
             _lib.check(code, "qi_kv8_append")
 
@@ -458,14 +469,19 @@ class _Codes:
         """What layer `layer` stands for: K and V (max_batch, kv_heads, max_len, head_dim)
         fp32 (qi_kv8_values). Dead positions give whatever their codes say."""
         d = self.layer(layer)
-        _require(self.k_scale, "values", self.k.device)
+        dev = self.k.device
+        if dev.type != "cuda":
+            _require(self.k_scale, "values", dev)
         if d.head_dim not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {d.head_dim}")
-        k = self.k_scale.new_empty((self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1]))
-        v = torch.empty_like(k)
-        with _lib.on_device(self.k.device):
-            _lib.check(_lib.lib().qi_kv8_values(C.byref(d), k.data_ptr(), v.data_ptr(),
-                                                _lib.stream_ptr(self.k.device)), "qi_kv8_values")
+        k, v = self.k_scale.new_empty((2, self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1])).unbind(0)
+        if _lib.ready(dev.index):
+            code = _lib.lib().qi_kv8_values(C.byref(d), k.data_ptr(), v.data_ptr(), _lib.stream_ptr(dev))
+        else:
+            with _lib.on_device(dev):
+                code = _lib.lib().qi_kv8_values(C.byref(d), k.data_ptr(), v.data_ptr(), _lib.stream_ptr(dev))
+        if code:
+            _lib.check(code, "qi_kv8_values")
         return k, v
 
     def update(self, layer: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor):

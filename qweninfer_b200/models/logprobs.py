@@ -55,7 +55,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
         _plans[key] = plan
     M, V, dtype, ld, nbytes = plan
     dev = logits.device
-    if targets is not None and not (targets.shape == (M,) and targets.dtype in _INTS and targets.device == dev
+    if targets is not None and not (targets.dtype in _INTS and targets.device == dev and targets.shape == (M,)
                                     and targets.is_contiguous()):
         targets = _targets(targets, M, V, dev)
     # the outputs share one allocation
@@ -68,17 +68,24 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
         r = TokenLogprobs(lp if targets is not None else None, ent, None, None)
     if M == 0:
         return r
-    base = buf.data_ptr()
-    with _lib.on_device(dev):
-        stream = _lib.stream_ptr(dev)
-        data, counters, _keep = _lib.scratch(dev, stream, nbytes, _lib.LOGPROBS_COUNTERS)
-        code = _lib.lib().qi_token_logprobs(
-            logits.data_ptr(), dtype, ld, None if targets is None else targets.data_ptr(),
-            targets is not None and targets.dtype == torch.int64, M, V, top, None if targets is None else base,
-            base + 4 * M, base + 8 * M, base + 8 * M + 4 * M * top, data, nbytes, counters, stream)
+    if _lib.ready(dev.index):
+        code = _call(logits, plan, targets, top, buf.data_ptr())
+    else:
+        with _lib.on_device(dev):
+            code = _call(logits, plan, targets, top, buf.data_ptr())
     if code:
         _lib.check(code, "qi_token_logprobs")
     return r
+
+
+def _call(logits: torch.Tensor, plan: tuple, targets: torch.Tensor | None, top: int, out: int) -> int:
+    M, V, dtype, ld, nbytes = plan
+    dev = logits.device
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    data, counters, _keep = _lib.scratch(dev, stream, nbytes, _lib.LOGPROBS_COUNTERS)
+    y, wide = (None, 0) if targets is None else (targets.data_ptr(), targets.dtype is torch.int64)
+    return _lib.lib().qi_token_logprobs(logits.data_ptr(), dtype, ld, y, wide, M, V, top, y and out, out + 4 * M,
+                                        out + 8 * M, out + 8 * M + 4 * M * top, data, nbytes, counters, stream)
 
 
 _INTS = (torch.int32, torch.int64)
