@@ -156,10 +156,14 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D>::kCtas) cache_attentio
     }
     return leave();
   }
-  if (p.only_single) {  // the tokens that the prompt kernel left out
-    const int n = kPromptRows / G, t = tok / n * n + tid;
-    const bool same = tid < n && t < p.M && p.rows[t] == row && token_ok(p, p.pos[t], row);
-    if (__syncthreads_count(same) != 1) return leave();
+  if (p.only_single) {  // the tokens that the prompt kernel left out: alone in their row of a CTA's
+    const int n = (D == 64 ? 2 : 1) * (kPromptRows / G), t0 = tok / n * n;
+    int same = 0;
+    for (int j = 0; j < n; j += kThreads) {
+      const int t = t0 + j + tid;
+      same += __syncthreads_count(j + tid < n && t < p.M && p.rows[t] == row && token_ok(p, p.pos[t], row));
+    }
+    if (same != 1) return leave();
   }
   const Seen<kGran> seen = seen_range<kGran>(ps, window_start(ps, p.window), p.sinks);
   const int nsplit = min(p.splits, (seen.n + kMinSplit - 1) / kMinSplit);

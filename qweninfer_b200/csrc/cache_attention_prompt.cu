@@ -72,8 +72,8 @@ struct Shape {
   static constexpr uint32_t kQ = kRows * D * 2;   // one part of a tile's Q
   static constexpr uint32_t kT = kKeys * D * 2;   // K or V tile, two stages each
   static constexpr uint32_t kOffK = kTiles * PARTS * kQ, kOffV = kOffK + 2 * kT, kOffMisc = kOffV + 2 * kT;
-  // TMEM columns: S of the tiles (P in its place), then T
-  static constexpr uint32_t kColT = kTiles * 128, kCols = kTiles == 2 ? 512 : 256;
+  // TMEM columns: three S (each with its P in its place) that the tiles take in turn, then T
+  static constexpr uint32_t kColT = 3 * 128, kCols = 512;
   static_assert(kColT + kTiles * D <= kCols, "tensor memory");
   // Registers of a thread: of the launch, and of the warpgroups, which together have no more.
   static constexpr int kRegLaunch = D == 64 ? 80 : 128;
@@ -89,16 +89,17 @@ struct Seg {
 };
 
 struct Misc {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], t_full[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[3], p_full[3], t_full[2], done;
   uint32_t tmem;
   int nseg, ntiles;
   int abort;  // a wait of this CTA gave up: the others do not wait any more
   int pos[kMaxTok], row[kMaxTok], seg[kMaxTok];  // per token
   Seg segs[kMaxTok];
+  Seg one;  // of tokens that all have one cache row (first: how many)
   // of 16 keys, by stage: K scale, exponent and significand of the V scale (s = 2^e * f; a
   // scale that is not finite has f = NaN)
   float ks[2][8], ve[2][8], vf[2][8];
-  float2 pair[2][2 * kRows];  // what the two threads of a row tell each other
+  float2 pair[2][2][2 * kRows];  // what the two threads of a row tell each other, by turns
   float2 ml[2 * kRows];       // maximum and sum of the rows' partials
 };
 constexpr uint32_t kMiscBytes = (sizeof(Misc) + 15) / 16 * 16;
@@ -340,11 +341,15 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       mbar_init(&X.v_full[s], H::kLoadWarps);
       mbar_init(&X.k_empty[s], 1);
       mbar_init(&X.v_empty[s], 1);
-      mbar_init(&X.s_full[s], 1);
-      mbar_init(&X.p_full[s], 8);
       mbar_init(&X.t_full[s], 1);
     }
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(&X.s_full[s], 1);
+      mbar_init(&X.p_full[s], 8);
+    }
+    mbar_init(&X.done, 1);
     X.abort = 0;
+    X.one = Seg{0, 0x7fffffff, -1, 0, 0};
     fence_barrier_init();
   }
   if (tid < kMaxTok) {
@@ -360,41 +365,60 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
     X.row[tid] = rw;
   }
   __syncthreads();
-  // segments: the first token of each cache row gathers what its tokens see
-  if (tid < ntok) {
-    int first = -1;
-    Seg s = {0, 0x7fffffff, -1, 0, 0};
-    if (X.pos[tid] >= 0) {
-      int n = 0;
-      for (int i = 0; i < ntok; ++i) {
-        if (X.pos[i] < 0 || X.row[i] != X.row[tid]) continue;
-        if (first < 0) first = i;
-        if (first != tid) break;
-        const int ps = X.pos[i], lo = window_start(ps, p.window);
-        ++n;
-        s.lo = min(s.lo, lo);
-        s.hi = max(s.hi, ps);
-        s.sinks = max(s.sinks, min(p.sinks, lo));
+  // The tokens' segments. Mostly there is one: all of one cache row.
+  const bool valid = tid < ntok && X.pos[tid] >= 0;
+  if (!__syncthreads_or(valid && X.row[tid] != X.row[0])) {
+    if (valid) {
+      const int ps = X.pos[tid], lo = window_start(ps, p.window);
+      atomicMin(&X.one.lo, lo);
+      atomicMax(&X.one.hi, ps);
+      atomicMax(&X.one.sinks, min(p.sinks, lo));
+      atomicAdd(&X.one.first, 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      const int tokens = X.one.first;
+      X.segs[0] = Seg{X.row[0], X.one.lo, X.one.hi, X.one.sinks, 0};
+      X.nseg = tokens > (p.skip_single ? 1 : 0);  // a single token is left to the per-token kernel
+      X.ntiles = X.nseg ? seen_range<kKeys>(X.one.hi, X.one.lo, X.one.sinks).n : 0;
+    }
+  } else {
+    // the first token of each cache row gathers what its tokens see
+    if (tid < ntok) {
+      int first = -1;
+      Seg s = {0, 0x7fffffff, -1, 0, 0};
+      if (X.pos[tid] >= 0) {
+        int n = 0;
+        for (int i = 0; i < ntok; ++i) {
+          if (X.pos[i] < 0 || X.row[i] != X.row[tid]) continue;
+          if (first < 0) first = i;
+          if (first != tid) break;
+          const int ps = X.pos[i], lo = window_start(ps, p.window);
+          ++n;
+          s.lo = min(s.lo, lo);
+          s.hi = max(s.hi, ps);
+          s.sinks = max(s.sinks, min(p.sinks, lo));
+        }
+        s.row = X.row[tid];
+        if (p.skip_single && first == tid && n == 1) s.hi = -1;  // left to the per-token kernel
       }
-      s.row = X.row[tid];
-      if (p.skip_single && first == tid && n == 1) s.hi = -1;  // left to the per-token kernel
+      X.seg[tid] = first;
+      X.segs[tid] = s;
     }
-    X.seg[tid] = first;
-    X.segs[tid] = s;
-  }
-  __syncthreads();
-  if (tid == 0) {  // the list of key tiles: segment after segment
-    int n = 0, t = 0;
-    for (int i = 0; i < ntok; ++i) {
-      if (X.seg[i] != i || X.segs[i].hi < 0) continue;
-      Seg s = X.segs[i];
-      s.first = t;
-      t += seen_range<kKeys>(s.hi, s.lo, s.sinks).n;
-      // compacted in place: the segments before it are at places up to i
-      X.segs[n++] = s;
+    __syncthreads();
+    if (tid == 0) {  // the list of key tiles: segment after segment
+      int n = 0, t = 0;
+      for (int i = 0; i < ntok; ++i) {
+        if (X.seg[i] != i || X.segs[i].hi < 0) continue;
+        Seg s = X.segs[i];
+        s.first = t;
+        t += seen_range<kKeys>(s.hi, s.lo, s.sinks).n;
+        // compacted in place: the segments before it are at places up to i
+        X.segs[n++] = s;
+      }
+      X.nseg = n;
+      X.ntiles = t;
     }
-    X.nseg = n;
-    X.ntiles = t;
   }
   tc_fence_before();
   __syncthreads();
@@ -412,50 +436,50 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       asm volatile("bar.sync 1, %0;" ::"n"(32 * (H::kSoftWarps + 1)) : "memory");  // Q is in place
       const uint32_t sb = smem_u32(smem), lead = lane == 0;
       const uint32_t id_s = idesc_f16(false, kKeys), id_t = idesc_f16(true, D);
-      // S(i) of tile t; it takes the place of P(i - 1), whose product was issued before
-      auto scores = [&](int i, int t) {
+      // Products of the key tiles i, of each for the query tiles t: number x = i ntl + t. S of x
+      // goes to buffer x % 3, where S of x - 3 was, whose P the product T of x - 3, issued
+      // before, has read. Scores run `ahead` products before T, so that those of a tile's next
+      // keys are ready when it is done with these; with one query tile only 2, since its third
+      // would wait for keys whose stage the first T has to free.
+      const int lg = ntl - 1, total = n << lg;
+      auto scores = [&](int x, int buf) {
+        const int i = x >> lg, t = x & lg;
+        wait(&X.k_full[i & 1], (uint32_t)(i >> 1) & 1u, X, p.err);
+        tc_fence_after();
         const uint64_t qd = desc(sb + t * PARTS * H::kQ, 128, D * 16);
         const uint64_t kd = desc(sb + H::kOffK + (i & 1) * H::kT, 128, D * 16);
 #pragma unroll
         for (int q = PARTS - 1; q >= 0; --q)
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma_ss(lead, tmem + 128 * t, qd + (uint64_t)(q * (H::kQ >> 4) + k * 16), kd + (uint64_t)(k * 16), id_s,
+            umma_ss(lead, tmem + 128 * buf, qd + (uint64_t)(q * (H::kQ >> 4) + k * 16), kd + (uint64_t)(k * 16), id_s,
                     q < PARTS - 1 || k > 0 ? 1u : 0u);
-        commit(lead, &X.s_full[t]);
-        if (t == ntl - 1) commit(lead, &X.k_empty[i & 1]);
+        commit(lead, &X.s_full[buf]);
+        if (t == lg) commit(lead, &X.k_empty[i & 1]);
       };
-      if (n > 0) {
-        wait(&X.k_full[0], 0u, X, p.err);
+      const int ahead = 2 + lg;
+      for (int x = 0; x < min(ahead, total); ++x) scores(x, x);
+      int buf = 0;
+      uint32_t ph = 0u;
+      for (int x = 0; x < total; ++x) {
+        const int i = x >> lg, t = x & lg, st = i & 1;
+        wait(&X.v_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);
+        wait(&X.p_full[buf], ph, X, p.err);
         tc_fence_after();
-        for (int t = 0; t < ntl; ++t) scores(0, t);
-      }
-      for (int i = 0; i < n; ++i) {
-        const int st = i & 1;
-        for (int t = 0; t < ntl; ++t) {
-          if (t == 0) wait(&X.v_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);
-          wait(&X.p_full[t], (uint32_t)i & 1u, X, p.err);
-          tc_fence_after();
-          const uint64_t vd = desc(sb + H::kOffV + st * H::kT, D * 16, 128);
+        const uint64_t vd = desc(sb + H::kOffV + st * H::kT, D * 16, 128);
 #pragma unroll
-          for (int q = PARTS - 1; q >= 0; --q)
+        for (int q = PARTS - 1; q >= 0; --q)
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              // 16 keys: 8 columns of P for each part; 2 key groups of V
-              umma_ts(lead, tmem + H::kColT + D * t, tmem + 128 * t + 16 * k + 8 * q, vd + (uint64_t)(k * 2 * D), id_t,
-                      q < PARTS - 1 || k > 0 ? 1u : 0u);
-          if (t == ntl - 1) commit(lead, &X.v_empty[st]);
-          if (i + 1 < n) {
-            if (t == 0) {
-              wait(&X.k_full[st ^ 1], (uint32_t)((i + 1) >> 1) & 1u, X, p.err);
-              tc_fence_after();
-            }
-            scores(i + 1, t);
-          } else {
-            commit(lead, &X.t_full[t]);
-          }
-        }
+          for (int k = 0; k < kKeys / 16; ++k)
+            // 16 keys: 8 columns of P for each part; 2 key groups of V
+            umma_ts(lead, tmem + H::kColT + D * t, tmem + 128 * buf + 16 * k + 8 * q, vd + (uint64_t)(k * 2 * D), id_t,
+                    q < PARTS - 1 || k > 0 ? 1u : 0u);
+        commit(lead, &X.t_full[t]);
+        if (t == lg) commit(lead, &X.v_empty[st]);
+        if (x + ahead < total) scores(x + ahead, buf + ahead >= 3 ? buf + ahead - 3 : buf + ahead);
+        if (++buf == 3) buf = 0, ph ^= 1u;
       }
+      commit(lead, &X.done);
       __syncwarp();
     }
     __syncthreads();
@@ -589,7 +613,8 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       const uint32_t ph = (uint32_t)((i >> 1) - 1) & 1u;
       uint8_t* kt = smem + H::kOffK + st * H::kT;
       uint8_t* vt = smem + H::kOffV + st * H::kT;
-      if (i >= 2) {  // tile i - 2 is done with: its products, and its scales
+      // tile i - 2 is done with: its products, and its scales (all of them after the last T)
+      if (i >= 2) {
         wait(&X.k_empty[st], ph, X, p.err);
         wait(&X.v_empty[st], ph, X, p.err);
       }
@@ -633,9 +658,9 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         const float2 x = row_pair<PARTS == 2>(raw, i, p.dtype);
         am = fmaxf(am, fmaxf(fabsf(x.x), fabsf(x.y)));
       }
-      X.pair[hf][rr].x = am;
+      X.pair[1][hf][rr].x = am;
       pair_bar();
-      am = fmaxf(am, X.pair[hf ^ 1][rr].x);
+      am = fmaxf(am, X.pair[1][hf ^ 1][rr].x);
       float inv = live ? 1.f : 0.f;
       const uint32_t e = __float_as_uint(am) >> 23;
       if (live && e > 0 && e < 253) {
@@ -660,7 +685,6 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
     asm volatile("bar.sync 1, %0;" ::"n"(32 * (H::kSoftWarps + 1)) : "memory");
     const Seen<kKeys> mine = seen_range<kKeys>(live ? ps : 0, live ? window_start(ps, p.window) : 0, p.sinks);
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t srow = trow + 128 * qt + 64 * hf;          // this half's scores
     const uint32_t orow = trow + H::kColT + D * qt + DH * hf;  // and dims
 
     float m = -INFINITY, l = 0.f;  // maximum of the scores (log2 units), sum of 2^(x - m)
@@ -684,6 +708,8 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
     };
     int si = 0;
     const int n_mine = qt < ntl ? n : 0;
+    int buf = qt;  // S of the tile at hand, and its phase
+    uint32_t sph = 0u;
     for (int i = 0; i < n_mine; ++i) {
       const int at = tbeg + i, st = i & 1;
       while (si + 1 < X.nseg && at >= X.segs[si + 1].first) ++si;
@@ -704,9 +730,9 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       float ks[4], ve[4];  // of this half's 4 blocks
 #pragma unroll
       for (int c = 0; c < 4; ++c) ks[c] = qs * X.ks[st][4 * hf + c], ve[c] = X.ve[st][4 * hf + c];
-      wait(&X.s_full[qt], (uint32_t)i & 1u, X, p.err);  // S(i), and T(i - 1) before it
+      wait(&X.s_full[buf], sph, X, p.err);
       tc_fence_after();
-      if (i > 0) add_tile();
+      const uint32_t srow = trow + 128 * buf + 64 * hf;  // this half's scores
       // pass 1: the maxima of the scores and of score + log2(V scale)
       float mx = -INFINITY, R = -INFINITY;
       auto maxima = [&](auto some_masked) {
@@ -728,11 +754,16 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       };
       if (masked) maxima(True{});
       else maxima(False{});
-      X.pair[hf][rr] = make_float2(mx, R);
-      pair_bar();  // (the next tile's values are written after both halves' weights of this one)
-      const float2 other = X.pair[hf ^ 1][rr];
+      X.pair[st][hf][rr] = make_float2(mx, R);
+      pair_bar();
+      const float2 other = X.pair[st][hf ^ 1][rr];
       R = fmaxf(R, other.y);
       const float mn = fmaxf(m, fmaxf(mx, other.x));
+      if (i > 0) {  // T of the tile before, with its factors
+        wait(&X.t_full[qt], (uint32_t)(i - 1) & 1u, X, p.err);
+        tc_fence_after();
+        add_tile();
+      }
       oa = m == -INFINITY ? 1.f : ex2(m - mn);  // nothing summed yet: nothing to rescale
       l *= oa;
       m = mn;
@@ -780,10 +811,12 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&X.p_full[qt]);
+      if (lane == 0) mbar_arrive(&X.p_full[buf]);
+      buf += ntl;
+      if (buf >= 3) buf -= 3, sph ^= 1u;
     }
     if (n_mine > 0) {
-      wait(&X.t_full[qt], 0u, X, p.err);
+      wait(&X.t_full[qt], (uint32_t)(n - 1) & 1u, X, p.err);
       tc_fence_after();
       add_tile();
     }
@@ -803,9 +836,9 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       for (int d = 0; d < DH; ++d) bad |= !(fabsf(of[d]) <= 3.402823466e38f);
     }
     pair_bar();
-    X.pair[hf][rr] = make_float2(l, bad ? 1.f : 0.f);
+    X.pair[0][hf][rr] = make_float2(l, bad ? 1.f : 0.f);
     pair_bar();
-    const float2 other = X.pair[hf ^ 1][rr];
+    const float2 other = X.pair[0][hf ^ 1][rr];
     l = hf ? other.x + l : l + other.x;
     if constexpr (BF) {
       if (row_in && live && (bad || other.y != 0.f)) {
@@ -816,8 +849,7 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
     }
     // The split's partial (relative to m) into shared memory, in the place of Q and K, which
     // all products are done with: rows of D + 4 floats, so that rows 8 apart share a bank.
-    if (n > 0)
-      for (int t = 0; t < ntl; ++t) wait(&X.t_full[t], 0u, X, p.err);
+    wait(&X.done, 0u, X, p.err);
     float* po = reinterpret_cast<float*>(smem) + rr * kPitch + hf * DH;
 #pragma unroll
     for (int d = 0; d < DH; d += 4) *reinterpret_cast<float4*>(po + d) = make_float4(of[d], of[d + 1], of[d + 2], of[d + 3]);
