@@ -77,7 +77,8 @@ struct Shape {
   static_assert(kColT + kTiles * D <= kCols, "tensor memory");
   // Registers of a thread: of the launch, and of the warpgroups, which together have no more.
   static constexpr int kRegLaunch = D == 64 ? 80 : 128;
-  static constexpr int kRegSoft = D == 64 ? 88 : 152, kRegLoad = D == 64 ? 88 : 160, kRegMma = D == 64 ? 40 : 48;
+  static constexpr int kRegSoft = D == 64 ? (FMT == QI_KV_BF16 ? 88 : 96) : 152;
+  static constexpr int kRegLoad = D == 64 ? (FMT == QI_KV_BF16 ? 88 : 56) : 160, kRegMma = D == 64 ? 40 : 48;
   static_assert(2 * kTiles * kRegSoft + kRegLoad + kRegMma <= (2 * kTiles + 2) * kRegLaunch, "the increase must be covered");
 };
 
@@ -99,6 +100,7 @@ struct Misc {
   // of 16 keys, by stage: K scale, exponent and significand of the V scale (s = 2^e * f; a
   // scale that is not finite has f = NaN)
   float ks[2][8], ve[2][8], vf[2][8];
+  int k0[2], sg[2];  // first position and segment of the stage's keys
   float2 pair[2][2][2 * kRows];  // what the two threads of a row tell each other, by turns
   float2 ml[2 * kRows];       // maximum and sum of the rows' partials
 };
@@ -498,12 +500,13 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
     };
     uint4 kr[kN], vr[BF ? 1 : kN];  // bf16: V follows K in the same registers
     float sc = 1.f;
-    int si = 0;  // segment of the tile at hand (entries come in order)
+    int si = 0, first_key = 0;  // segment of the tile at hand (entries come in order), its first key
     auto fetch = [&](int i, bool k_side) {
       while (si + 1 < X.nseg && i >= X.segs[si + 1].first) ++si;
       const Seg& sg = X.segs[si];
       const Seen<kKeys> list = seen_range<kKeys>(sg.hi, sg.lo, sg.sinks);
       const int k0 = list.granule(i - sg.first) * kKeys;
+      first_key = k0;
       const long long o = layer_offset(c, D, sg.row, g, k0);
       if (o < 0 && lt == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
       const long long base = (o < 0 ? 0 : o) * (BF ? 2 : 1);
@@ -618,6 +621,7 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         wait(&X.k_empty[st], ph, X, p.err);
         wait(&X.v_empty[st], ph, X, p.err);
       }
+      if (lt == 0) X.k0[st] = first_key, X.sg[st] = si;
       if constexpr (BF) {
         store16(kr, kt, st, true);
         publish(&X.k_full[st]);
@@ -706,17 +710,15 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
           o[8 * c + j] = fma2(pack2(__uint_as_float(t[2 * j]), __uint_as_float(t[2 * j + 1])), f, o[8 * c + j]);
       });
     };
-    int si = 0;
     const int n_mine = qt < ntl ? n : 0;
     int buf = qt;  // S of the tile at hand, and its phase
     uint32_t sph = 0u;
     for (int i = 0; i < n_mine; ++i) {
-      const int at = tbeg + i, st = i & 1;
-      while (si + 1 < X.nseg && at >= X.segs[si + 1].first) ++si;
-      const Seen<kKeys> list = seen_range<kKeys>(X.segs[si].hi, X.segs[si].lo, X.segs[si].sinks);
-      const int k0 = list.granule(at - X.segs[si].first) * kKeys;
+      const int st = i & 1;
+      wait(&X.v_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);  // the scales and the place of the keys
+      const int k0 = X.k0[st];
       // the row's keys of this tile: [a, b] and [0, s0)
-      const int b = live && seg == si ? min(mine.p - k0, kKeys - 1) : -1;
+      const int b = live && seg == X.sg[st] ? min(mine.p - k0, kKeys - 1) : -1;
       const int a = mine.lo - k0, s0 = min(mine.sinks - k0, b + 1);
       // (what rows without a token do is not used)
       const bool whole = !live || (b == kKeys - 1 && (a <= 0 || s0 >= kKeys));
@@ -725,8 +727,6 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         auto below = [](int x) { return x <= 0 ? 0u : x >= 16 ? 0xffffu : (1u << x) - 1u; };
         return (below(b + 1 - c0) & ~below(a - c0)) | below(s0 - c0);
       };
-      wait(&X.k_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);  // the scales
-      wait(&X.v_full[st], (uint32_t)(i >> 1) & 1u, X, p.err);
       float ks[4], ve[4];  // of this half's 4 blocks
 #pragma unroll
       for (int c = 0; c < 4; ++c) ks[c] = qs * X.ks[st][4 * hf + c], ve[c] = X.ve[st][4 * hf + c];
