@@ -67,7 +67,7 @@ template <int FMT, int D, int PARTS>
 struct Shape {
   static constexpr int kTiles = D == 64 ? 2 : 1;  // query tiles of a CTA
   // warpgroups: two of softmax for each tile, producers, and one whose first warp issues MMAs
-  static constexpr int kSoftWarps = 8 * kTiles, kLoadWarp = kSoftWarps, kLoadWarps = 4, kMmaWarp = kLoadWarp + kLoadWarps;
+  static constexpr int kSoftWarps = 8 * kTiles, kLoadWarp = kSoftWarps, kLoadWarps = FMT == QI_KV_BF16 && D == 64 ? 8 : 4, kMmaWarp = kLoadWarp + kLoadWarps;
   static constexpr int kThreads = 32 * (kMmaWarp + 4);
   static constexpr uint32_t kQ = kRows * D * 2;   // one part of a tile's Q
   static constexpr uint32_t kT = kKeys * D * 2;   // K or V tile, two stages each
@@ -76,10 +76,10 @@ struct Shape {
   static constexpr uint32_t kColT = 3 * 128, kCols = 512;
   static_assert(kColT + kTiles * D <= kCols, "tensor memory");
   // Registers of a thread: of the launch, and of the warpgroups, which together have no more.
-  static constexpr int kRegLaunch = D == 64 ? 80 : 128;
+  static constexpr int kRegLaunch = D == 64 ? (kLoadWarps == 8 ? 72 : 80) : 128;
   static constexpr int kRegSoft = D == 64 ? (FMT == QI_KV_BF16 ? 88 : 96) : 152;
-  static constexpr int kRegLoad = D == 64 ? (FMT == QI_KV_BF16 ? 88 : 56) : 160, kRegMma = D == 64 ? 40 : 48;
-  static_assert(2 * kTiles * kRegSoft + kRegLoad + kRegMma <= (2 * kTiles + 2) * kRegLaunch, "the increase must be covered");
+  static constexpr int kRegLoad = D == 64 ? 56 : 160, kRegMma = D == 64 ? 40 : 48;
+  static_assert(kSoftWarps * kRegSoft + kLoadWarps * kRegLoad + 4 * kRegMma <= kThreads / 32 * kRegLaunch, "the increase must be covered");
 };
 
 constexpr int kMaxTok = 2 * kRows;  // tokens of a CTA
@@ -495,10 +495,11 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
     // a warp takes 32 keys; one of its loads is 8 keys x 4 chunks: whole lines, and the
     // lanes of a store phase hold 8 keys
     auto place = [&](int j, int& r, int& ch) {
-      r = lw * 32 + (j / (kCh / 4)) * 8 + (lane & 7);
+      r = lw * (kKeys / H::kLoadWarps) + (j / (kCh / 4)) * 8 + (lane & 7);
       ch = (j % (kCh / 4)) * 4 + (lane >> 3);
     };
-    uint4 kr[kN], vr[BF ? 1 : kN];  // bf16: V follows K in the same registers
+    constexpr bool kBoth = !BF || H::kLoadWarps == 8;  // else V follows K in the same registers
+    uint4 kr[kN], vr[kBoth ? kN : 1];
     float sc = 1.f;
     int si = 0, first_key = 0;  // segment of the tile at hand (entries come in order), its first key
     auto fetch = [&](int i, bool k_side) {
@@ -519,7 +520,7 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         place(j, r, ch);
         const bool in = o >= 0 && list.sees(k0 + r);
         const int x = (r * kCh + ch) * 16;
-        if constexpr (BF) {
+        if constexpr (!kBoth) {
           kr[j] = in ? __ldcg(reinterpret_cast<const uint4*>((k_side ? kb : vb) + x)) : z;
         } else {
           kr[j] = in ? __ldcg(reinterpret_cast<const uint4*>(kb + x)) : z;
@@ -548,11 +549,11 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         *reinterpret_cast<uint4*>(t + core<D>(r, 2 * ch + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
     };
-    // bf16 values -> fp16 operand rows, and the scales of the warp's two blocks of 16 keys
+    // bf16 values -> fp16 operand rows, and the scales of the warp's blocks of 16 keys
     auto store16 = [&](const uint4* regs, uint8_t* t, int st, bool k_side) {
-      constexpr int kB = kN / 2;  // chunks of a block
+      constexpr int kBlocks = 8 / H::kLoadWarps, kB = kN / kBlocks;  // blocks of the warp, chunks of a block
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < kBlocks; ++b) {
         uint32_t m2 = 0u;  // largest magnitudes of the low and the high halves
 #pragma unroll
         for (int j = b * kB; j < (b + 1) * kB; ++j)
@@ -577,8 +578,8 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         // scale and its reciprocal are normal); tiny blocks are left with a smaller maximum
         const uint32_t e = min(max(mx >> 7, 15u), 253u);
         if (lane == 0) {
-          if (k_side) X.ks[st][lw * 2 + b] = __uint_as_float((e - 14u) << 23);
-          else X.ve[st][lw * 2 + b] = (float)((int)e - 141), X.vf[st][lw * 2 + b] = 1.f;
+          if (k_side) X.ks[st][lw * kBlocks + b] = __uint_as_float((e - 14u) << 23);
+          else X.ve[st][lw * kBlocks + b] = (float)((int)e - 141), X.vf[st][lw * kBlocks + b] = 1.f;
         }
         // bf16 to fp16 at that scale: the exponent field moves by e - 29 (from e to 29, that
         // of 2^14) and the significand gains three zeros; values below fp16's normal range, 2^-28
@@ -625,8 +626,8 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       if constexpr (BF) {
         store16(kr, kt, st, true);
         publish(&X.k_full[st]);
-        fetch(tbeg + i, false);
-        store16(kr, vt, st, false);
+        if constexpr (!kBoth) fetch(tbeg + i, false);
+        store16(kBoth ? vr : kr, vt, st, false);
         publish(&X.v_full[st]);
       } else {
         if (lt < 8) X.ks[st][lt] = sc;
