@@ -69,16 +69,17 @@ __device__ __forceinline__ void append_block(const Kv8AppendParams& p, int t, in
   };
   if (tid < p.M) note(tid, q0, r0);
   constexpr int kBatch = 8;  // loads under way together
-  for (int i0 = tid + kAppendThreads; i0 < p.M; i0 += kBatch * kAppendThreads) {
+  const unsigned last = p.M - 1;
+  for (unsigned i0 = tid + kAppendThreads; i0 <= last; i0 += kBatch * kAppendThreads) {
     int q[kBatch], r[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int i = min(i0 + j * kAppendThreads, p.M - 1);  // the last token more than once does no harm
+      const unsigned i = min(i0 + j * kAppendThreads, last);  // the last token more than once does no harm
       q[j] = __ldg(p.pos + i);
       r[j] = __ldg(p.rows + i);
     }
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) note(min(i0 + j * kAppendThreads, p.M - 1), q[j], r[j]);
+    for (int j = 0; j < kBatch; ++j) note((int)min(i0 + j * kAppendThreads, last), q[j], r[j]);
   }
   __syncthreads();
   int f = 0;

@@ -9,6 +9,7 @@ the output's own rounding."""
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -157,6 +158,38 @@ def test_append_same_position_twice_idle_and_outside():
     cache.append(0, k[:3], v[:3], i32([0, 2, -1]), i32([64, 0, 0]))
     after = (cache.k.view(torch.int8), cache.v.view(torch.int8), cache.k_scale, cache.v_scale)
     assert all(torch.equal(a, b) for a, b in zip(before, after))
+    with pytest.raises(_lib.QiError):
+        cache.check()
+
+
+@pytest.mark.parametrize("fmt,block,dtype", [("int8", 16, torch.float32), ("e4m3", 128, torch.bfloat16)])
+def test_append_many_tokens_in_any_order(fmt, block, dtype):
+    """Enough tokens that a CTA takes several: whole prompts, then the same rows' next tokens
+    shuffled among idle slots, tokens outside the cache and positions that come twice."""
+    g, r = gen(8), random.Random(8)
+    n, length = 9, 400
+    cache = Kv8Cache(config(), n, length, device="cuda", format=fmt, block_tokens=block)
+    want = [Oracle8(n, 2, length, 64, fmt, block) for _ in range(2)]
+
+    def append(cells):
+        rows, pos = [c[0] for c in cells], [c[1] for c in cells]
+        k, v = (randn(g, len(cells), 2, 64).to(dtype) for _ in range(2))
+        cache.append(0, k, v, i32(rows), i32(pos))
+        inside = [i for i, c in enumerate(cells) if 0 <= c[0] < n and 0 <= c[1] < length]
+        for o, x in zip(want, (k, v)):
+            o.append(x[inside], [rows[i] for i in inside], [pos[i] for i in inside])
+
+    lengths = [r.randrange(100, 250) for _ in range(n)]
+    append([(i, p) for i in range(n) for p in range(lengths[i])])
+    same_values(cache, want, dict(enumerate(lengths)))
+    cache.check()
+    more = [r.randrange(1, 120) for _ in range(n)]
+    cells = [(i, lengths[i] + p) for i in range(n) for p in range(more[i])]
+    cells += r.choices(cells, k=40) + [(r.randrange(n), -1) for _ in range(60)]
+    cells += [(n, 3), (-1, 5), (2, length), (4, -2)]
+    r.shuffle(cells)
+    append(cells)
+    same_values(cache, want, {i: lengths[i] + more[i] for i in range(n)})
     with pytest.raises(_lib.QiError):
         cache.check()
 
