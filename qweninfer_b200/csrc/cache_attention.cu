@@ -553,17 +553,17 @@ int token_splits(const qi_kv_layer& c, int M, int window, int sinks) {
   return (int)(want > kMaxCluster ? want / kMaxCluster * kMaxCluster : want);
 }
 
-// Key splits of the prompt kernel, the CTAs of a cluster: as many as fill the CTAs that are
-// resident at once.
-int prompt_splits(const qi_kv_layer& c, int tiles, int window, int sinks) {
-  const long long slots = (c.head_dim == 64 ? 2LL : 1LL) * sm_count();
-  const long long n = slots / ((long long)tiles * c.kv_heads);
+// Key splits of the prompt kernel, the CTAs of a cluster: the most whose clusters all run at
+// once (a CTA takes an SM, and a cluster the SMs of one GPC, so large ones leave some idle:
+// 16 clusters of 8 do not fit, and took two rounds).
+int prompt_splits(const qi_kv_layer& c, int M, int group, int window, int sinks) {
+  const int tokens = kPromptRows / group * (c.head_dim == 64 ? 2 : 1);  // of a CTA
+  const long long clusters = (long long)((M - 1) / tokens + 1) * c.kv_heads;
   const long long most = (seen_at_most(c, window, sinks) / kPromptKeys + 2) / kMinTiles;
-  const long long want = n < most ? n : most;
-  return (int)(want > 8 ? 8 : want < 1 ? 1 : want);
+  int n = (int)(most > 8 ? 8 : most);
+  while (n > 1 && prompt_clusters(n) < clusters) --n;
+  return n < 1 ? 1 : n;
 }
-
-int prompt_tiles(int M, int group) { return (M + kPromptRows / group - 1) / (kPromptRows / group); }
 
 void sizes(CacheAttnPlan& r, const qi_kv_layer& c, int heads, int M) {
   r.part_floats = r.counters = 0;
@@ -579,7 +579,7 @@ CacheAttnPlan cache_attention_plan(const qi_kv_layer& c, int heads, int M, int w
   CacheAttnPlan r = {};
   r.prompt = query_run > 0 ? query_run >= 16 : M > 128;
   r.singles = r.prompt && query_run != M;
-  r.splits = r.prompt ? prompt_splits(c, prompt_tiles(M, heads / c.kv_heads), window, sinks) : 1;
+  r.splits = r.prompt ? prompt_splits(c, M, heads / c.kv_heads, window, sinks) : 1;
   r.token_splits = token_splits(c, M, window, sinks);
   sizes(r, c, heads, M);
   return r;

@@ -44,6 +44,8 @@ CacheAttnPlan cache_attention_plan(const qi_kv_layer& c, int heads, int M, int w
 void cache_attention_fit(CacheAttnPlan& plan, const qi_kv_layer& c, int heads, int M, long long part_floats,
                          long long counters);
 cudaError_t launch_cache_attention(const CacheAttnParams& p, const CacheAttnPlan& plan, cudaStream_t s, bool pdl);
+// Clusters of `size` CTAs (2..8) of that kernel that run at once on the current device.
+int prompt_clusters(int size);
 cudaError_t launch_cache_attention_prompt(const CacheAttnParams& p, cudaStream_t s, bool pdl);
 
 }  // namespace qi

@@ -40,6 +40,8 @@
 // tile sees are zero-filled; but in P V a zero weight times a NaN or infinity that another
 // row does see would be NaN. A row that ends up not finite is therefore computed again, key
 // by key (8-bit codes are always finite: only the bf16 cache needs it).
+#include <atomic>
+
 #include "cache_attention.cuh"
 #include "tc_device.cuh"
 
@@ -950,6 +952,40 @@ cudaError_t launch_dim(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
 }
 
 }  // namespace
+
+int prompt_clusters(int size) {
+  static std::atomic<int> known[kMaxDevices][9];  // 0: not yet queried
+  const int guess = sm_count() / size;
+  int dev = 0;
+  if (size < 2 || size > 8 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+    (void)cudaGetLastError();
+    return guess;
+  }
+  int n = known[dev][size].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  // one CTA on an SM in every variant; this one stands for all
+  using H = Shape<QI_KV_BF16, 128, 1>;
+  auto kernel = prompt_kernel<QI_KV_BF16, 128, 1>;
+  constexpr int smem = H::kOffMisc + kMiscBytes;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)size, 1, 1);
+  cfg.blockDim = dim3(H::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+    (void)cudaGetLastError();
+    return guess;
+  }
+  known[dev][size].store(n, std::memory_order_relaxed);
+  return n;
+}
 
 cudaError_t launch_cache_attention_prompt(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
   return p.c.head_dim == 64 ? launch_dim<64>(p, s, pdl) : launch_dim<128>(p, s, pdl);
