@@ -69,7 +69,7 @@ template <int FMT, int D, int PARTS>
 struct Shape {
   static constexpr int kTiles = D == 64 ? 2 : 1;  // query tiles of a CTA
   // warpgroups: two of softmax for each tile, producers, and one whose first warp issues MMAs
-  static constexpr int kSoftWarps = 8 * kTiles, kLoadWarp = kSoftWarps, kLoadWarps = FMT == QI_KV_BF16 && D == 64 ? 8 : 4, kMmaWarp = kLoadWarp + kLoadWarps;
+  static constexpr int kSoftWarps = 8 * kTiles, kLoadWarp = kSoftWarps, kLoadWarps = FMT == QI_KV_BF16 ? 8 : 4, kMmaWarp = kLoadWarp + kLoadWarps;
   static constexpr int kThreads = 32 * (kMmaWarp + 4);
   static constexpr uint32_t kQ = kRows * D * 2;   // one part of a tile's Q
   static constexpr uint32_t kT = kKeys * D * 2;   // K or V tile, two stages each
@@ -78,9 +78,9 @@ struct Shape {
   static constexpr uint32_t kColT = 3 * 128, kCols = 512;
   static_assert(kColT + kTiles * D <= kCols, "tensor memory");
   // Registers of a thread: of the launch, and of the warpgroups, which together have no more.
-  static constexpr int kRegLaunch = D == 64 ? (kLoadWarps == 8 ? 72 : 80) : 128;
+  static constexpr int kRegLaunch = kLoadWarps == 8 ? (D == 64 ? 72 : 96) : (D == 64 ? 80 : 128);
   static constexpr int kRegSoft = D == 64 ? (FMT == QI_KV_BF16 ? 88 : 96) : 152;
-  static constexpr int kRegLoad = D == 64 ? 56 : 160, kRegMma = D == 64 ? 40 : 48;
+  static constexpr int kRegLoad = D == 64 ? 56 : kLoadWarps == 8 ? 64 : 160, kRegMma = D == 64 ? 40 : 48;
   static_assert(kSoftWarps * kRegSoft + kLoadWarps * kRegLoad + 4 * kRegMma <= kThreads / 32 * kRegLaunch, "the increase must be covered");
 };
 
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       r = lw * (kKeys / H::kLoadWarps) + (j / (kCh / 4)) * 8 + (lane & 7);
       ch = (j % (kCh / 4)) * 4 + (lane >> 3);
     };
-    constexpr bool kBoth = !BF || H::kLoadWarps == 8;  // else V follows K in the same registers
+    constexpr bool kBoth = !BF || D == 64;  // else V follows K in the same registers
     uint4 kr[kN], vr[kBoth ? kN : 1];
     float sc = 1.f;
     int si = 0, first_key = 0;  // segment of the tile at hand (entries come in order), its first key
