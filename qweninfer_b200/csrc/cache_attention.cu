@@ -531,6 +531,18 @@ namespace {
 
 constexpr int kMinTiles = 4;
 
+// The tile kernel takes runs of kMinRun tokens and more of calls whose work, were every row
+// full, is at least kMinWork (tokens x KV heads x dims x keys). It starts at 18 to 39 us
+// whatever the work (tensor memory, the softmax chain of a CTA's few tiles, the cluster's
+// exchange), the per-token kernel at 7; but that reads and widens every key for each
+// token. Where positions are is known on the device only, so the choice goes by what the
+// layer lets them be. Measured at 4096 positions, us, per token / tiles, rows of 512 and of
+// 4000 keys; 14 heads on 2 of 64, int8, one row of 128 tokens (2^26): 10/28, 32/34; 256 (2^27):
+// 13/28, 57/38; 512: 16/29, 98/45; 16 on 2 of 128, bf16, 64 tokens (2^26): 12/40, 53/47; 128
+// (2^27): 23/40, 101/51; 8 on 8 of 64, int8, 32 tokens (2^26): 9/18, 31/20; 64 (2^27): 11/18, 55/21.
+constexpr int kMinRun = 16;
+constexpr long long kMinWork = 1LL << 27;
+
 long long seen_at_most(const qi_kv_layer& c, int window, int sinks) {
   const long long w = (long long)window + sinks;
   return window > 0 && w < c.max_len ? w : c.max_len;
@@ -577,7 +589,10 @@ void sizes(CacheAttnPlan& r, const qi_kv_layer& c, int heads, int M) {
 
 CacheAttnPlan cache_attention_plan(const qi_kv_layer& c, int heads, int M, int window, int sinks, int query_run) {
   CacheAttnPlan r = {};
-  r.prompt = query_run > 0 ? query_run >= 16 : M > 128;
+  const bool tiles = (query_run & QI_TILES) != 0;
+  query_run &= QI_TILES - 1;
+  const long long work = (long long)M * c.kv_heads * c.head_dim * seen_at_most(c, window, sinks);
+  r.prompt = tiles || ((query_run > 0 ? query_run >= kMinRun : M > 128) && work >= kMinWork);
   r.singles = r.prompt && query_run != M;
   r.splits = r.prompt ? prompt_splits(c, M, heads / c.kv_heads, window, sinks) : 1;
   r.token_splits = token_splits(c, M, window, sinks);

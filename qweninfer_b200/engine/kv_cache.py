@@ -136,7 +136,8 @@ class KVCache:
             raise ValueError(f"the last dimension of {name} must be contiguous")
 
     def attend(self, layer: int, q: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor, window: int = 0,
-               sinks: int = 0, query_run: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+               sinks: int = 0, query_run: int = 0, out: torch.Tensor | None = None,
+               tiles: bool = False) -> torch.Tensor:
         """Grouped-query attention of M query tokens over layer `layer` (qi_cache_attention).
 
         q: (M, heads, head_dim) float32, bfloat16 or float16, any strides of the first two
@@ -147,13 +148,14 @@ class KVCache:
         the host, which are checked (on the device, one outside the cache is recorded for
         `check()` and gives a zero output). `query_run`: the longest run of consecutive
         tokens of one row (a prompt's length), 1 for a decode step, 0 if unknown; it only
-        picks the kernel. Returns (M, heads, head_dim) of q's dtype (`out`, if given:
+        picks the kernel: long runs share their keys in tiles where that pays if the rows
+        are as long as max_len allows. `tiles`: whatever the size. Returns (M, heads, head_dim) of q's dtype (`out`, if given:
         contiguous, 16-byte aligned and apart from q), enqueued on the current stream.
 
         Scores, softmax and sums are fp32; q and the probabilities keep at least 22 bits for
         an 8-bit cache, 24 (16 for 16-bit q) for a bf16 one."""
         # what the shapes alone decide is checked once for each kind of call
-        key = (layer, q.shape, q.stride(), q.dtype, window, sinks, query_run)
+        key = (layer, q.shape, q.stride(), q.dtype, window, sinks, query_run, tiles)
         try:
             plan = self._plans.get(key)
         except AttributeError:
@@ -198,7 +200,8 @@ class KVCache:
             d, q.data_ptr(), st, sh, dtype, heads, rows.data_ptr(), pos.data_ptr(), q.shape[0], window, sinks,
             query_run, out.data_ptr(), part, part_floats, counters, n_counters, self._errors().data_ptr(), stream)
 
-    def _attend_plan(self, layer: int, q: torch.Tensor, window: int, sinks: int, query_run: int) -> tuple:
+    def _attend_plan(self, layer: int, q: torch.Tensor, window: int, sinks: int, query_run: int,
+                     tiles: bool) -> tuple:
         """The arguments of an `attend` call that its shapes decide, checked, and its scratch."""
         d = self.layer(layer)
         self._operand("q", q, None)
@@ -210,7 +213,8 @@ class KVCache:
         if window < 0 or sinks < 0 or query_run < 0:
             raise ValueError("window, sinks and query_run must not be negative")
         lim = 2**31 - 1
-        window, sinks, query_run = min(window, lim), min(sinks, lim), min(query_run, lim)
+        window, sinks = min(window, lim), min(sinks, lim)
+        query_run = min(query_run, _lib.QI_TILES - 1) | (_lib.QI_TILES if tiles else 0)
         a, b = C.c_longlong(), C.c_longlong()
         if M:
             with _lib.on_device(self.k.device):
@@ -316,12 +320,13 @@ class PagedKVCache(KVCache):
                               self.table.data_ptr(), self.page_size, self.pages_per_row, self.n_pages)
 
     def attend(self, layer: int, q: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor, window: int = 0,
-               sinks: int = 0, query_run: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+               sinks: int = 0, query_run: int = 0, out: torch.Tensor | None = None,
+               tiles: bool = False) -> torch.Tensor:
         """KVCache.attend; page-table changes are published first (`sync`). A page that a
         token sees but the table does not map is recorded for `check()` and counts as
         zeros."""
         self.sync()
-        return super().attend(layer, q, rows, pos, window, sinks, query_run, out)
+        return super().attend(layer, q, rows, pos, window, sinks, query_run, out, tiles)
 
     def reserve(self, row: int, length: int) -> None:
         if not 0 <= row < self.max_batch or not 0 <= length <= self.max_len:

@@ -265,7 +265,7 @@ def attention_bound(out, mags, vmax, keys, dtype, bits):
 
 
 def check_attend(cache, values, q, rows, pos, window, sinks, run, bits):
-    got = cache.attend(0, q, i32(rows), i32(pos), window=window, sinks=sinks, query_run=run)
+    got = cache.attend(0, q, i32(rows), i32(pos), window=window, sinks=sinks, query_run=run, tiles=run > 1)
     assert got.dtype == q.dtype and got.shape == q.shape
     pos_t = torch.as_tensor(pos).cuda()
     out, mags, vmax = reference(q, *values, rows, pos_t, window, sinks)
@@ -350,6 +350,29 @@ def test_attend_prompts(fmt, dtype, n, start, window, sinks):
     cache.check()
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 64), (5, 5, 128), (16, 2, 128), (3, 1, 64)])
+def test_attend_prompts_head_layouts(fmt, heads, kv, dim):
+    cache, values = filled(fmt, heads, kv, dim, 2, 300, 26)
+    q = 2 * randn(gen(27), 180, heads, dim)
+    check_attend(cache, values, q, [1] * 130 + [0] * 50, list(range(170, 300)) + list(range(50)), 0, 0, 130,
+                 bits_of(fmt, torch.float32))
+    check_attend(cache, values, q, [1] * 130 + [0] * 50, list(range(170, 300)) + list(range(50)), 90, 7, 130,
+                 bits_of(fmt, torch.float32))
+
+
+@pytest.mark.parametrize("n", [511, 513])
+def test_attend_prompts_by_size(n):
+    """A run on either side of the work from which tiles are taken (2^27)."""
+    cache, values = filled("e4m3", 14, 2, 64, 1, 2048, 28)
+    q = 2 * randn(gen(29), n, 14, 64)
+    check = dict(bits=bits_of("e4m3", torch.float32), window=0, sinks=0)
+    got = cache.attend(0, q, i32([0] * n), i32(range(300, 300 + n)), query_run=n)
+    tiles = check_attend(cache, values, q, [0] * n, list(range(300, 300 + n)), run=n, **check)
+    single = check_attend(cache, values, q, [0] * n, list(range(300, 300 + n)), run=1, **check)
+    assert torch.equal(got, tiles if n * 2 * 64 * 2048 >= 2 ** 27 else single)
+
+
 def test_attend_dead_positions_are_not_read():
     """NaN, infinities and wild scales behind the rows' ends and before the window change
     nothing."""
@@ -357,7 +380,7 @@ def test_attend_dead_positions_are_not_read():
         cache, _ = filled(fmt, 14, 2, 64, 2, 400, 10)
         q = 2 * randn(gen(11), 40, 14, 64)
         rows, pos = i32([0] * 39 + [1]), i32(list(range(170, 209)) + [5])
-        clean = [cache.attend(0, q, rows, pos, window=60, sinks=5, query_run=r) for r in (1, 39)]
+        clean = [cache.attend(0, q, rows, pos, window=60, sinks=5, query_run=r, tiles=r > 1) for r in (1, 39)]
         lo, hi = 111, 208  # seen by row 0's tokens: the window's union, and the sinks
         for t in (cache.k, cache.v):
             if fmt == "bf16":
@@ -375,7 +398,7 @@ def test_attend_dead_positions_are_not_read():
                 s[0, 0, :, hi // 32 + 1:] = float("inf")
                 s[0, 1, :, 1:] = float("nan")
         for r, want in zip((1, 39), clean):
-            assert torch.equal(cache.attend(0, q, rows, pos, window=60, sinks=5, query_run=r), want)
+            assert torch.equal(cache.attend(0, q, rows, pos, window=60, sinks=5, query_run=r, tiles=r > 1), want)
 
 
 def test_attend_values_that_are_seen_show():
@@ -421,16 +444,16 @@ def test_attend_paged_matches_packed():
     rows, pos = i32([2] * 127 + [0, 1, 1]), i32(list(range(300, 427)) + [499, 128, -1])
     for run in (1, 127):
         for window, sinks in ((0, 0), (70, 3)):
-            assert torch.equal(paged.attend(0, q, rows, pos, window, sinks, run),
-                               packed.attend(0, q, rows, pos, window, sinks, run))
+            assert torch.equal(paged.attend(0, q, rows, pos, window, sinks, run, tiles=run > 1),
+                               packed.attend(0, q, rows, pos, window, sinks, run, tiles=run > 1))
     paged.check()
     # a window's released pages are not touched; a page that is seen and missing is reported
     paged._t[2, 0] = -1
     paged.dirty = True
-    assert torch.equal(paged.attend(0, q[:127], rows[:127], pos[:127], 100, 0, 127),
-                       packed.attend(0, q[:127], rows[:127], pos[:127], 100, 0, 127))
+    assert torch.equal(paged.attend(0, q[:127], rows[:127], pos[:127], 100, 0, 127, tiles=True),
+                       packed.attend(0, q[:127], rows[:127], pos[:127], 100, 0, 127, tiles=True))
     paged.check()
-    paged.attend(0, q[:127], rows[:127], pos[:127], 100, 4, 127)
+    paged.attend(0, q[:127], rows[:127], pos[:127], 100, 4, 127, tiles=True)
     with pytest.raises(_lib.QiError):
         paged.check()
 
@@ -440,7 +463,7 @@ def test_attend_outside_the_cache_is_reported():
     q = randn(gen(18), 5, 14, 64)
     for run in (1, 5):
         cache._errors().zero_()
-        got = cache.attend(0, q, i32([0, 0, 2, -1, 1]), i32([64, -2, 3, 3, 63]), query_run=run)
+        got = cache.attend(0, q, i32([0, 0, 2, -1, 1]), i32([64, -2, 3, 3, 63]), query_run=run, tiles=run > 1)
         assert not got[:4].any() and got[4].any()
         with pytest.raises(_lib.QiError):
             cache.check()
