@@ -128,6 +128,23 @@ def test_forward_matches_the_restatement(model, weights, fmt, window, sinks, pag
     model.check()
 
 
+@pytest.mark.parametrize("fmt,window,sinks,paged", [("bf16", 2700, 4, False), ("int8", 0, 0, True)])
+def test_long_prompt_matches_the_restatement(model, weights, fmt, window, sinks, paged):
+    """A prompt whose attention shares keys in tiles (400 tokens x 2 x 64 x window or length is
+    above 2^27), and a token behind it."""
+    ids = prompt(401, 2)
+    ref = Reference(weights, fmt, window, sinks)
+    cache = make_cache(fmt, window, sinks, 2, 4096, paged)
+    cache.row_start = 1
+    for lo, hi in [(0, 400), (400, 401)]:
+        want = ref.step(ids[lo:hi])
+        got = model(torch.tensor([ids[lo:hi]]), positions=torch.arange(lo, hi), cache=cache, logits_dtype=torch.float32)[0]
+        for t in range(hi - lo):
+            err, cos = logit_report(got[t].cpu().numpy(), want[t].numpy())
+            assert err <= LOGIT_ATOL and cos >= LOGIT_MIN_COS, (lo + t, err, cos)
+    model.check()
+
+
 @pytest.mark.parametrize("fmt,window,sinks", OPTIONS)
 @pytest.mark.parametrize("page_size", [0, 128])
 def test_engine_matches_solo_generation(model, fmt, window, sinks, page_size):
