@@ -83,8 +83,8 @@ __device__ __forceinline__ void append_block(const Kv8AppendParams& p, int t, in
   }
   __syncthreads();
   int f = 0;
-  while (slot[f] < 0) ++f;  // ends: this token's own slot is taken
-  if (slot[f] != t) return;
+  while (f < block && slot[f] < 0) ++f;  // (this token's own slot is taken, unless pos changes meanwhile)
+  if (f == block || slot[f] != t) return;
   if (base < 0) {
     if (tid == 0 && p.err) atomicExch(p.err, QI_ERR_INDEX);
     return;

@@ -425,6 +425,38 @@ def test_attend_ranges(scale):
     assert float((got.double() - out).abs().max()) <= tol * float(values[1].abs().max())
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_offsets_beyond_32_bits(fmt):
+    """A row whose last heads lie more than 2^32 elements into the layer, against a short one
+    with the same keys: positions apart by a multiple of every block and tile."""
+    long, short, n = 2 ** 22 + 2 ** 18, 256, 200
+    base = long - short
+    g, cfg = gen(31), config(8, 8, 128)
+    k, v = (randn(g, n, 8, 128) for _ in range(2))
+    q = 2 * randn(g, 40, 8, 128)
+    pos = list(range(n - 40, n))
+
+    def make(length, at):
+        if fmt == "int8":
+            c = Kv8Cache(cfg, 1, length, device="cuda")
+            c.append(0, k, v, i32([0] * n), i32(range(at, at + n)))
+            return c
+        c = KVCache(cfg, 1, length, dtype=torch.bfloat16, device="cuda")
+        c.k[0, 0, :, at:at + n], c.v[0, 0, :, at:at + n] = k.transpose(0, 1), v.transpose(0, 1)
+        return c
+
+    near, far = make(short, 0), make(long, base)
+    assert far.k[0].numel() > 2 ** 32
+    values = near.values(0) if fmt == "int8" else (near.k[0], near.v[0])
+    for window in (1, 100):
+        out, mags, vmax = reference(q, *values, [0] * 40, i32(pos), window, 0)
+        tol = attention_bound(out, mags, vmax, n, q.dtype, bits_of(fmt, q.dtype))
+        for tiles in (False, True):
+            got = far.attend(0, q, i32([0] * 40), i32([base + p for p in pos]), window=window, query_run=40, tiles=tiles)
+            assert ((got.double() - out).abs() <= tol).all()
+    far.check()
+
+
 def test_attend_paged_matches_packed():
     g = gen(16)
     cfg = config()
