@@ -223,9 +223,9 @@ int qi_kv8_values(const qi_kv_layer* layer, float* k_out, float* v_out, qi_strea
  * F16, element strides of token and head, dims contiguous; heads = group * kv_heads, group
  * 1..8. out: (M, heads, head_dim) of the same dtype, 16-byte aligned, must not overlap q. query_run: longest
  * run of consecutive tokens of one cache row (a prompt's length), 1 for a decode step, 0 if
- * unknown (at most QI_TILES - 1); it picks the kernel, any value gives the same result up to
+ * unknown (at most QI_RUN_TILES - 1); it picks the kernel, any value gives the same result up to
  * rounding. Runs of 16 tokens and more share their keys in tiles, if the call is large enough
- * for that to pay on rows as long as the layer allows; query_run | QI_TILES takes tiles in
+ * for that to pay on rows as long as the layer allows; query_run | QI_RUN_TILES takes tiles in
  * any case (rows are known to be long, say).
  * part: scratch of part_floats floats; counters: counters_len uint32, zero before the first
  * call and left zero. qi_cache_attention_scratch gives the sizes that use the whole GPU;
@@ -233,7 +233,7 @@ int qi_kv8_values(const qi_kv_layer* layer, float* k_out, float* v_out, qi_strea
  * and an unmapped page set *err to QI_ERR_INDEX; the token's output is zero, or the page's
  * keys count as zeros. Replaces the attention core of qweninfer/models/qwen2.py:184-199,
  * which has no window. */
-#define QI_TILES 0x40000000
+#define QI_RUN_TILES 0x40000000
 int qi_cache_attention(const qi_kv_layer* layer, const void* q, long long q_token_stride, long long q_head_stride,
                        int dtype, int heads, const int32_t* rows, const int32_t* pos, int M, int window, int sinks,
                        int query_run, void* out, float* part, long long part_floats, unsigned int* counters,

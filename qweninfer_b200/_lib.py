@@ -22,7 +22,7 @@ QI_ERR_DEVICE = 1003
 QI_ERR_TOO_LARGE = 1004
 QI_ERR_INDEX = 1005
 QI_KV_BF16, QI_KV_INT8, QI_KV_E4M3 = 0, 1, 2
-QI_TILES = 0x40000000
+QI_RUN_TILES = 0x40000000
 LOGPROBS_COUNTERS = 1024
 # element types of activations (QI_F32, QI_BF16, QI_F16)
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}

@@ -91,7 +91,8 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Granules a split has at least: one for each warp.
+// Granules a split has at least: one for each warp. (One row of 700 keys: 6.2 us, with twice as
+// many 7.5.)
 constexpr int kMinSplit = kWarps;
 constexpr int kMaxCluster = 8;
 
@@ -529,17 +530,20 @@ cudaError_t launch_dim(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
 
 namespace {
 
-constexpr int kMinTiles = 4;
+// Key tiles a CTA of the tile kernel has at least: the exchange in a cluster costs less than
+// another tile's softmax. 128 tokens, 14 heads on 2 of 64, int8, rows of 512 keys: 19.7 us, with
+// two tiles 21.7, four 27.3; 1500 keys: 24.4, 26.2, 34.4.
+constexpr int kMinTiles = 1;
 
 // The tile kernel takes runs of kMinRun tokens and more of calls whose work, were every row
-// full, is at least kMinWork (tokens x KV heads x dims x keys). It starts at 18 to 39 us
+// full, is at least kMinWork (tokens x KV heads x dims x keys). It starts at 13 to 27 us
 // whatever the work (tensor memory, the softmax chain of a CTA's few tiles, the cluster's
 // exchange), the per-token kernel at 7; but that reads and widens every key for each
 // token. Where positions are is known on the device only, so the choice goes by what the
 // layer lets them be. Measured at 4096 positions, us, per token / tiles, rows of 512 and of
-// 4000 keys; 14 heads on 2 of 64, int8, one row of 128 tokens (2^26): 10/28, 32/34; 256 (2^27):
-// 13/28, 57/38; 512: 16/29, 98/45; 16 on 2 of 128, bf16, 64 tokens (2^26): 12/40, 53/47; 128
-// (2^27): 23/40, 101/51; 8 on 8 of 64, int8, 32 tokens (2^26): 9/18, 31/20; 64 (2^27): 11/18, 55/21.
+// 4000 keys; 14 heads on 2 of 64, int8, one row of 128 tokens (2^26): 10/20, 32/32; 256 (2^27):
+// 13/20, 57/38; 512: 16/21, 98/45; 16 on 2 of 128, bf16, 64 tokens (2^26): 13/26, 53/42; 128
+// (2^27): 23/27, 100/51; 8 on 8 of 64, int8, 32 tokens (2^26): 9/13, 31/20; 64 (2^27): 12/13, 54/21.
 constexpr int kMinRun = 16;
 constexpr long long kMinWork = 1LL << 27;
 
@@ -562,6 +566,12 @@ int token_splits(const qi_kv_layer& c, int M, int window, int sinks) {
   long long want = (long long)ctas * sm_count() * 9 / 10 / units;
   want = want > most ? most : want;
   want = want > kMaxTokenSplits ? kMaxTokenSplits : want < 1 ? 1 : want;
+  // Where a warp has only a few granules, no more splits than leave it as few: 8 rows' 8064 keys
+  // of 2 heads are 2 for each warp of 40 splits and of 32, which take 16.5 and 14.5 us. (Over
+  // many granules the last one counts for little, and rows shorter than the longest use
+  // every split: 31.9 us against 29.8 on ragged rows of up to 32768.)
+  const long long rounds = (gran + want * kWarps - 1) / (want * kWarps);
+  if (rounds <= 4) want = (gran + rounds * kWarps - 1) / (rounds * kWarps);
   return (int)(want > kMaxCluster ? want / kMaxCluster * kMaxCluster : want);
 }
 
@@ -589,8 +599,8 @@ void sizes(CacheAttnPlan& r, const qi_kv_layer& c, int heads, int M) {
 
 CacheAttnPlan cache_attention_plan(const qi_kv_layer& c, int heads, int M, int window, int sinks, int query_run) {
   CacheAttnPlan r = {};
-  const bool tiles = (query_run & QI_TILES) != 0;
-  query_run &= QI_TILES - 1;
+  const bool tiles = (query_run & QI_RUN_TILES) != 0;
+  query_run &= QI_RUN_TILES - 1;
   const long long work = (long long)M * c.kv_heads * c.head_dim * seen_at_most(c, window, sinks);
   r.prompt = tiles || ((query_run > 0 ? query_run >= kMinRun : M > 128) && work >= kMinWork);
   r.singles = r.prompt && query_run != M;

@@ -214,7 +214,7 @@ class KVCache:
             raise ValueError("window, sinks and query_run must not be negative")
         lim = 2**31 - 1
         window, sinks = min(window, lim), min(sinks, lim)
-        query_run = min(query_run, _lib.QI_TILES - 1) | (_lib.QI_TILES if tiles else 0)
+        query_run = min(query_run, _lib.QI_RUN_TILES - 1) | (_lib.QI_RUN_TILES if tiles else 0)
         a, b = C.c_longlong(), C.c_longlong()
         if M:
             with _lib.on_device(self.k.device):
