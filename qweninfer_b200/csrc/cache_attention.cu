@@ -50,8 +50,10 @@ struct Shape {
   static constexpr int kStage = 2 * kTensor + 16;                // + 2 K scales, 2 V scales
   static constexpr int kStages = 2;
   static constexpr size_t kRing = (size_t)kWarps * kStages * kStage;
-  // CTAs of an SM: by registers for 8-bit codes, by shared memory otherwise
-  static constexpr int kCtas = FMT == QI_KV_BF16 ? (D == 64 ? 3 : 1) : (D == 64 ? 5 : 3);
+  // CTAs of an SM: by registers for 8-bit codes (head_dim 64: 26.7 us on two rows of 131072, with
+  // 5 CTAs 29.5, with 3 27.3; 128: 3 CTAs 29.4 us on 64 rows of 4096, with 2 34.8), by shared
+  // memory otherwise
+  static constexpr int kCtas = FMT == QI_KV_BF16 ? (D == 64 ? 3 : 1) : (D == 64 ? 4 : 3);
   static_assert((kRing + 6 * 1024) * kCtas <= 228 * 1024, "shared memory of an SM");
 };
 
@@ -566,12 +568,10 @@ int token_splits(const qi_kv_layer& c, int M, int window, int sinks) {
   long long want = (long long)ctas * sm_count() * 9 / 10 / units;
   want = want > most ? most : want;
   want = want > kMaxTokenSplits ? kMaxTokenSplits : want < 1 ? 1 : want;
-  // Where a warp has only a few granules, no more splits than leave it as few: 8 rows' 8064 keys
-  // of 2 heads are 2 for each warp of 40 splits and of 32, which take 16.5 and 14.5 us. (Over
-  // many granules the last one counts for little, and rows shorter than the longest use
-  // every split: 31.9 us against 29.8 on ragged rows of up to 32768.)
-  const long long rounds = (gran + want * kWarps - 1) / (want * kWarps);
-  if (rounds <= 4) want = (gran + rounds * kWarps - 1) / (rounds * kWarps);
+  // Sums of several clusters go through global memory, 3 us: up to 9 rounds of a cluster's warps
+  // (9216 keys) cost less. 8 rows of 4096, int8, 2 heads of 64: 8.8 us in one cluster, 12.9 in
+  // two; one row of 16384 (16 rounds): 17.0 in one, 14.3 in several.
+  if (want > kMaxCluster && gran <= 9 * kMaxCluster * kWarps) want = kMaxCluster;
   return (int)(want > kMaxCluster ? want / kMaxCluster * kMaxCluster : want);
 }
 
