@@ -31,8 +31,11 @@ namespace {
 constexpr int kWarps = 8;                     // that compute; one more copies
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kStages = 2;
-constexpr int kChunk = 32768;                 // bytes; a warp's share is 8 vectors of every lane
-constexpr int kCtas = 3;                      // of an SM
+// Bytes of a chunk (a warp's share is 8 vectors of every lane) and CTAs of an SM. 64 rows of
+// 151936 bf16, top 20: 19.8 us, 1000 rows of fp32: 100 (0.94 of the copy rate); with chunks of 16 KB in
+// four stages 22.3 and 97, with two CTAs of three stages 25.2 and 101.
+constexpr int kChunk = 32768;
+constexpr int kCtas = 3;
 constexpr int kList = 32;
 constexpr int kPairs = 128;                   // steps that are read again
 constexpr float kLog2e = 1.4426950408889634f;
