@@ -389,6 +389,10 @@ int grid_for(int n_tiles, int KB, int max_contrib) {
   return (int)(g < sms ? g : sms);
 }
 
+// NULL, or not aligned to `bytes`
+bool bad_align(const void* p, int bytes) { return !p || (uintptr_t)p % bytes != 0; }
+int elem_bytes(int dtype) { return dtype == QI_F32 ? 4 : 2; }
+
 bool bad_attention(const qi_kv_layer* c, int heads, int M, int window, int sinks, int query_run) {
   return bad_layer(c) || heads <= 0 || heads % c->kv_heads != 0 || heads / c->kv_heads > 8 || M <= 0 || window < 0 ||
          sinks < 0 || query_run < 0 || c->kv_heads > 65535 || (long long)M * 256 > 0x7fffffffLL;
@@ -788,8 +792,8 @@ int qi_move_rows(uint16_t* k, uint16_t* v, int layers, int cache_rows, int max_l
 int qi_kv8_append(const qi_kv_layer* layer, const void* k, long long k_token_stride, long long k_head_stride,
                   const void* v, long long v_token_stride, long long v_head_stride, int dtype, const int32_t* rows,
                   const int32_t* pos, int M, int* err, qi_stream_t stream) {
-  if (bad_layer(layer) || layer->format == QI_KV_BF16 || bad_ptr(k) || bad_ptr(v) || bad_dtype(dtype) ||
-      bad_ptr(rows) || bad_ptr(pos) || M <= 0 || layer->kv_heads > 65535)
+  if (bad_layer(layer) || layer->format == QI_KV_BF16 || bad_dtype(dtype) || bad_align(k, elem_bytes(dtype)) ||
+      bad_align(v, elem_bytes(dtype)) || bad_align(rows, 4) || bad_align(pos, 4) || M <= 0 || layer->kv_heads > 65535)
     return QI_ERR_ARG;
   return rc(launch_kv8_append(*layer, k, v, dtype, k_token_stride, k_head_stride, v_token_stride, v_head_stride, rows,
                               pos, M, err, as_stream(stream), false));
@@ -815,8 +819,8 @@ int qi_cache_attention(const qi_kv_layer* layer, const void* q, long long q_toke
                        int dtype, int heads, const int32_t* rows, const int32_t* pos, int M, int window, int sinks,
                        int query_run, void* out, float* part, long long part_floats, unsigned int* counters,
                        long long counters_len, int* err, qi_stream_t stream) {
-  if (bad_attention(layer, heads, M, window, sinks, query_run) || bad_ptr(q) || bad_dtype(dtype) || bad_ptr(rows) ||
-      bad_ptr(pos) || bad_ptr(out) || ((uintptr_t)out & 15) || ((uintptr_t)part & 7))
+  if (bad_attention(layer, heads, M, window, sinks, query_run) || bad_dtype(dtype) || bad_align(q, elem_bytes(dtype)) ||
+      bad_align(rows, 4) || bad_align(pos, 4) || bad_align(out, 16) || ((uintptr_t)part & 7) || ((uintptr_t)counters & 3))
     return QI_ERR_ARG;
   CacheAttnParams p = {};
   p.c = *layer;
@@ -848,7 +852,9 @@ long long qi_token_logprobs_scratch(int M, int V, int dtype) {
 int qi_token_logprobs(const void* logits, int dtype, long long ld, const void* targets, int targets_64, int M, int V,
                       int top, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, void* scratch,
                       long long scratch_bytes, unsigned int* counters, qi_stream_t stream) {
-  if (bad_ptr(logits) || bad_dtype(dtype) || M <= 0 || V <= 0 || ld < V || top < 0 || top > 32 || top > V ||
+  if (bad_dtype(dtype) || bad_align(logits, elem_bytes(dtype)) || (uintptr_t)targets % (targets_64 ? 8 : 4) != 0 ||
+      (((uintptr_t)logprob | (uintptr_t)entropy | (uintptr_t)top_ids | (uintptr_t)top_logprobs | (uintptr_t)counters) & 3) ||
+      M <= 0 || V <= 0 || ld < V || top < 0 || top > 32 || top > V ||
       (top > 0 && (bad_ptr(top_ids) || bad_ptr(top_logprobs))) || ((uintptr_t)scratch & 15))
     return QI_ERR_ARG;
   LogprobPlan plan = logprob_plan(M, V, dtype);

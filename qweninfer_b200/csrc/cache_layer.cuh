@@ -141,6 +141,7 @@ inline bool bad_layer(const qi_kv_layer* c) {
     return true;
   if (c->format == QI_KV_BF16) return false;
   if (c->format != QI_KV_INT8 && c->format != QI_KV_E4M3) return true;
+  if (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3) return true;
   return !c->k_scale || !c->v_scale || (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128);
 }
 inline bool bad_dtype(int dt) { return dt != QI_F32 && dt != QI_BF16 && dt != QI_F16; }

@@ -75,6 +75,27 @@ def test_bad_calls(lib):
         assert logprobs(**kw) == E, kw
 
 
+def test_misaligned_pointers(lib):
+    d = layer()
+    for kw in (dict(k=2), dict(v=6), dict(k=1, dt=1), dict(v=3, dt=2), dict(rows=2), dict(pos=6)):
+        assert append(lib, d, **{"k": 16, "v": 16, "rows": 16, "pos": 16, **kw}) == E, kw
+    for kw in (dict(q=2), dict(q=1, dt=1), dict(rows=2), dict(pos=1), dict(out=4), dict(part=4)):
+        assert attend(lib, d, **{"q": 16, "rows": 16, "pos": 16, **kw}) == E, kw
+    assert append(lib, layer(k_scale=2), k=16, v=16, rows=16, pos=16) == E
+    for i, x in ((0, 2), (3, 4), (8, 2), (9, 1), (10, 2), (11, 2), (14, 2)):
+        args = [16, 0, 100, 16, 1, 1, 100, 1, 16, 16, 16, 16, 16, 0, 16, None]
+        args[i] = x
+        assert lib.qi_token_logprobs(*args) == E, (i, x)
+
+
+def test_scratch_of_runs_in_tiles(lib):
+    """QI_RUN_TILES belongs to the run's length: no other check takes it for one."""
+    a, b = C.c_longlong(-1), C.c_longlong(-1)
+    run = _lib.QI_RUN_TILES | 77
+    assert lib.qi_cache_attention_scratch(C.byref(layer(max_len=64)), 14, 77, 0, 0, run, C.byref(a), C.byref(b)) == 0
+    assert a.value == b.value == 0
+
+
 def test_scratch_sizes(lib):
     a, b = C.c_longlong(-1), C.c_longlong(-1)
     assert lib.qi_cache_attention_scratch(C.byref(layer(max_len=64)), 14, 4, 0, 0, 1, C.byref(a), C.byref(b)) == 0
