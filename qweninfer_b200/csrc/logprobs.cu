@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
     const f2 log2e = pack2(kLog2e, kLog2e);
     for (int k = k0; k < k1; ++k, ++u) {
       const int i = u - u0, st = i % kStages, n = vecs_in(nvec, k);
-      mbar_wait(&ring.full[st], (uint32_t)((i / kStages) & 1), nullptr);
+      // a copy that never came makes the row's results NaN
+      if (!mbar_wait(&ring.full[st], (uint32_t)((i / kStages) & 1), nullptr)) z = pack2(NAN, NAN);
       const int v0 = warp * (kVecs / kWarps) + lane;  // this lane's first vector of the chunk
       const uint4* c = reinterpret_cast<const uint4*>(smem + st * kChunk) + v0;
       auto chunk = [&](auto whole) {
