@@ -535,6 +535,31 @@ def test_streams_graphs_and_reuse():
         assert all(torch.equal(out, want[i]) for _, out in graphs) and torch.equal(eager, one)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_captured_prompts(fmt):
+    """A prompt with another row's single token behind it, captured and replayed over changing
+    queries and positions while eager calls run on another stream: the eager calls' bits."""
+    cache, _ = filled(fmt, 14, 2, 64, 3, 700, 32)
+    q = [2 * randn(gen(33 + i), 151, 14, 64) for i in range(2)]
+    rows = i32([1] * 150 + [2])
+    pos = [i32(list(range(a, a + 150)) + [a]) for a in (400, 17)]
+    want = [cache.attend(0, q[i], rows, pos[i], query_run=150, tiles=True) for i in range(2)]
+    qb, pb = q[0].clone(), pos[0].clone()
+    side, gr = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(gr):
+        out = cache.attend(0, qb, rows, pb, query_run=150, tiles=True)
+    for i in (0, 1, 0):
+        qb.copy_(q[i])
+        pb.copy_(pos[i])
+        gr.replay()
+        with torch.cuda.stream(side):
+            eager = cache.attend(0, q[1 - i], rows, pos[1 - i], query_run=150, tiles=True)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i]) and torch.equal(eager, want[1 - i])
+    cache.check()
+
+
 def test_append_then_attend_as_a_server_does():
     """A prompt and decode steps through append and attend, against attention over what the
     cache stands for; a row move keeps a row's outputs; rows behind the last are untouched."""
