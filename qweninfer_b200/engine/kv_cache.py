@@ -23,6 +23,7 @@ sliding window and first tokens that stay visible.
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import numpy as np
 import torch
@@ -171,7 +172,7 @@ class KVCache:
         M = q.shape[0]
         rows, pos = self._tokens(M, rows, pos)
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)  # 1 us less than new_empty
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {q.device}")
         elif out.data_ptr() % 16:
@@ -473,18 +474,27 @@ class _Codes:
     def values(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
         """What layer `layer` stands for: K and V (max_batch, kv_heads, max_len, head_dim)
         fp32 (qi_kv8_values). Dead positions give whatever their codes say."""
-        d = self.layer(layer)
-        dev = self.k.device
-        if dev.type != "cuda":
-            _require(self.k_scale, "values", dev)
-        if d.head_dim not in (64, 128):
-            raise ValueError(f"head_dim must be 64 or 128, got {d.head_dim}")
-        k, v = self.k_scale.new_empty((2, self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1])).unbind(0)
+        try:
+            plan = self._value_plans.get(layer)
+        except AttributeError:
+            self._value_plans, plan = {}, None
+        if plan is None:
+            d = self.layer(layer)
+            dev = self.k.device
+            if dev.type != "cuda":
+                _require(self.k_scale, "values", dev)
+            if d.head_dim not in (64, 128):
+                raise ValueError(f"head_dim must be 64 or 128, got {d.head_dim}")
+            shape = (self.max_batch, d.kv_heads, self.max_len, d.head_dim)
+            strides = tuple(math.prod(shape[i + 1:]) for i in range(4))
+            plan = self._value_plans[layer] = C.byref(d), dev, shape, strides
+        d, dev, shape, strides = plan
+        k, v = (torch.empty_strided(shape, strides, dtype=torch.float32, device=dev) for _ in range(2))
         if _lib.ready(dev.index):
-            code = _lib.lib().qi_kv8_values(C.byref(d), k.data_ptr(), v.data_ptr(), _lib.stream_ptr(dev))
+            code = _lib.lib().qi_kv8_values(d, k.data_ptr(), v.data_ptr(), torch._C._cuda_getCurrentRawStream(dev.index))
         else:
             with _lib.on_device(dev):
-                code = _lib.lib().qi_kv8_values(C.byref(d), k.data_ptr(), v.data_ptr(), _lib.stream_ptr(dev))
+                code = _lib.lib().qi_kv8_values(d, k.data_ptr(), v.data_ptr(), _lib.stream_ptr(dev))
         if code:
             _lib.check(code, "qi_kv8_values")
         return k, v
