@@ -58,34 +58,33 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     if targets is not None and not (targets.dtype in _INTS and targets.device == dev and targets.shape == (M,)
                                     and targets.is_contiguous()):
         targets = _targets(targets, M, V, dev)
-    # the outputs share one allocation
-    buf = torch.empty(2 * M * (1 + top), dtype=torch.float32, device=dev)
-    if top:
-        lp, ent, ids, lps = buf.split((M, M, M * top, M * top))
-        r = TokenLogprobs(lp if targets is not None else None, ent, ids.view(torch.int32).view(M, top), lps.view(M, top))
-    else:
-        lp, ent = buf.split(M) if M else (buf, buf)
-        r = TokenLogprobs(lp if targets is not None else None, ent, None, None)
+    f32, new = torch.float32, torch.empty_strided  # (the cheapest of the ways to allocate)
+    ent = new((M,), (1,), dtype=f32, device=dev)
+    lp = new((M,), (1,), dtype=f32, device=dev) if targets is not None else None
+    ids = new((M, top), (top, 1), dtype=torch.int32, device=dev) if top else None
+    lps = new((M, top), (top, 1), dtype=f32, device=dev) if top else None
+    r = TokenLogprobs(lp, ent, ids, lps)
     if M == 0:
         return r
     if _lib.ready(dev.index):
-        code = _call(logits, plan, targets, top, buf.data_ptr())
+        code = _call(logits, plan, targets, top, r)
     else:
         with _lib.on_device(dev):
-            code = _call(logits, plan, targets, top, buf.data_ptr())
+            code = _call(logits, plan, targets, top, r)
     if code:
         _lib.check(code, "qi_token_logprobs")
     return r
 
 
-def _call(logits: torch.Tensor, plan: tuple, targets: torch.Tensor | None, top: int, out: int) -> int:
+def _call(logits: torch.Tensor, plan: tuple, targets: torch.Tensor | None, top: int, r: TokenLogprobs) -> int:
     M, V, dtype, ld, nbytes = plan
     dev = logits.device
     stream = torch._C._cuda_getCurrentRawStream(dev.index)
     data, counters, _keep = _lib.scratch(dev, stream, nbytes, _lib.LOGPROBS_COUNTERS)
     y, wide = (None, 0) if targets is None else (targets.data_ptr(), targets.dtype is torch.int64)
-    return _lib.lib().qi_token_logprobs(logits.data_ptr(), dtype, ld, y, wide, M, V, top, y and out, out + 4 * M,
-                                        out + 8 * M, out + 8 * M + 4 * M * top, data, nbytes, counters, stream)
+    return _lib.lib().qi_token_logprobs(
+        logits.data_ptr(), dtype, ld, y, wide, M, V, top, y and r.logprob.data_ptr(), r.entropy.data_ptr(),
+        r.top_ids.data_ptr() if top else None, r.top_logprobs.data_ptr() if top else None, data, nbytes, counters, stream)
 
 
 _INTS = (torch.int32, torch.int64)
