@@ -225,8 +225,8 @@ class KVCache:
                 b.value)
 
     # storage management hooks of the paged cache (every slot of a packed row exists)
-    def reserve(self, row: int, length: int) -> None:
-        """Make positions [0, length) of `row` writable (no-op for packed rows)."""
+    def reserve(self, row: int, length: int, start: int = 0) -> None:
+        """Make positions [start, length) of `row` writable (no-op for packed rows)."""
 
     def release(self, row: int) -> None:
         """The row's request is gone (no-op for packed rows)."""
@@ -298,8 +298,9 @@ class PagedKVCache(KVCache):
                                      pin_memory=dev.type == "cuda")
         self.table = self.table_host.to(dev)
         self._t = self.table_host.numpy()
-        self.mapped = np.zeros(max_batch, dtype=np.int64)   # pages mapped per row (a prefix)
-        self.trimmed = np.zeros(max_batch, dtype=np.int64)  # of them, looked at by `trim`
+        # by row: pages mapped (a prefix, less what `trim` gave back), of them those that `trim` has
+        # looked at, and the furthest position that it was told of
+        self.mapped, self.trimmed, self.trim_at = (np.zeros(max_batch, dtype=np.int64) for _ in range(3))
         self.free = list(range(self.n_pages - 1, -1, -1))   # stack of free page ids
         self.dirty = False
         self._native = None
@@ -329,16 +330,32 @@ class PagedKVCache(KVCache):
         self.sync()
         return super().attend(layer, q, rows, pos, window, sinks, query_run, out, tiles)
 
-    def reserve(self, row: int, length: int) -> None:
-        if not 0 <= row < self.max_batch or not 0 <= length <= self.max_len:
-            raise IndexError(f"row {row} / length {length} outside the cache")
-        need = -(-length // self.page_size)
-        while self.mapped[row] < need:
-            if not self.free:
-                raise RuntimeError(f"KV page pool of {self.n_pages} pages exhausted")
-            self._t[row, self.mapped[row]] = self.free.pop()
-            self.mapped[row] += 1
-            self.dirty = True
+    def reserve(self, row: int, length: int, start: int = 0) -> None:
+        """Map the pages of positions [start, length), `start` being the first position about
+        to be written: 0 for a text that begins, the row's length for one that goes on. Pages
+        that `trim` has given back are mapped again from `start` on (a text that begins gives
+        back the others of such a row too); raises if a query at `start` would see positions
+        that went back."""
+        if not 0 <= row < self.max_batch or not 0 <= start <= length <= self.max_len:
+            raise IndexError(f"row {row} / positions [{start}, {length}) outside the cache")
+        if start == 0 and self.trim_at[row]:
+            self.release(row)
+        size, need, mapped = self.page_size, -(-length // self.page_size), int(self.mapped[row])
+        first = start // size
+        if start < self.trim_at[row]:  # pages seen from `start` on and not written (else all of them are there)
+            seen = ((0, -(-min(self.attn_sinks, start) // size)),
+                    (max(0, start - self.attn_window + 1) // size, -(-start // size)))
+            if any((self._t[row, a:min(b, mapped)] < 0).any() for a, b in seen):
+                raise RuntimeError(f"row {row} cannot go on at position {start}: positions before it that are seen "
+                                   f"from there went back behind the window")
+            self.trimmed[row] = min(int(self.trimmed[row]), first)
+        for j in range(min(first, mapped), need):
+            if self._t[row, j] < 0:
+                if not self.free:
+                    raise RuntimeError(f"KV page pool of {self.n_pages} pages exhausted")
+                self._t[row, j] = self.free.pop()
+                self.dirty = True
+            self.mapped[row] = max(int(self.mapped[row]), j + 1)
 
     def release(self, row: int) -> None:
         for j in range(int(self.mapped[row]) - 1, -1, -1):
@@ -347,13 +364,15 @@ class PagedKVCache(KVCache):
             self._t[row, j] = -1
         if self.mapped[row]:
             self.dirty = True
-        self.mapped[row] = self.trimmed[row] = 0
+        self.mapped[row] = self.trimmed[row] = self.trim_at[row] = 0
 
     def trim(self, row: int, length: int) -> None:
         """With a window, return the pages that no query at position `length` or later sees:
-        those that end before its window and hold no first tokens."""
+        those that end before its window and hold no first tokens. (`reserve` maps them again
+        for a text that begins anew.)"""
         if not self.attn_window:
             return
+        self.trim_at[row] = max(int(self.trim_at[row]), length)
         end = min(max(0, length - self.attn_window + 1) // self.page_size, int(self.mapped[row]))
         for j in range(int(self.trimmed[row]), end):
             if j * self.page_size >= self.attn_sinks and self._t[row, j] >= 0:
@@ -369,9 +388,9 @@ class PagedKVCache(KVCache):
             return
         self.release(dst)
         self._t[dst] = self._t[src]
-        self.mapped[dst], self.trimmed[dst] = self.mapped[src], self.trimmed[src]
         self._t[src] = -1
-        self.mapped[src] = self.trimmed[src] = 0
+        for n in (self.mapped, self.trimmed, self.trim_at):
+            n[dst], n[src] = n[src], 0
         self.dirty = True
 
     def move_rows(self, moves: list[tuple[int, int, int]]) -> None:

@@ -203,7 +203,7 @@ class DecodeRunner:
         if self.paged:
             for b, q in enumerate(pos):
                 self.cache.trim(row_start + b, int(q))
-                self.cache.reserve(row_start + b, int(q) + 1)
+                self.cache.reserve(row_start + b, int(q) + 1, int(q))
             # page-table changes go out before the step, graph replays included (nothing is
             # left to copy when a graph is captured, so no copy is recorded into it)
             self.cache.sync()
@@ -239,7 +239,7 @@ class DecodeRunner:
         self._check_ids(toks)
         if self.paged:
             for b, q in enumerate(pos):
-                self.cache.reserve(row_start + b, int(q) + 1)
+                self.cache.reserve(row_start + b, int(q) + 1, int(q))
             self.cache.sync()
         self.dec.put(toks, pos, np.arange(row_start, row_start + B))
         self.ws.plan(B, 1)

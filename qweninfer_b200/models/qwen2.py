@@ -509,9 +509,9 @@ class Qwen2(nn.Module):
             # a paged cache maps the pages of the positions this forward writes and reads
             if positions.device.type != "cpu":
                 raise ValueError("a paged KV cache needs the positions on the host")
-            last = positions.reshape(B, S).max(dim=1).values
+            first, last = positions.reshape(B, S).aminmax(dim=1)
             for b in range(B):
-                cache.reserve(cache.row_start + b, int(last[b]) + 1)
+                cache.reserve(cache.row_start + b, int(last[b]) + 1, int(first[b]))
             cache.sync()
         ids32 = input_ids.reshape(M).to(device=dev, dtype=torch.int32, non_blocking=True).contiguous()
         pos32 = positions.reshape(M).to(device=dev, dtype=torch.int32, non_blocking=True).contiguous()
