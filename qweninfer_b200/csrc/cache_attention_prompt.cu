@@ -29,7 +29,10 @@
 // Every format is multiplied in fp16 with a scale for 16 keys: 8-bit codes are exact and
 // have their block's scale; bf16 values get a power of two that puts the largest of 16 keys
 // in [2^14, 2^15), which leaves all within 2^-28 of it exact and the others off by less than
-// that. q is scaled per row to a maximum in [1, 2). fp32 callers: q and p in two fp16
+// that. Where that is too coarse for one of the 16 (its own largest value more than 2^kSpread below;
+// the large one may be masked for a row, or have no weight), each key gets a scale of its own, and
+// the softmax applies them key by key: a row's result does not depend on what the keys beside its own
+// hold. q is scaled per row to a maximum in [1, 2). fp32 callers: q and p in two fp16
 // parts (22 bits), each part one UMMA chain into the same accumulator, the small ones first.
 // 16-bit callers: one part, exact for q (to 2^-25 of the row's largest) and good to 2^-12 for
 // p, below the output's own rounding.
@@ -66,6 +69,10 @@ constexpr int kRows = 128;   // query rows of a tile
 constexpr int kKeys = 128;   // keys of a tile
 constexpr float kLift = 14.f;
 constexpr uint32_t kMag = 0x7fff7fffu;  // magnitudes of a bf16 pair
+// Exponents that the largest values of 16 bf16 keys may lie apart under one scale: all of the smallest
+// key's are then known to 2^-22 of its largest. (4000 tokens, window 1024, head_dim 64, fp32 queries:
+// 120.6 us where none lies further apart, 119.0 without looking; 241 with such keys in every tile.)
+constexpr uint32_t kSpread = 7;
 constexpr unsigned kAll = 0xffffffffu;
 
 struct True {
@@ -112,6 +119,10 @@ struct Misc {
   // of 16 keys, by stage: K scale, exponent and significand of the V scale (s = 2^e * f; a
   // scale that is not finite has f = NaN)
   float ks[2][8], ve[2][8], vf[2][8];
+  // bf16 layers: whether the 16 keys have scales of their own, of K (bit 0) and V (bit 1); then K scale
+  // and exponent of the V scale of each
+  __align__(4) uint8_t wide[2][8];
+  __align__(16) float kk[2][kKeys], vk[2][kKeys];
   int k0[2], sg[2];  // first position and segment of the stage's keys
   float2 pair[2][2][2 * kRows];  // what the two threads of a row tell each other, by turns
   float2 ml[2 * kRows];       // maximum and sum of the rows' partials
@@ -288,6 +299,64 @@ __device__ __noinline__ void plain_row(const CacheAttnParams& p, const Seg& sg, 
         for (int d = 0; d < D / 2; ++d) o[d] = fmaf(w, bf16_to_f32(v[d0 + d]), o[d]);
     }
   }
+}
+
+// The two passes of the softmax over a thread's 64 scores where some of the keys have scales of their
+// own (`wide`: Misc's bytes); bit j of `seen`: key j is seen. Out of line: rare, and the registers of the
+// passes without them stay as they are.
+struct KeyScales {
+  const float *k, *v;
+  int ks, vs;  // steps from key to key
+  __device__ __forceinline__ KeyScales(const Misc& X, int st, int hf, uint32_t wide, int c) {
+    const uint32_t w = wide >> (8 * c);
+    ks = w & 1u, vs = (w >> 1) & 1u;
+    k = ks ? &X.kk[st][64 * hf + 16 * c] : &X.ks[st][4 * hf + c];
+    v = vs ? &X.vk[st][64 * hf + 16 * c] : &X.ve[st][4 * hf + c];
+  }
+};
+// The maxima of the scores and of score + exponent of the V scale.
+__device__ __noinline__ float2 key_maxima(const Misc& X, int st, int hf, uint32_t wide, uint32_t srow, uint64_t seen, float qs) {
+  float mx = -INFINITY, R = -INFINITY;
+  tmem_each16<4>(srow, [&](int c, const uint32_t(&s)[16]) {
+    const KeyScales y(X, st, hf, wide, c);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float x = (seen >> (16 * c + j)) & 1u ? __uint_as_float(s[j]) * (qs * y.k[j * y.ks]) : -INFINITY;
+      R = fmaxf(R, x + y.v[j * y.vs]);
+      mx = fmaxf(mx, x);
+    }
+  });
+  return make_float2(mx, R);
+}
+// P into the place of the scores; returns the weights' sum.
+template <int PARTS>
+__device__ __noinline__ float key_weights(const Misc& X, int st, int hf, uint32_t wide, uint32_t srow, uint64_t seen, float qs,
+                                          float mr, float rest) {
+  float sum[2] = {0.f, 0.f};
+  tmem_each16<4>(srow, [&](int c, const uint32_t(&s)[16]) {
+    const KeyScales y(X, st, hf, wide, c);
+    uint32_t part[PARTS][8];
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      float u[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool in = (seen >> (16 * c + j + i)) & 1u;
+        const float x = fmaf(__uint_as_float(s[j + i]), qs * y.k[(j + i) * y.ks], -mr);
+        sum[i] += in ? ex2(x) : 0.f;
+        // (not as weight times factor: a weight that underflows may have the largest product)
+        u[i] = in ? ex2(x + (y.v[(j + i) * y.vs] + rest)) : 0.f;
+      }
+      uint32_t h[PARTS];
+      split<true, PARTS>(u[0], u[1], h);
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) part[q][j / 2] = h[q];
+    }
+    // the 16 columns of S are read: their P takes them
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) tmem_put8(srow + 16 * c + 8 * q, part[q]);
+  });
+  return sum[0] + sum[1];
 }
 
 // the same shared memory of CTA w of the cluster (of C CTAs)
@@ -561,62 +630,84 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         *reinterpret_cast<uint4*>(t + core<D>(r, 2 * ch + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
     };
-    // bf16 values -> fp16 operand rows, and the scales of the warp's blocks of 16 keys
-    auto store16 = [&](const uint4* regs, uint8_t* t, int st, bool k_side) {
-      constexpr int kBlocks = 8 / H::kLoadWarps, kB = kN / kBlocks;  // blocks of the warp, chunks of a block
+    // bf16 values -> fp16 operand rows, and the scales of the warp's 16 keys, or of each of them
+    // (returned: whether they are wide)
+    auto store16 = [&](const uint4* regs, uint8_t* t, int st, bool k_side) -> bool {
+      static_assert(!BF || H::kLoadWarps == 8, "a warp has 16 keys");
+      constexpr int kHalf = kN / 2;  // chunks of the thread's keys lane & 7 and 8 + (lane & 7)
+      // Largest magnitudes of the two keys' chunks here (of the low and the high halves, then of both):
+      // where every lane's lie within the spread, all keys do; else the lanes that have the keys' other
+      // chunks are asked.
+      uint32_t m2[2] = {0u, 0u};
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        uint32_t m2 = 0u;  // largest magnitudes of the low and the high halves
+      for (int j = 0; j < kN; ++j) {
+        uint32_t& m = m2[j / kHalf];
+        m = __vmaxu2(__vmaxu2(m, __vmaxu2(regs[j].x & kMag, regs[j].y & kMag)),
+                     __vmaxu2(regs[j].z & kMag, regs[j].w & kMag));
+      }
+      uint32_t k0 = max(m2[0] >> 16, m2[0] & 0xffffu), k1 = max(m2[1] >> 16, m2[1] & 0xffffu);
+      // the exponent e of a largest value 2^(e - 127) * [1, 2), whose scale is 2^(e - 127 - 14): in
+      // 15..253 (the scale and its reciprocal are normal); tiny keys are left with a smaller maximum
+      auto exponent = [](uint32_t m) { return min(max(m >> 7, 15u), 253u); };
+      uint32_t mx = __reduce_max_sync(kAll, max(k0, k1)), e = exponent(mx);
+      bool wide = false;
+      if (!__any_sync(kAll, mx >= 0x7f80u || e < 29u || exponent(min(k0, k1)) + kSpread < e)) {
+        // bf16 to fp16 at that scale: the exponent field moves by e - 29 (from e to 29, that
+        // of 2^14) and the significand gains three zeros; values below fp16's normal range, 2^-28
+        // of the largest, come out off by less than that. Both halves at once: neither borrows
+        // nor overflows.
+        const uint32_t off2 = ((e - 29u) << 7) * 0x10001u;
+        auto half2_of = [&](uint32_t w) -> uint32_t { return ((__vmaxu2(w & kMag, off2) - off2) << 3) | (w & ~kMag); };
 #pragma unroll
-        for (int j = b * kB; j < (b + 1) * kB; ++j)
-          m2 = __vmaxu2(__vmaxu2(m2, __vmaxu2(regs[j].x & kMag, regs[j].y & kMag)),
-                        __vmaxu2(regs[j].z & kMag, regs[j].w & kMag));
-        uint32_t mx = __reduce_max_sync(kAll, max(m2 >> 16, m2 & 0xffffu));
-        const bool odd = mx >= 0x7f80u;  // infinities or NaN: the scale goes by the finite values
-        if (odd) {
-          mx = 0u;
+        for (int j = 0; j < kN; ++j) {
+          int r, ch;
+          place(j, r, ch);
+          *reinterpret_cast<uint4*>(t + core<D>(r, ch)) =
+              make_uint4(half2_of(regs[j].x), half2_of(regs[j].y), half2_of(regs[j].z), half2_of(regs[j].w));
+        }
+      } else {  // wide blocks, those with infinities or NaN (scaled by the finite values) and tiny ones: by way of fp32
+        if (mx >= 0x7f80u) {
+          k0 = k1 = 0u;
 #pragma unroll
-          for (int j = b * kB; j < (b + 1) * kB; ++j) {
+          for (int j = 0; j < kN; ++j) {
             const uint32_t w[4] = {regs[j].x, regs[j].y, regs[j].z, regs[j].w};
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const uint32_t lo = w[x] & 0x7fffu, hi = (w[x] >> 16) & 0x7fffu;
-              mx = max(mx, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+              uint32_t& m = j < kHalf ? k0 : k1;
+              m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
             }
           }
-          mx = __reduce_max_sync(kAll, mx);
         }
-        // largest value 2^(e - 127) * [1, 2): scale 2^(e - 127 - 14), for e in 15..253 (the
-        // scale and its reciprocal are normal); tiny blocks are left with a smaller maximum
-        const uint32_t e = min(max(mx >> 7, 15u), 253u);
-        if (lane == 0) {
-          if (k_side) X.ks[st][lw * kBlocks + b] = __uint_as_float((e - 14u) << 23);
-          else X.ve[st][lw * kBlocks + b] = (float)((int)e - 141), X.vf[st][lw * kBlocks + b] = 1.f;
+        uint32_t km = k0 | k1 << 16;
+        km = __vmaxu2(km, __shfl_xor_sync(kAll, km, 8));
+        km = __vmaxu2(km, __shfl_xor_sync(kAll, km, 16));
+        k0 = km & 0xffffu, k1 = km >> 16;
+        e = exponent(__reduce_max_sync(kAll, max(k0, k1)));
+        wide = __any_sync(kAll, (k0 != 0u && exponent(k0) + kSpread < e) || (k1 != 0u && exponent(k1) + kSpread < e));
+        const uint32_t e0 = wide ? exponent(k0) : e, e1 = wide ? exponent(k1) : e;
+        if (wide && lane < 8) {
+          const int i = lw * 16 + lane;
+          if (k_side) X.kk[st][i] = __uint_as_float((e0 - 14u) << 23), X.kk[st][i + 8] = __uint_as_float((e1 - 14u) << 23);
+          else X.vk[st][i] = (float)((int)e0 - 141), X.vk[st][i + 8] = (float)((int)e1 - 141);
         }
-        // bf16 to fp16 at that scale: the exponent field moves by e - 29 (from e to 29, that
-        // of 2^14) and the significand gains three zeros; values below fp16's normal range, 2^-28
-        // of the largest, come out off by less than that. Both halves at once: neither borrows
-        // nor overflows. (Blocks with infinities or NaN, and tiny ones, whose exponent is below
-        // 29, go through fp32.)
-        const uint32_t off2 = ((e - 29u) << 7) * 0x10001u;
-        auto half2_of = [&](uint32_t w) -> uint32_t { return ((__vmaxu2(w & kMag, off2) - off2) << 3) | (w & ~kMag); };
 #pragma unroll
-        for (int j = b * kB; j < (b + 1) * kB; ++j) {
+        for (int j = 0; j < kN; ++j) {
           int r, ch;
           place(j, r, ch);
+          const float inv = __uint_as_float((268u - (j < kHalf ? e0 : e1)) << 23);
           const uint32_t w[4] = {regs[j].x, regs[j].y, regs[j].z, regs[j].w};
           uint32_t h[4];
-          if (odd || e < 29u) {
-            const float inv = __uint_as_float((268u - e) << 23);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) h[x] = f16x2(bf16lo(w[x]) * inv, bf16hi(w[x]) * inv);
-          } else {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) h[x] = half2_of(w[x]);
-          }
+          for (int x = 0; x < 4; ++x) h[x] = f16x2(bf16lo(w[x]) * inv, bf16hi(w[x]) * inv);
           *reinterpret_cast<uint4*>(t + core<D>(r, ch)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
       }
+      if (lane == 0) {
+        if (k_side) X.ks[st][lw] = __uint_as_float((e - 14u) << 23);
+        else X.ve[st][lw] = (float)((int)e - 141), X.vf[st][lw] = 1.f;
+      }
+      return wide;
     };
     auto publish = [&](uint64_t* bar) {
       fence_async_smem();
@@ -636,10 +727,11 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       }
       if (lt == 0) X.k0[st] = first_key, X.sg[st] = si;
       if constexpr (BF) {
-        store16(kr, kt, st, true);
+        const bool wide_k = store16(kr, kt, st, true);
         publish(&X.k_full[st]);
         if constexpr (!kBoth) fetch(tbeg + i, false);
-        store16(kBoth ? vr : kr, vt, st, false);
+        const bool wide_v = store16(kBoth ? vr : kr, vt, st, false);
+        if (lane == 0) X.wide[st][lw] = (uint8_t)((wide_k ? 1 : 0) | (wide_v ? 2 : 0));
         publish(&X.v_full[st]);
       } else {
         if (lt < 8) X.ks[st][lt] = sc;
@@ -740,9 +832,15 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         auto below = [](int x) { return x <= 0 ? 0u : x >= 16 ? 0xffffu : (1u << x) - 1u; };
         return (below(b + 1 - c0) & ~below(a - c0)) | below(s0 - c0);
       };
+      auto seen64 = [&]() -> uint64_t {
+        uint64_t m = 0ull;
+        for (int c = 3; c >= 0; --c) m = m << 16 | mask16(64 * hf + 16 * c);
+        return m;
+      };
       float ks[4], ve[4];  // of this half's 4 blocks
 #pragma unroll
       for (int c = 0; c < 4; ++c) ks[c] = qs * X.ks[st][4 * hf + c], ve[c] = X.ve[st][4 * hf + c];
+      const uint32_t wide = BF ? *reinterpret_cast<const uint32_t*>(&X.wide[st][4 * hf]) : 0u;  // a byte for each
       wait(&X.s_full[buf], sph, X, p.err);
       tc_fence_after();
       const uint32_t srow = trow + 128 * buf + 64 * hf;  // this half's scores
@@ -765,7 +863,10 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
           mx = fmaxf(mx, v);
         });
       };
-      if (masked) maxima(True{});
+      if (wide) {
+        const float2 r = key_maxima(X, st, hf, wide, srow, seen64(), qs);
+        mx = r.x, R = r.y;
+      } else if (masked) maxima(True{});
       else maxima(False{});
       X.pair[st][hf][rr] = make_float2(mx, R);
       pair_bar();
@@ -781,8 +882,9 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       l *= oa;
       m = mn;
       const float mr = m == -INFINITY ? 0.f : m, Rr = R == -INFINITY ? 0.f : R;
-      ob = ex2(Rr - kLift - mr);
+      // (one rounded exponent both ways: what P is raised by, T is lowered by)
       const float rest = mr - Rr + kLift;
+      ob = ex2(-rest);
       // pass 2: weights and their parts
       f2 sum[2] = {0ull, 0ull};
       auto weights = [&](auto some_masked) {
@@ -817,7 +919,9 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
           for (int q = 0; q < PARTS; ++q) tmem_put8(srow + 16 * c + 8 * q, part[q]);
         });
       };
-      if (masked) weights(True{});
+      if (wide) {
+        l += key_weights<PARTS>(X, st, hf, wide, srow, seen64(), qs, mr, rest);
+      } else if (masked) weights(True{});
       else weights(False{});
       const float2 sum2 = unpack2(add2(sum[0], sum[1]));
       l += sum2.x + sum2.y;
