@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D>::kCtas) cache_attentio
   }
 
   float m = -INFINITY, l = 0.f, o[kOut];
+  bool far = false;  // a maximum of this warp's is beyond kFarScore
 #pragma unroll
   for (int i = 0; i < kOut; ++i) o[i] = 0.f;
 
@@ -337,6 +338,7 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D>::kCtas) cache_attentio
       const float mn = fmaxf(m, mx);
       const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
       m = mn;
+      far = __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) >= kFarScore);
       l *= alpha;
 #pragma unroll
       for (int d = 0; d < kOut; ++d) o[d] *= alpha;
@@ -345,9 +347,21 @@ __global__ void __launch_bounds__(kThreads, Shape<FMT, D>::kCtas) cache_attentio
     // second fp16 part of small ones above the subnormal range)
     const float mref = (F16 ? 12.f : 0.f) - (m == -INFINITY ? 0.f : m);
     uint32_t pa[2][kA][4];
+    if (far) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          sc[t][e] = __fmul_rn(sc[t][e], f[t]) - (m == -INFINITY ? 0.f : m) + (F16 ? 12.f : 0.f);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sc[t][e] = fmaf(sc[t][e], f[t], mref);
+    }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const float p0 = ex2(fmaf(sc[t][0], f[t], mref)), p1 = ex2(fmaf(sc[t][1], f[t], mref));
+      const float p0 = ex2(sc[t][0]), p1 = ex2(sc[t][1]);
       l += p0 + p1;
       uint32_t r[kParts];
       split<F16, kParts>(p0, p1, r);

@@ -10,6 +10,11 @@ namespace qi {
 namespace cattn {
 
 constexpr int kMaxGroup = 8;
+// Scores (log2 units) are subtracted from their maximum in the multiplication that scales them, whose
+// product is not rounded where the maximum is: all weights are off by one factor, which the
+// normalisation takes out again. From this size of the maximum on (a factor of 2^(1/4)) the factor
+// could leave the range of the weights: products are rounded before the subtraction.
+constexpr float kFarScore = 4194304.f;  // 2^22
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");

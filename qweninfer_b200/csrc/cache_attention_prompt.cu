@@ -52,7 +52,8 @@
 // What masked keys hold must not reach a row. Scores are replaced, keys that no row of the
 // tile sees are zero-filled; but in P V a zero weight times a NaN or infinity that another
 // row does see would be NaN. A row that ends up not finite is therefore computed again, key
-// by key (8-bit codes are always finite: only the bf16 cache needs it).
+// by key (8-bit codes are always finite: only the bf16 cache needs it), and so is one whose scores
+// are as far from 0 as kFarScore says.
 #include <atomic>
 
 #include "cache_attention.cuh"
@@ -71,7 +72,7 @@ constexpr float kLift = 14.f;
 constexpr uint32_t kMag = 0x7fff7fffu;  // magnitudes of a bf16 pair
 // Exponents that the largest values of 16 bf16 keys may lie apart under one scale: all of the smallest
 // key's are then known to 2^-22 of its largest. (4000 tokens, window 1024, head_dim 64, fp32 queries:
-// 120.6 us where none lies further apart, 119.0 without looking; 241 with such keys in every tile.)
+// 113 us where none lies further apart, 236 with such keys in every tile.)
 constexpr uint32_t kSpread = 7;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -266,27 +267,38 @@ __device__ __forceinline__ float load_q(const CacheAttnParams& p, long long i) {
   return p.dtype == QI_F32 ? load_elem<QI_F32>(p.q, i) : p.dtype == QI_BF16 ? load_elem<QI_BF16>(p.q, i) : load_elem<QI_F16>(p.q, i);
 }
 
-// Key by key: the partial of token t's head over the given tiles of its segment (bf16
-// layers), dims d0 .. d0 + D / 2 - 1 of the output. The weights of masked keys are left out, not multiplied by zero.
-template <int D>
-__device__ __noinline__ void plain_row(const CacheAttnParams& p, const Seg& sg, int tbeg, int tend, int tok, int head, int g,
-                                       int ps, int d0, float& m, float& l, float* o) {
+// Key by key: the partial of token t's head over the given tiles of its segment, dims d0 .. d0 + D / 2 - 1 of
+// the output into o (shared memory); returns its maximum and sum. The weights of masked keys are left out, not
+// multiplied by zero.
+template <int FMT, int D>
+__device__ __noinline__ float2 plain_row(const CacheAttnParams& p, const Seg& sg, int tbeg, int tend, int tok, int head, int g,
+                                         int ps, int d0, float* o) {
+  auto value = [](const void* x, long long i) -> float {
+    if constexpr (FMT == QI_KV_BF16) return bf16_to_f32(static_cast<const uint16_t*>(x)[i]);
+    else return decode<FMT>(static_cast<const uint8_t*>(x)[i]);
+  };
   const Seen<kKeys> list = seen_range<kKeys>(sg.hi, sg.lo, sg.sinks);
   const Seen<kKeys> mine = seen_range<kKeys>(ps, window_start(ps, p.window), p.sinks);
   const long long qo = (long long)tok * p.q_st + (long long)head * p.q_sh;
-  m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f;
   for (int d = 0; d < D / 2; ++d) o[d] = 0.f;
   for (int i = tbeg; i < tend; ++i) {
     const int k0 = list.granule(i) * kKeys;
     const long long base = layer_offset(p.c, D, sg.row, g, k0);
     for (int j = 0; j < kKeys; ++j) {
       if (!mine.sees(k0 + j)) continue;
-      float s = 0.f;
-      const uint16_t* k = static_cast<const uint16_t*>(p.c.k) + (base < 0 ? 0 : base) + j * D;
-      const uint16_t* v = static_cast<const uint16_t*>(p.c.v) + (base < 0 ? 0 : base) + j * D;
-      if (base >= 0)
-        for (int d = 0; d < D; ++d) s = fmaf(load_q(p, qo + d), bf16_to_f32(k[d]), s);
-      s *= p.scale_log2;
+      float s = 0.f, fv = 0.f;
+      const long long at = base + j * D;
+      if (base >= 0) {
+        float fk = 1.f;
+        fv = 1.f;
+        if constexpr (FMT != QI_KV_BF16) {
+          const long long si = scale_index(p.c, sg.row, g, k0 + j);
+          fk = __ldg(p.c.k_scale + si), fv = __ldg(p.c.v_scale + si);
+        }
+        for (int d = 0; d < D; ++d) s = fmaf(load_q(p, qo + d), value(p.c.k, at + d) * fk, s);
+      }
+      s = __fmul_rn(s, p.scale_log2);  // rounded, as the maximum is
       if (s > m) {
         const float a = m == -INFINITY ? 0.f : ex2(m - s);
         l *= a;
@@ -296,9 +308,10 @@ __device__ __noinline__ void plain_row(const CacheAttnParams& p, const Seg& sg, 
       const float w = ex2(s - (m == -INFINITY ? 0.f : m));
       l += w;
       if (base >= 0)
-        for (int d = 0; d < D / 2; ++d) o[d] = fmaf(w, bf16_to_f32(v[d0 + d]), o[d]);
+        for (int d = 0; d < D / 2; ++d) o[d] = fmaf(w, value(p.c.v, at + d0 + d) * fv, o[d]);
     }
   }
+  return make_float2(m, l);
 }
 
 // The two passes of the softmax over a thread's 64 scores where some of the keys have scales of their
@@ -358,7 +371,6 @@ __device__ __noinline__ float key_weights(const Misc& X, int st, int hf, uint32_
   });
   return sum[0] + sum[1];
 }
-
 // the same shared memory of CTA w of the cluster (of C CTAs)
 __device__ __forceinline__ float peer(const float* x, int w, int C) {
   if (C == 1) return *x;
@@ -386,7 +398,7 @@ __device__ __forceinline__ void fewer_regs() {
 }
 
 template <int FMT, int D, int PARTS>
-__global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kernel(const __grid_constant__ CacheAttnParams p) {
   using H = Shape<FMT, D, PARTS>;
   constexpr bool BF = FMT == QI_KV_BF16;
   constexpr int kPitch = D + 4;  // floats of a row of partial outputs
@@ -797,6 +809,7 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
     const uint32_t orow = trow + H::kColT + D * qt + DH * hf;  // and dims
 
     float m = -INFINITY, l = 0.f;  // maximum of the scores (log2 units), sum of 2^(x - m)
+    float size = 0.f;              // the largest that |m| was
     f2 o[DH / 2];                  // sum of 2^(x - m) v (this half's dims; l: this half's keys)
 #pragma unroll
     for (int d = 0; d < DH / 2; ++d) o[d] = 0ull;
@@ -885,6 +898,7 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       // (one rounded exponent both ways: what P is raised by, T is lowered by)
       const float rest = mr - Rr + kLift;
       ob = ex2(-rest);
+      size = fmaxf(size, fabsf(mr));
       // pass 2: weights and their parts
       f2 sum[2] = {0ull, 0ull};
       auto weights = [&](auto some_masked) {
@@ -947,7 +961,7 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       of[d] = live ? x.x : 0.f, of[d + 1] = live ? x.y : 0.f;
     }
     if (!live) m = -INFINITY, l = 0.f;
-    bool bad = false;
+    bool bad = size >= kFarScore;
     if constexpr (BF) {
 #pragma unroll
       for (int d = 0; d < DH; ++d) bad |= !(fabsf(of[d]) <= 3.402823466e38f);
@@ -957,19 +971,20 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
     pair_bar();
     const float2 other = X.pair[0][hf ^ 1][rr];
     l = hf ? other.x + l : l + other.x;
-    if constexpr (BF) {
-      if (row_in && live && (bad || other.y != 0.f)) {
-        const Seg sg = X.segs[seg];
-        const int end = sg.first + seen_range<kKeys>(sg.hi, sg.lo, sg.sinks).n;
-        plain_row<D>(p, sg, max(tbeg, sg.first) - sg.first, min(tend, end) - sg.first, t0 + tl, head, g, ps, hf * DH, m, l, of);
-      }
-    }
     // The split's partial (relative to m) into shared memory, in the place of Q and K, which
     // all products are done with: rows of D + 4 floats, so that rows 8 apart share a bank.
     wait(&X.done, 0u, X, p.err);
     float* po = reinterpret_cast<float*>(smem) + rr * kPitch + hf * DH;
+    if (row_in && live && (bad || other.y != 0.f)) {
+      const Seg sg = X.segs[seg];
+      const int end = sg.first + seen_range<kKeys>(sg.hi, sg.lo, sg.sinks).n;
+      const float2 y = plain_row<FMT, D>(p, sg, max(tbeg, sg.first) - sg.first, min(tend, end) - sg.first, t0 + tl, head, g, ps,
+                                         hf * DH, po);
+      m = y.x, l = y.y;
+    } else {
 #pragma unroll
-    for (int d = 0; d < DH; d += 4) *reinterpret_cast<float4*>(po + d) = make_float4(of[d], of[d + 1], of[d + 2], of[d + 3]);
+      for (int d = 0; d < DH; d += 4) *reinterpret_cast<float4*>(po + d) = make_float4(of[d], of[d + 1], of[d + 2], of[d + 3]);
+    }
     if (hf == 0) X.ml[rr] = make_float2(m, l);
     tc_fence_before();
     __syncthreads();
