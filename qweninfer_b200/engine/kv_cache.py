@@ -294,9 +294,10 @@ class PagedKVCache(KVCache):
         self.row_start = 0
         self.attn_window, self.attn_sinks = _window(attn_window, attn_sinks)
         dev = torch.device(device)
-        self.table_host = torch.full((max_batch, self.pages_per_row), -1, dtype=torch.int32,
-                                     pin_memory=dev.type == "cuda")
+        self.table_host = torch.full((max_batch, self.pages_per_row), -1, dtype=torch.int32)
         self.table = self.table_host.to(dev)
+        self._published: torch.cuda.Event | None = None  # the last copy to the device
+        self._ordered: set[int] = set()                  # streams whose work comes behind it
         self._t = self.table_host.numpy()
         # by row: pages mapped (a prefix, less what `trim` gave back), of them those that `trim` has
         # looked at, and the furthest position that it was told of
@@ -398,9 +399,37 @@ class PagedKVCache(KVCache):
             self.move_row(src, dst, length)
 
     def sync(self) -> None:
-        if self.dirty:
-            self.table.copy_(self.table_host, non_blocking=True)
-            self.dirty = False
+        """Publish page-table changes to the device, before the call that reads them. The copy is
+        enqueued on the current stream, out of memory of its own (the host goes on changing
+        the table), and calls on other streams wait for it. A call that is being captured
+        cannot publish: `sync` is called before the capture, and before a replay that
+        follows changes."""
+        dev = self.table.device
+        if dev.type != "cuda":
+            if self.dirty:
+                self.table.copy_(self.table_host)
+                self.dirty = False
+            return
+        stream = torch._C._cuda_getCurrentRawStream(dev.index)
+        if not self.dirty and (self._published is None or stream in self._ordered):
+            return
+        with torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                if self.dirty:
+                    raise _lib.QiError("page-table changes cannot be published while a graph is being captured: "
+                                       "call sync() before")
+                return  # (what is captured runs when it is replayed)
+            if self.dirty:
+                if self._published is not None and stream not in self._ordered:
+                    torch.cuda.current_stream().wait_event(self._published)  # copies arrive in their order
+                self.table.copy_(self.table_host.pin_memory(), non_blocking=True)
+                self.dirty = False
+                self._published = torch.cuda.Event()
+                self._published.record()
+                self._ordered = {stream}
+            else:
+                torch.cuda.current_stream().wait_event(self._published)
+                self._ordered.add(stream)
 
     def pages_in_use(self) -> int:
         return self.n_pages - len(self.free)
