@@ -72,9 +72,10 @@ __device__ __forceinline__ uint32_t f32_order_key(float f) {
 }
 
 // Argmax slot: (value key << 32) | (0xffffffff - index). atomicMax keeps the largest
-// value and, among equal values, the lowest index (torch.argmax's first-maximum rule).
+// value and, among equal values, the lowest index (torch.argmax's first-maximum rule). Zeros of
+// either sign are equal: + 0 makes them +0 and leaves every other value as it is.
 __device__ __forceinline__ unsigned long long argmax_pack(float v, int idx) {
-  return ((unsigned long long)f32_order_key(v) << 32) | (unsigned long long)(0xffffffffu - (uint32_t)idx);
+  return ((unsigned long long)f32_order_key(__fadd_rn(v, 0.f)) << 32) | (unsigned long long)(0xffffffffu - (uint32_t)idx);
 }
 
 // ------------------------------------------------------------ PTX wrappers
