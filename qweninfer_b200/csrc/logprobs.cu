@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
           }
           if constexpr (TOP) {
             const int step = (k - k0) * kSteps + j0;
-            if (step == 0) first_bound = __shfl_sync(kAll, sort_lanes(m, lane), p.top - 1);
+            // (a step of nothing but NaN has no say: sorted, it would pass another lane's maximum on twice)
+            if (step == 0) first_bound = __shfl_sync(kAll, sort_lanes(m == m ? m : -INFINITY, lane), p.top - 1);
             hot |= (m >= first_bound ? 1u : 0u) << (step & 31);
           }
         }

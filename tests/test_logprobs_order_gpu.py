@@ -31,3 +31,27 @@ def test_zeros_of_either_sign_are_equal(dtype, V):
         r = token_logprobs(x, None, top)
         assert torch.equal(r.top_ids.long(), best(x, top))
         assert torch.equal(r.top_logprobs[0, 0], token_logprobs(x[:1] + 0.0, None, 1).top_logprobs[0, 0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [8, 200, 5000, 40000])
+def test_rows_that_begin_with_nan(dtype, n):
+    """Lanes whose first values are all NaN: the alternatives are those of the other values."""
+    V = 60000
+    g = torch.Generator("cuda").manual_seed(n)
+    x = torch.randn(5, V, generator=g, device="cuda")
+    x[0, :n] = torch.nan
+    x[1, torch.randperm(V, generator=g, device="cuda")[:n]] = torch.nan
+    x[2, :n] = torch.nan
+    x[2, n:] = x[2, n:].round()
+    for t in range(n // 256 + 1):  # 8 values of every 256
+        x[3, 256 * t:256 * t + 8] = torch.nan
+    x[4] = torch.nan
+    x[4, -3:] = torch.tensor([1.0, 2.0, 1.0])
+    x = x.to(dtype)
+    for top in (1, 7, 32):
+        r = token_logprobs(x, None, top)
+        want = best(x, top)
+        want[4, 3:] = -1
+        assert torch.equal(r.top_ids.long(), want), [int((a != b).sum()) for a, b in zip(r.top_ids.long(), want)]
+        assert r.entropy.isnan().all()
