@@ -34,8 +34,10 @@
 // the softmax applies them key by key: a row's result does not depend on what the keys beside its own
 // hold. q is scaled per row to a maximum in [1, 2). fp32 callers: q and p in two fp16
 // parts (22 bits), each part one UMMA chain into the same accumulator, the small ones first.
-// 16-bit callers: one part, exact for q (to 2^-25 of the row's largest) and good to 2^-12 for
-// p, below the output's own rounding.
+// 16-bit callers: q in one part, exact for it (to 2^-25 of the row's largest). p in two for fp16, whose
+// outputs have 11 bits themselves, and in one for bf16: off by 2^-11, an eighth of the output's own
+// rounding. (1024 tokens on 4096 keys, int8: 64 us in two parts, 55 in one, where the error of bf16 outputs
+// against 64 bits is 1.66e-3, as that of their rounding alone is.)
 //
 // The K scale multiplies scores, the V scale of a block its probabilities: P holds 2^(x_j +
 // log2 s_j - R + 14), where R is the largest x + log2 s of the row in the tile, so that what
@@ -83,7 +85,7 @@ struct False {
   static constexpr bool value = false;
 };
 
-template <int FMT, int D, int PARTS>
+template <int FMT, int D, int QP>
 struct Shape {
   static constexpr int kTiles = D == 64 ? 2 : 1;  // query tiles of a CTA
   // warpgroups: two of softmax for each tile, producers, and one whose first warp issues MMAs
@@ -91,7 +93,7 @@ struct Shape {
   static constexpr int kThreads = 32 * (kMmaWarp + 4);
   static constexpr uint32_t kQ = kRows * D * 2;   // one part of a tile's Q
   static constexpr uint32_t kT = kKeys * D * 2;   // K or V tile, two stages each
-  static constexpr uint32_t kOffK = kTiles * PARTS * kQ, kOffV = kOffK + 2 * kT, kOffMisc = kOffV + 2 * kT;
+  static constexpr uint32_t kOffK = kTiles * QP * kQ, kOffV = kOffK + 2 * kT, kOffMisc = kOffV + 2 * kT;
   // TMEM columns: three S (each with its P in its place) that the tiles take in turn, then T
   static constexpr uint32_t kColT = 3 * 128, kCols = 512;
   static_assert(kColT + kTiles * D <= kCols, "tensor memory");
@@ -397,9 +399,9 @@ __device__ __forceinline__ void fewer_regs() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-template <int FMT, int D, int PARTS>
-__global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kernel(const __grid_constant__ CacheAttnParams p) {
-  using H = Shape<FMT, D, PARTS>;
+template <int FMT, int D, int QP, int PP>
+__global__ void __launch_bounds__(Shape<FMT, D, QP>::kThreads, 1) prompt_kernel(const __grid_constant__ CacheAttnParams p) {
+  using H = Shape<FMT, D, QP>;
   constexpr bool BF = FMT == QI_KV_BF16;
   constexpr int kPitch = D + 4;  // floats of a row of partial outputs
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -422,14 +424,14 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
   grid_dep_launch();
   // Threads r and r + 128 of a tile's softmax warps: query row r = (token, head), half of
   // its dims (and 64 of a tile's keys). The loads overlap the setup.
-  constexpr int DH = D / 2, kRaw = DH / (PARTS == 2 ? 4 : 8);
+  constexpr int DH = D / 2, kRaw = DH / (QP == 2 ? 4 : 8);
   const int qt = tid >> 8, r = tid & (kRows - 1), hf = (tid >> 7) & 1;
   const int rr = qt * kRows + r;  // row of the CTA
   // its token of the CTA, none (ntok) for rows past the tile's last whole token
   const int tl = r / G < TT ? min(qt * TT + r / G, ntok) : ntok, head = g * G + r % G;
   uint4 raw[kRaw];
   if (warp < H::kSoftWarps)
-    load_row<kRaw, PARTS == 2>(p, (long long)(t0 + min(tl, ntok - 1)) * p.q_st + (long long)head * p.q_sh + hf * DH, raw);
+    load_row<kRaw, QP == 2>(p, (long long)(t0 + min(tl, ntok - 1)) * p.q_st + (long long)head * p.q_sh + hf * DH, raw);
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&X.k_full[s], H::kLoadWarps);
@@ -541,14 +543,14 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         const int i = x >> lg, t = x & lg;
         wait(&X.k_full[i & 1], (uint32_t)(i >> 1) & 1u, X, p.err);
         tc_fence_after();
-        const uint64_t qd = desc(sb + t * PARTS * H::kQ, 128, D * 16);
+        const uint64_t qd = desc(sb + t * QP * H::kQ, 128, D * 16);
         const uint64_t kd = desc(sb + H::kOffK + (i & 1) * H::kT, 128, D * 16);
 #pragma unroll
-        for (int q = PARTS - 1; q >= 0; --q)
+        for (int q = QP - 1; q >= 0; --q)
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
             umma_ss(lead, tmem + 128 * buf, qd + (uint64_t)(q * (H::kQ >> 4) + k * 16), kd + (uint64_t)(k * 16), id_s,
-                    q < PARTS - 1 || k > 0 ? 1u : 0u);
+                    q < QP - 1 || k > 0 ? 1u : 0u);
         commit(lead, &X.s_full[buf]);
         if (t == lg) commit(lead, &X.k_empty[i & 1]);
       };
@@ -563,12 +565,12 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
         tc_fence_after();
         const uint64_t vd = desc(sb + H::kOffV + st * H::kT, D * 16, 128);
 #pragma unroll
-        for (int q = PARTS - 1; q >= 0; --q)
+        for (int q = PP - 1; q >= 0; --q)
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
             // 16 keys: 8 columns of P for each part; 2 key groups of V
             umma_ts(lead, tmem + H::kColT + D * t, tmem + 128 * buf + 16 * k + 8 * q, vd + (uint64_t)(k * 2 * D), id_t,
-                    q < PARTS - 1 || k > 0 ? 1u : 0u);
+                    q < PP - 1 || k > 0 ? 1u : 0u);
         commit(lead, &X.t_full[t]);
         if (t == lg) commit(lead, &X.v_empty[st]);
         if (x + ahead < total) scores(x + ahead, buf + ahead >= 3 ? buf + ahead - 3 : buf + ahead);
@@ -776,7 +778,7 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       float am = 0.f;
 #pragma unroll
       for (int i = 0; i < DH / 2; ++i) {
-        const float2 x = row_pair<PARTS == 2>(raw, i, p.dtype);
+        const float2 x = row_pair<QP == 2>(raw, i, p.dtype);
         am = fmaxf(am, fmaxf(fabsf(x.x), fabsf(x.y)));
       }
       X.pair[1][hf][rr].x = am;
@@ -790,15 +792,15 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
       }
 #pragma unroll
       for (int ch = 0; ch < DH / 8; ++ch) {
-        uint32_t w[4][PARTS];
+        uint32_t w[4][QP];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 x = row_pair<PARTS == 2>(raw, 4 * ch + i, p.dtype);
-          split<true, PARTS>(live ? x.x * inv : 0.f, live ? x.y * inv : 0.f, w[i]);
+          const float2 x = row_pair<QP == 2>(raw, 4 * ch + i, p.dtype);
+          split<true, QP>(live ? x.x * inv : 0.f, live ? x.y * inv : 0.f, w[i]);
         }
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q)
-          *reinterpret_cast<uint4*>(smem + (qt * PARTS + q) * H::kQ + core<D>(r, hf * (DH / 8) + ch)) =
+        for (int q = 0; q < QP; ++q)
+          *reinterpret_cast<uint4*>(smem + (qt * QP + q) * H::kQ + core<D>(r, hf * (DH / 8) + ch)) =
               make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
       }
       fence_async_smem();
@@ -907,7 +909,7 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
           const float fv = X.vf[st][4 * hf + c] * ex2(fminf(ve[c] + rest, 126.f));
           const f2 fk2 = pack2(ks[c], ks[c]), fv2 = pack2(fv, fv), mr2 = pack2(-mr, -mr);
           const uint32_t mk = decltype(some_masked)::value ? mask16(64 * hf + 16 * c) : 0u;
-          uint32_t part[PARTS][8];
+          uint32_t part[PP][8];
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             const float2 x = unpack2(fma2(pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), fk2, mr2));
@@ -923,18 +925,18 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
               u.x = (mk >> j) & 1u ? u.x : 0.f;
               u.y = (mk >> (j + 1)) & 1u ? u.y : 0.f;
             }
-            uint32_t y[PARTS];
-            split<true, PARTS>(u.x, u.y, y);
+            uint32_t y[PP];
+            split<true, PP>(u.x, u.y, y);
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q) part[q][j / 2] = y[q];
+            for (int q = 0; q < PP; ++q) part[q][j / 2] = y[q];
           }
           // the block's 16 columns of S are read: its P takes them
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) tmem_put8(srow + 16 * c + 8 * q, part[q]);
+          for (int q = 0; q < PP; ++q) tmem_put8(srow + 16 * c + 8 * q, part[q]);
         });
       };
       if (wide) {
-        l += key_weights<PARTS>(X, st, hf, wide, srow, seen64(), qs, mr, rest);
+        l += key_weights<PP>(X, st, hf, wide, srow, seen64(), qs, mr, rest);
       } else if (masked) weights(True{});
       else weights(False{});
       const float2 sum2 = unpack2(add2(sum[0], sum[1]));
@@ -1034,10 +1036,10 @@ __global__ void __launch_bounds__(Shape<FMT, D, PARTS>::kThreads, 1) prompt_kern
   }
 }
 
-template <int FMT, int D, int PARTS>
+template <int FMT, int D, int QP, int PP>
 cudaError_t launch(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
-  using H = Shape<FMT, D, PARTS>;
-  auto kernel = prompt_kernel<FMT, D, PARTS>;
+  using H = Shape<FMT, D, QP>;
+  auto kernel = prompt_kernel<FMT, D, QP, PP>;
   constexpr int smem = H::kOffMisc + kMiscBytes;
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
@@ -1072,12 +1074,17 @@ cudaError_t launch(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+template <int FMT, int D>
+cudaError_t launch_parts(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
+  if (p.dtype == QI_F32) return launch<FMT, D, 2, 2>(p, s, pdl);
+  return p.dtype == QI_F16 ? launch<FMT, D, 1, 2>(p, s, pdl) : launch<FMT, D, 1, 1>(p, s, pdl);
+}
+
 template <int D>
 cudaError_t launch_dim(const CacheAttnParams& p, cudaStream_t s, bool pdl) {
-  const bool f32 = p.dtype == QI_F32;
-  if (p.c.format == QI_KV_INT8) return f32 ? launch<QI_KV_INT8, D, 2>(p, s, pdl) : launch<QI_KV_INT8, D, 1>(p, s, pdl);
-  if (p.c.format == QI_KV_E4M3) return f32 ? launch<QI_KV_E4M3, D, 2>(p, s, pdl) : launch<QI_KV_E4M3, D, 1>(p, s, pdl);
-  return f32 ? launch<QI_KV_BF16, D, 2>(p, s, pdl) : launch<QI_KV_BF16, D, 1>(p, s, pdl);
+  if (p.c.format == QI_KV_INT8) return launch_parts<QI_KV_INT8, D>(p, s, pdl);
+  if (p.c.format == QI_KV_E4M3) return launch_parts<QI_KV_E4M3, D>(p, s, pdl);
+  return launch_parts<QI_KV_BF16, D>(p, s, pdl);
 }
 
 }  // namespace
@@ -1094,7 +1101,7 @@ int prompt_clusters(int size) {
   if (n > 0) return n;
   // one CTA on an SM in every variant; this one stands for all
   using H = Shape<QI_KV_BF16, 128, 1>;
-  auto kernel = prompt_kernel<QI_KV_BF16, 128, 1>;
+  auto kernel = prompt_kernel<QI_KV_BF16, 128, 1, 1>;
   constexpr int smem = H::kOffMisc + kMiscBytes;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)size, 1, 1);

@@ -153,8 +153,9 @@ class KVCache:
         are as long as max_len allows. `tiles`: whatever the size. Returns (M, heads, head_dim) of q's dtype (`out`, if given:
         contiguous, 16-byte aligned and apart from q), enqueued on the current stream.
 
-        Scores, softmax and sums are fp32; q and the probabilities keep at least 22 bits for
-        an 8-bit cache, 24 (16 for 16-bit q) for a bf16 one."""
+        Scores, softmax and sums are fp32. q and the probabilities keep 22 bits over an 8-bit
+        cache and 24 (16 for 16-bit q) over a bf16 one where each token reads its own keys; in
+        tiles 22 bits over both, and 11 of the probabilities for bfloat16 q, whose outputs have 8."""
         # what the shapes alone decide is checked once for each kind of call
         key = (layer, q.shape, q.stride(), q.dtype, window, sinks, query_run, tiles)
         try:

@@ -133,3 +133,19 @@ def test_scores_far_from_zero(fmt, dim, tiles, size):
     q[:, 4:6] *= -1
     check(cache, k, v, q, 0, list(range(50, 200)), tiles=tiles)
     check(cache, k, v, q, 0, list(range(50, 200)), tiles=tiles, window=33, sinks=2)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tiles", [False, True])
+def test_half_precision_outputs_are_rounded_once(fmt, dim, tiles):
+    """fp16 callers: the error is the output's own rounding. Its norm, of the 64-bit result
+    rounded to fp16, is within 5 % the same for any result as near as 2^-18 (roundings are as good as random over
+    10^5 elements); what comes before it adds at most 2^-18 of the norm, the bar of fp32 callers."""
+    cache, vals = filled(fmt, 8, 2, dim, 1, 420, 49)
+    q = randn(gen(50), 200, 8, dim).to(torch.float16)
+    pos = list(range(220, 420))
+    got = cache.attend(0, q, i32([0] * 200), i32(pos), query_run=200 if tiles else 1, tiles=tiles)
+    out, _ = exact(q, *vals, 0, pos)
+    own = float((out.to(torch.float16).double() - out).norm())
+    assert float((got.double() - out).norm()) <= 1.05 * own + 2.0 ** -18 * float(out.norm())
