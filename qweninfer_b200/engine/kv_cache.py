@@ -67,6 +67,7 @@ class KVCache:
         self.window = 0
         self.row_start = 0
         self.attn_window, self.attn_sinks = _window(attn_window, attn_sinks)
+        self._err = torch.zeros(1, dtype=torch.int32, device=device)
         self._native: _lib.QiCache | None = None
 
     def native(self) -> _lib.QiCache:
@@ -92,11 +93,9 @@ class KVCache:
                               self.max_batch, self.k.shape[2], self.max_len, self.k.shape[-1], None, 0, 0, 0)
 
     def _errors(self) -> torch.Tensor:
-        try:
-            return self._err
-        except AttributeError:
-            self._err = torch.zeros(1, dtype=torch.int32, device=self.k.device)
-            return self._err
+        """The error word of `attend` and `append`. It is made with the cache: made by a call that
+        is being captured, it would lie in the graph's memory and be zeroed by each replay."""
+        return self._err
 
     def check(self) -> None:
         """Raise if an `attend` or `append` of this cache met a position, cache row or page
@@ -294,6 +293,7 @@ class PagedKVCache(KVCache):
         self.window = 0
         self.row_start = 0
         self.attn_window, self.attn_sinks = _window(attn_window, attn_sinks)
+        self._err = torch.zeros(1, dtype=torch.int32, device=device)
         dev = torch.device(device)
         self.table_host = torch.full((max_batch, self.pages_per_row), -1, dtype=torch.int32)
         self.table = self.table_host.to(dev)
@@ -581,6 +581,7 @@ class Kv8Cache(_Codes, KVCache):
         self.window = 0
         self.row_start = 0
         self.attn_window, self.attn_sinks = _window(attn_window, attn_sinks)
+        self._err = torch.zeros(1, dtype=torch.int32, device=device)
         self._native = None
 
     def move_rows(self, moves: list[tuple[int, int, int]]) -> None:
