@@ -527,6 +527,11 @@ class Qwen2(nn.Module):
     @torch.inference_mode()
     def forward(self, input_ids: torch.Tensor, positions: torch.Tensor | None = None, cache=None,
                 last_only: bool = False, logits_dtype: torch.dtype | None = None) -> torch.Tensor:
+        return self._forward(input_ids, positions, cache, last_only, logits_dtype)
+
+    @torch.inference_mode()
+    def _forward(self, input_ids, positions, cache, last_only, logits_dtype, ws: Workspace | None = None) -> torch.Tensor:
+        """`forward`, in a workspace of at least the call's tokens and the cache's length if given."""
         dev = self.device
         B, S = input_ids.shape
         cache, M, ids32, pos32, rows32 = self._inputs(input_ids, positions, cache)
@@ -537,7 +542,7 @@ class Qwen2(nn.Module):
         ldt = torch.bfloat16 if want == torch.bfloat16 else torch.float32
         logits = torch.empty(n_head, self.cfg.vocab_size, dtype=ldt, device=dev)
         slots = torch.zeros(M, dtype=torch.int64, device=dev)
-        ws = self.workspace(max(M, 1), cache.max_len).plan(M, S)
+        ws = (ws or self.workspace(max(M, 1), cache.max_len)).plan(M, S)
         _lib.check(_lib.lib().qi_forward(
             C.byref(self.native()), C.byref(cache.native()), C.byref(ws.struct), ids32.data_ptr(),
             pos32.data_ptr(), rows32.data_ptr(), M, head_lo, head_stride, n_head, logits.data_ptr(),
@@ -565,11 +570,14 @@ class Qwen2(nn.Module):
         if cache is None:
             cache = KVCache(self.cfg, B, S - 1, dtype=torch.bfloat16, device=self.device)
         ids = input_ids.to(self.device)
+        # workspaces are kept: one for all chunks, its sizes powers of two, so that texts of any length
+        # share a few
+        chunk = min(chunk, S - 1)
+        ws = self.workspace(*(1 << max(6, (n - 1).bit_length()) for n in (B * chunk, cache.max_len)))
         parts = []
         for lo in range(0, S - 1, chunk):
             hi = min(S - 1, lo + chunk)
-            logits = self.forward(input_ids[:, lo:hi], positions=torch.arange(lo, hi), cache=cache,
-                                  logits_dtype=torch.float32)
+            logits = self._forward(input_ids[:, lo:hi], torch.arange(lo, hi), cache, False, torch.float32, ws)
             r = token_logprobs(logits.reshape(B * (hi - lo), -1), ids[:, lo + 1:hi + 1].reshape(-1), top)
             parts.append([t if t is None else t.view(B, hi - lo, *t.shape[1:])
                           for t in (r.logprob, r.entropy, r.top_ids, r.top_logprobs)])
