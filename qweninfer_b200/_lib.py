@@ -174,7 +174,11 @@ class on_device:
             self.other.__enter__()
         # the library's current device is per thread, and other calls may have moved it
         if self.idx not in _inited or torch.cuda.device_count() > 1:
-            check(lib().qi_init(self.idx), "qi_init")
+            try:
+                check(lib().qi_init(self.idx), "qi_init")
+            except BaseException:
+                self.__exit__()  # (a context that is not entered is not left either)
+                raise
             _inited.add(self.idx)
             _current[0] = self.idx
 
