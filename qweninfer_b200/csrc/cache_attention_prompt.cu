@@ -296,7 +296,7 @@ __device__ __noinline__ float2 plain_row(const CacheAttnParams& p, const Seg& sg
         fv = 1.f;
         if constexpr (FMT != QI_KV_BF16) {
           const long long si = scale_index(p.c, sg.row, g, k0 + j);
-          fk = __ldg(p.c.k_scale + si), fv = __ldg(p.c.v_scale + si);
+          fk = __ldcg(p.c.k_scale + si), fv = __ldcg(p.c.v_scale + si);
         }
         for (int d = 0; d < D; ++d) s = fmaf(load_q(p, qo + d), value(p.c.k, at + d) * fk, s);
       }
@@ -626,7 +626,8 @@ __global__ void __launch_bounds__(Shape<FMT, D, QP>::kThreads, 1) prompt_kernel(
         if (lt < 16) {
           const int h0 = k0 + 16 * (lt & 7);
           const bool any = o >= 0 && list.sees16(h0);
-          sc = any ? __ldg((lt < 8 ? c.k_scale : c.v_scale) + scale_index(c, sg.row, g, h0)) : 1.f;
+          // (not a read-only load: this kernel may have been launched before the append wrote them)
+          sc = any ? __ldcg((lt < 8 ? c.k_scale : c.v_scale) + scale_index(c, sg.row, g, h0)) : 1.f;
         }
       }
     };
