@@ -897,7 +897,8 @@ __global__ void __launch_bounds__(Shape<FMT, D, QP>::kThreads, 1) prompt_kernel(
       oa = m == -INFINITY ? 1.f : ex2(m - mn);  // nothing summed yet: nothing to rescale
       l *= oa;
       m = mn;
-      const float mr = m == -INFINITY ? 0.f : m, Rr = R == -INFINITY ? 0.f : R;
+      // (a tile of which the row sees nothing: P is zero, and T's factor stays finite whatever the maximum is)
+      const float mr = m == -INFINITY ? 0.f : m, Rr = R == -INFINITY ? mr : R;
       // (one rounded exponent both ways: what P is raised by, T is lowered by)
       const float rest = mr - Rr + kLift;
       ob = ex2(-rest);

@@ -149,3 +149,40 @@ def test_half_precision_outputs_are_rounded_once(fmt, dim, tiles):
     out, _ = exact(q, *vals, 0, pos)
     own = float((out.to(torch.float16).double() - out).norm())
     assert float((got.double() - out).norm()) <= 1.05 * own + 2.0 ** -18 * float(out.norm())
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("low", [-60, -150, -1500])
+def test_scores_far_below_zero(fmt, heads, kv, dim, dtype, low):
+    """All scores of a row around `low`, in tiles of keys of which some rows see nothing: prompts of
+    several cache rows next to each other, and the first tokens of a prompt that runs on into the
+    next keys."""
+    from test_cache_ops_gpu import config
+    from qweninfer_b200.engine.kv_cache import Kv8Cache, KVCache
+    g, n = gen(53), 300
+    k = randn(g, 3, kv, n, dim) * 0.5 + low / math.sqrt(dim)
+    v = randn(g, 3, kv, n, dim)
+    if fmt == "bf16":
+        cache = KVCache(config(heads, kv, dim), 3, n, device="cuda")
+        cache.k[0].copy_(k)
+        cache.v[0].copy_(v)
+        k, v = cache.k[0], cache.v[0]
+    else:
+        cache = Kv8Cache(config(heads, kv, dim), 3, n, device="cuda", format=fmt)
+        for r in range(3):
+            cache.append(0, k[r].transpose(0, 1), v[r].transpose(0, 1), i32([r] * n), i32(range(n)))
+        k, v = cache.values(0)
+    runs = [(0, 110, 30), (2, 0, 3), (1, 250, 50), (0, 5, 9), (2, 120, 150)]  # row, first position, tokens
+    rows = [r for r, a, m in runs for _ in range(m)]
+    pos = [p for r, a, m in runs for p in range(a, a + m)]
+    q = (1 + 0.05 * randn(g, len(pos), heads, dim)).to(dtype)
+    bits = 11 if dtype == torch.bfloat16 else 22
+    for window, sinks in ((0, 0), (20, 2)):
+        got = cache.attend(0, q, i32(rows), i32(pos), window=window, sinks=sinks, query_run=150, tiles=True)
+        for r in range(3):
+            at = [i for i, x in enumerate(rows) if x == r]
+            out, tol = exact(q[at], k, v, r, [pos[i] for i in at], window, sinks, bits)
+            assert ((got[at].double() - out).abs() <= tol).all()
+    cache.check()
