@@ -14,14 +14,14 @@
 // as do the two tiles of a CTA, which share the keys that producer warps bring into the
 // K-major layout of UMMA descriptors as fp16. The widening costs about as much as a tile's
 // softmax: eight warps for bf16 values (4000 tokens, window 1024, head_dim 64: 119 us, with
-// four 130; 2048 tokens on 4000 keys of 128 dims: 377, with four 724), four for 8-bit codes,
-// whose registers the softmax warps use better (1024 tokens on 4096 keys: 54.4 us, with
-// eight 55.9). V in the same layout is the MN-major operand of the second product, so nothing
+// four 130; 2048 tokens on 4000 keys of 128 dims: 377, with four 724; the eight have become faster
+// since), four for 8-bit codes, whose registers the softmax warps use better (1024 tokens on 4096
+// keys: 54 us, with eight 56). V in the same layout is the MN-major operand of the second product, so nothing
 // is transposed. One warp issues the MMAs.
 //
 // Measured: 1024 tokens on 4096 keys, 14 heads on 2 of 64, int8, bf16 queries: 54 us, 0.15 of
 // the tensor cores' rate (8.1 us at the measured peak is the floor of 13.2 GFLOP); 4000 tokens
-// under a window of 1024 on bf16 keys, fp32 queries: 119 us (floor 7.9 us, each product is
+// under a window of 1024 on bf16 keys, fp32 queries: 111 us (floor 7.9 us, each product is
 // two). What bounds it is the softmax: a pair of tiles takes 5300 to 6400 cycles for 128
 // keys, of which the 64 exponentials of each of the 512 threads need 2048 of the one unit
 // that makes them; the two products need 1500 (3000 in two parts).
@@ -55,7 +55,8 @@
 // tile sees are zero-filled; but in P V a zero weight times a NaN or infinity that another
 // row does see would be NaN. A row that ends up not finite is therefore computed again, key
 // by key (8-bit codes are always finite: only the bf16 cache needs it), and so is one whose scores
-// are as far from 0 as kFarScore says.
+// are as far from 0 as kFarScore says. That costs milliseconds a row of some thousand keys; neither
+// comes up in a working model.
 #include <atomic>
 
 #include "cache_attention.cuh"
