@@ -340,11 +340,14 @@ class PagedKVCache(KVCache):
         that went back."""
         if not 0 <= row < self.max_batch or not 0 <= start <= length <= self.max_len:
             raise IndexError(f"row {row} / positions [{start}, {length}) outside the cache")
-        if start == 0 and self.trim_at[row]:
+        size, need = self.page_size, -(-length // self.page_size)
+        went_back = start < self.trim_at[row]  # pages from `start` on, or seen from there, may be gone
+        if not went_back and need <= self.mapped[row]:
+            return
+        if went_back and start == 0:
             self.release(row)
-        size, need, mapped = self.page_size, -(-length // self.page_size), int(self.mapped[row])
-        first = start // size
-        if start < self.trim_at[row]:  # pages seen from `start` on and not written (else all of them are there)
+        mapped, first = int(self.mapped[row]), start // size
+        if went_back and start:
             seen = ((0, -(-min(self.attn_sinks, start) // size)),
                     (max(0, start - self.attn_window + 1) // size, -(-start // size)))
             if any((self._t[row, a:min(b, mapped)] < 0).any() for a, b in seen):
