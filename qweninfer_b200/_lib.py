@@ -177,7 +177,7 @@ class on_device:
             try:
                 check(lib().qi_init(self.idx), "qi_init")
             except BaseException:
-                self.__exit__()  # (a context that is not entered is not left either)
+                self.__exit__(None, None, None)  # (a context that is not entered is not left either)
                 raise
             _inited.add(self.idx)
             _current[0] = self.idx

@@ -22,7 +22,7 @@ class Machine:
             def __enter__(self):
                 self.before, m.current = m.current, self.idx
 
-            def __exit__(self, *exc):
+            def __exit__(self, kind, value, trace):
                 m.current = self.before
 
         class Lib:

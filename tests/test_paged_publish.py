@@ -37,7 +37,7 @@ class Device:
             def __enter__(self):
                 pass
 
-            def __exit__(self, *exc):
+            def __exit__(self, kind, value, trace):
                 pass
 
         for name, f in (("Event", Event), ("current_stream", Stream), ("device", Guard),
