@@ -219,8 +219,8 @@ int qi_kv8_values(const qi_kv_layer* layer, float* k_out, float* v_out, qi_strea
  * Token t at position pos[t] of cache row rows[t] sees key j if 0 <= j <= pos[t] and
  * (window == 0 or j > pos[t] - window or j < sinks): a sliding window of `window` keys, its
  * own among them, and the row's first `sinks` keys. pos[t] = -1 (an idle slot) sees
- * nothing: its output is zero. Keys that are not seen are not read. q: dtype QI_F32/BF16/
- * F16, element strides of token and head, dims contiguous; heads = group * kv_heads, group
+ * nothing: its output is zero. What keys that a token does not see hold has no effect on it. q:
+ * dtype QI_F32/BF16/F16, element strides of token and head, dims contiguous; heads = group * kv_heads, group
  * 1..8. out: (M, heads, head_dim) of the same dtype, 16-byte aligned, must not overlap q. query_run: longest
  * run of consecutive tokens of one cache row (a prompt's length), 1 for a decode step, 0 if
  * unknown (at most QI_RUN_TILES - 1); it picks the kernel, any value gives the same result up to
